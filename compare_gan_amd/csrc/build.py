@@ -15,6 +15,8 @@ SOURCES = ["cg_error.hip", "cg_gconv.hip", "cg_conv_fast.hip", "cg_conv_halo.hip
            "cg_optim.hip", "cg_attn.hip", "cg_fid.hip", "cg_tridiag.hip", "cg_calib.hip", "cg_ln.hip", "cg_head.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
+         # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-I" + os.path.join(ROOT, "include"), "-I" + HERE]
 
 
