@@ -1,0 +1,1088 @@
+// Softmax attention with grouped heads over packed sequences, forward and backward (cgamd.h:
+// cg_packed_attention_*).  Per sequence and key head, with the G = heads / kv_heads query heads that share it:
+//
+//   S = scale Q K^T,  P = softmax(S) over the keys a row may see,  O = P V
+//   delta_i = sum_d dO_id O_id,  dS = P o (dO V^T - delta),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
+//
+// ROWS.  A "row" is one (query token, shared head) pair, r = token * G + head: all G heads of a key head
+// run through the same tiles, so K and V are staged once for all of them, a single new token fills G columns
+// of a matrix instruction instead of one, and the sum over shared heads that dK and dV need is part of the
+// contraction (no atomics, one fixed order).
+//
+// REGISTERS.  Everything is computed transposed with v_mfma_f32_32x32x16_bf16: S^T[key][row] = K Q^T puts one
+// row into a lane (16 keys of it a lane half), so the running maximum and sum of the softmax are per-lane
+// values plus one exchange between the halves, and P^T leaves the accumulator in the layout that the next
+// product's second operand has, up to a permutation of the 16 keys of a step:
+//   element e of lane half h  <->  key 16 ks + 4 h + (e & 3) + 8 (e >> 2)
+// which the first operand matches by reading V transposed (ds_read_b64_tr_b16) at those keys.  P, dS and
+// all the sums never touch LDS.  Statistics and accumulators are fp32; P and dS are rounded to bf16 on their
+// way into the matrix instruction (half a step of 2^-9 relative each, independent errors over the sum).
+//
+// LDS.  Tiles are copied by buffer_load ... lds (16 bytes a lane), two buffers: tile i + 1 is in flight while
+// tile i is multiplied, one barrier a tile.  Rows keep their pitch of 2 DP bytes; instead of padding, the
+// 16-byte chunks of a row are exchanged by an XOR with bits of the row number (mha_swz) so that both the
+// b128 reads of K (32 rows, one chunk) and the transposed reads of V (8 rows, 4 chunks) spread over all banks.
+// Rows behind the end of a sequence and columns behind D are outside the buffer descriptor and arrive as zeros.
+#include "cg_common.h"
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) short mha_s16x4_t;
+typedef __attribute__((address_space(3))) mha_s16x4_t* mha_tr_ptr;
+typedef __attribute__((address_space(3))) unsigned char* mha_lds_ptr;
+typedef __attribute__((address_space(3))) const bf16x8_t* mha_frag_ptr;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int KT = 64;           // keys of a tile (rows of a tile in the dK / dV kernel)
+constexpr int ROW_TILE = 128;    // rows of a forward / dQ work item: 4 waves of 32
+constexpr int KEY_TILE = 128;    // keys of a dK / dV work item: 4 waves of 32
+constexpr int THIN_ROWS = 32;    // rows of a thin work item: one wave's
+
+struct MhaArgs {
+  const bf16_t *q, *k, *v;
+  int64_t qt, qh, kt, kh, vt, vh;
+  const int4* seqs;         // {q_start, q_len, k_start, k_len}
+  const int4* items;        // two int4 an item
+  bf16_t* out;
+  float* lse;
+  float* ws_o;              // partial results, in units of 32 rows: [unit][32][Dv]
+  float* ws_ml;             //                                        [unit][32][2]
+  const bf16_t* o_in;
+  const bf16_t* dout;
+  const float* lse_in;
+  const float* delta;
+  bf16_t *dq, *dk, *dv;
+  int heads, G, kv_heads, D, Dv, causal;
+  float c, scale;           // scale * log2(e)
+  FastDiv dG;
+};
+
+struct MhaItem {
+  int seq, hk, row0, k0, k1, part, units;
+  int q_start, Lq, k_start, Lk, rows, shift;   // rows = Lq G; row of token t sees keys <= t + shift
+};
+
+__device__ __forceinline__ MhaItem mha_item(const MhaArgs& a, int index) {
+  const int4 x = a.items[2 * index], y = a.items[2 * index + 1];
+  MhaItem it;
+  it.seq = __builtin_amdgcn_readfirstlane(x.x);
+  it.hk = __builtin_amdgcn_readfirstlane(x.y);
+  it.row0 = __builtin_amdgcn_readfirstlane(x.z);
+  it.k0 = __builtin_amdgcn_readfirstlane(x.w);
+  it.k1 = __builtin_amdgcn_readfirstlane(y.x);
+  it.part = __builtin_amdgcn_readfirstlane(y.y);
+  it.units = __builtin_amdgcn_readfirstlane(y.z);
+  const int4 s = a.seqs[it.seq];
+  it.q_start = __builtin_amdgcn_readfirstlane(s.x);
+  it.Lq = __builtin_amdgcn_readfirstlane(s.y);
+  it.k_start = __builtin_amdgcn_readfirstlane(s.z);
+  it.Lk = __builtin_amdgcn_readfirstlane(s.w);
+  it.rows = it.Lq * a.G;
+  it.shift = a.causal ? it.Lk - it.Lq : 0x40000000;
+  return it;
+}
+
+// XOR applied to the chunk number of row r (pitch 2 DP bytes).  64 banks of 4 bytes = 256 bytes: rows whose
+// pitch is a multiple of that need the spread from the XOR alone (two low row bits move a 64-byte group,
+// the next two a chunk inside it); shorter pitches already rotate.
+template <int DP>
+__device__ __forceinline__ int mha_swz(int r) {
+  if constexpr (DP == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else if constexpr (DP == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  else return (r >> 2) & 3;    // DP = 32: pitch 64; DP = 96: pitch 192 (chunk ^ 0..3 stays inside 12)
+}
+
+// Copies ROWS rows of 2 DP bytes into LDS.  Chunk i (of ROWS * DP / 8) is lane i % 64 of copy i / 64;
+// copy c belongs to wave c % NW.
+template <int DP, int ROWS, int NW>
+struct MhaStage {
+  static constexpr int CH = DP / 8;
+  static constexpr int COPIES = ROWS * CH / 64;
+  static constexpr int N = COPIES / NW;
+  static_assert(COPIES % NW == 0, "copies per wave");
+  // row and column (elements) of this lane's chunk in copy n; column >= D: outside
+  static __device__ __forceinline__ void place(int n, int wave, int lane, int* row, int* col) {
+    const int i = (n * NW + wave) * 64 + lane;
+    const int r = i / CH, s = i - r * CH;
+    *row = r;
+    *col = (s ^ mha_swz<DP>(r)) * 8;
+  }
+};
+
+constexpr uint32_t OUTSIDE = 0x80000000u;
+
+// per-lane byte offsets of consecutive rows (keys): row * stride + column
+template <int DP, int ROWS, int NW, int N>
+__device__ __forceinline__ void mha_offsets(uint32_t (&off)[N], int wave, int lane,
+                                            int64_t stride, int D) {
+  static_assert(N == MhaStage<DP, ROWS, NW>::N, "one offset a copy");
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    int r, c;
+    MhaStage<DP, ROWS, NW>::place(n, wave, lane, &r, &c);
+    off[n] = c < D ? (uint32_t)(r * (uint32_t)(stride * 2) + c * 2) : OUTSIDE;
+  }
+}
+template <int DP, int ROWS, int NW, int N>
+__device__ __forceinline__ void mha_copy(const uint32_t (&off)[N], cg_i32x4_t rs,
+                                         uint32_t lds, int wave) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    cg_dma16_asm(rs, off[n], 0u, lds + (uint32_t)(n * NW + wave) * 1024u);
+}
+// descriptor of rows [row, row + ROWS) of a [.., stride] tensor that ends with row `end` (exclusive)
+template <int ROWS>
+__device__ __forceinline__ cg_i32x4_t mha_rows(const bf16_t* base, int64_t row, int left, int64_t stride, int D) {
+  const int n = left < ROWS ? left : ROWS;
+  return cg_make_rsrc(base + row * stride, n <= 0 ? 0u : (uint32_t)(n - 1) * (uint32_t)(stride * 2) + (uint32_t)D * 2u);
+}
+
+__device__ __forceinline__ bf16x8_t mha_tr2(mha_lds_ptr lo, mha_lds_ptr hi) {
+  const mha_s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mha_tr_ptr)lo);
+  const mha_s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mha_tr_ptr)hi);
+  const s16x8_t v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  return __builtin_bit_cast(bf16x8_t, v);
+}
+__device__ __forceinline__ bf16x8_t mha_pack(const f32x16_t& v, int at) {
+  const f32x8_t f = {v[at], v[at + 1], v[at + 2], v[at + 3], v[at + 4], v[at + 5], v[at + 6], v[at + 7]};
+  return __builtin_convertvector(f, bf16x8_t);
+}
+__device__ __forceinline__ f32x16_t mha_zero() {
+  f32x16_t z;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) z[v] = 0.f;
+  return z;
+}
+// one row's (or key's) operand fragments: columns kd * 16 + half * 8 + 0..7
+template <int KD>
+__device__ __forceinline__ void mha_row_frags(bf16x8_t (&f)[KD], const bf16_t* p, bool ok, int D, int half) {
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd) {
+    const int d = kd * 16 + half * 8;
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (ok && d < D) x = *reinterpret_cast<const uint4*>(p + d);
+    f[kd] = __builtin_bit_cast(bf16x8_t, x);
+  }
+}
+
+// LDS offsets of a lane's reads in a tile of 2 DP byte rows
+template <int DP>
+struct MhaReads {
+  uint32_t row[DP / 16];       // b128: row lane & 31, columns kd 16 + half 8 ..
+  uint32_t tr[DP / 32][2];     // b64 transposed: rows 4 half + 0..3 (+ 8), columns t 32 ..
+};
+template <int DP>
+__device__ __forceinline__ MhaReads<DP> mha_reads(int lane) {
+  MhaReads<DP> m;
+  const int col = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int kd = 0; kd < DP / 16; ++kd)
+    m.row[kd] = (uint32_t)(col * 2 * DP + (((kd * 2 + half) ^ mha_swz<DP>(col)) << 4));
+  const int l16 = lane & 15, tcol = ((lane >> 4) & 1) * 16 + (l16 & 3) * 4;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int r = 4 * half + 8 * p + (l16 >> 2), c = t * 32 + tcol;
+      m.tr[t][p] = (uint32_t)(r * 2 * DP + (((c >> 3) ^ mha_swz<DP>(r)) << 4) + (c & 7) * 2);
+    }
+  return m;
+}
+
+// S^T tile of 32 keys (rows `sub` of the LDS tile) and one wave's 32 rows
+template <int DP>
+__device__ __forceinline__ f32x16_t mha_product(mha_lds_ptr tile, const MhaReads<DP>& m,
+                                                const bf16x8_t (&f)[DP / 16], int sub) {
+  f32x16_t s = mha_zero();
+#pragma unroll
+  for (int kd = 0; kd < DP / 16; ++kd) {
+    const bf16x8_t x = *(mha_frag_ptr)(tile + m.row[kd] + sub * 64 * DP);
+    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, f[kd], s, 0, 0, 0);
+  }
+  return s;
+}
+// acc[t] += (tile^T)[t 32 .. +31][32 keys of sub] * p
+template <int DP>
+__device__ __forceinline__ void mha_accumulate(f32x16_t (&acc)[DP / 32], mha_lds_ptr tile, const MhaReads<DP>& m,
+                                               const f32x16_t& p, int sub) {
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    const bf16x8_t pf = mha_pack(p, 8 * ks);
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) {
+      const uint32_t at = (uint32_t)(sub * 64 * DP + ks * 32 * DP);
+      const bf16x8_t x = mha_tr2(tile + m.tr[t][0] + at, tile + m.tr[t][1] + at);
+      acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, pf, acc[t], 0, 0, 0);
+    }
+  }
+}
+__device__ __forceinline__ int mha_key(int v, int half) { return (v & 3) + 8 * (v >> 2) + 4 * half; }
+
+// Running softmax over the 64 (NS = 2) or 32 (NS = 1) keys of s: in s the scores, out the weights
+// 2^(c s - m).  m, the reference exponent, is only raised when a row's maximum has passed it by more than 8:
+// weights stay below 2^8 (the same relative rounding in bf16, no danger in the fp32 sums) and the rescaling
+// of the accumulators is skipped in nearly every tile.
+constexpr float RAISE = 8.f;
+template <int NS, int NT>
+__device__ __forceinline__ void mha_softmax(f32x16_t (&s)[NS], float c, float& m, float& l, f32x16_t (&o)[NT]) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < NS; ++n)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[n][v]);
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+  if (__any(mx > m + RAISE)) {      // (m = -inf: raised by the first finite maximum)
+    const float up = fmaxf(m, mx);
+    const float f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
+    m = up;
+    l *= f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[t][v] *= f;
+  }
+  const float ref = m == -INFINITY ? 0.f : m;     // nothing seen yet: the weights are 2^-inf = 0
+#pragma unroll
+  for (int n = 0; n < NS; ++n)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      s[n][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][v], c, -ref));
+      l += s[n][v];
+    }
+}
+
+// factor that brings a result with reference exponent m to the common one; m = -inf: nothing was seen
+// (its sums are 0, or NaN where a score was NaN, which has to stay)
+__device__ __forceinline__ float mha_weight(float m, float top) {
+  return m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+}
+
+// row r of the item's sequence: offset of its (token, head) in a [rows, heads] tensor, and its address
+__device__ __forceinline__ void mha_token(const MhaArgs& a, const MhaItem& it, int r, int* t, int* h) {
+  *t = (int)fdiv((uint32_t)r, a.dG);
+  *h = it.hk * a.G + (r - *t * a.G);
+}
+
+// what a wave leaves behind: O^T in registers -> out, or a partial result
+template <int DP>
+__device__ __forceinline__ void mha_store(const MhaArgs& a, const MhaItem& it, int r, float m, float l,
+                                          f32x16_t (&o)[DP / 32], int half) {
+  if (r >= it.rows) return;
+  if (it.part >= 0) {
+    const int64_t at = (int64_t)it.part * THIN_ROWS + (r - it.row0);
+    float* dst = a.ws_o + at * a.Dv;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = t * 32 + g * 8 + 4 * half;
+        if (d < a.Dv)
+          *reinterpret_cast<float4*>(dst + d) = make_float4(o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]);
+      }
+    if (half == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m, l);
+    return;
+  }
+  int t_, h;
+  mha_token(a, it, r, &t_, &h);
+  const int64_t row = (int64_t)(it.q_start + t_) * a.heads + h;
+  const float inv = l == 0.f ? 0.f : 1.f / l;       // a row that sees no key: 0
+  bf16_t* dst = a.out + row * a.Dv;
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = t * 32 + g * 8 + 4 * half;
+      if (d < a.Dv) {
+        const float w[4] = {o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv};
+        *reinterpret_cast<uint2*>(dst + d) = pack4_bf16(w);
+      }
+    }
+  if (a.lse && half == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * (1.f / LOG2E);
+}
+
+// ---- forward, 128 rows x all keys of the item ---------------------------------------------------
+template <int DP>
+__global__ __launch_bounds__(256, 2) void mha_fwd_kernel(MhaArgs a) {
+  constexpr int TILE = KT * DP * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const MhaItem it = mha_item(a, blockIdx.x);
+  const int r = it.row0 + wave * 32 + col;
+  int t, h;
+  mha_token(a, it, r, &t, &h);
+  const bool ok = r < it.rows;
+  bf16x8_t qf[DP / 16];
+  mha_row_frags(qf, a.q + (int64_t)(it.q_start + t) * a.qt + (int64_t)h * a.qh, ok, a.D, half);
+  // last key this row sees (exclusive end of the item's keys included)
+  const int last = ok ? min(it.k1 - 1, t + it.shift) : -1;
+  int least = last, most = last;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    least = min(least, __shfl_xor(least, s, 64));
+    most = max(most, __shfl_xor(most, s, 64));
+  }
+  least = __builtin_amdgcn_readfirstlane(least);
+  most = __builtin_amdgcn_readfirstlane(most);
+  using Stage = MhaStage<DP, KT, 4>;
+  uint32_t koff[Stage::N], voff[Stage::N];
+  mha_offsets<DP, KT, 4>(koff, wave, lane, a.kt, a.D);
+  mha_offsets<DP, KT, 4>(voff, wave, lane, a.vt, a.Dv);
+  const MhaReads<DP> rd = mha_reads<DP>(lane);
+  const bf16_t* kb = a.k + (int64_t)it.hk * a.kh;
+  const bf16_t* vb = a.v + (int64_t)it.hk * a.vh;
+  const uint32_t lds = cg_lds_addr(smem);
+  mha_lds_ptr sm = (mha_lds_ptr)smem;
+  auto stage = [&](int k0, int buf) {
+    mha_copy<DP, KT, 4>(koff, mha_rows<KT>(kb, it.k_start + k0, it.Lk - k0, a.kt, a.D), lds + buf * 2 * TILE, wave);
+    mha_copy<DP, KT, 4>(voff, mha_rows<KT>(vb, it.k_start + k0, it.Lk - k0, a.vt, a.Dv), lds + buf * 2 * TILE + TILE, wave);
+  };
+  f32x16_t o[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) o[i] = mha_zero();
+  float m = -INFINITY, l = 0.f;
+  if (it.k0 < it.k1) stage(it.k0, 0);
+  int buf = 0;
+  for (int k0 = it.k0; k0 < it.k1; k0 += KT, buf ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (k0 + KT < it.k1) stage(k0 + KT, buf ^ 1);
+    if (k0 > most) continue;
+    mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
+    f32x16_t s[2];
+    s[0] = mha_product<DP>(ks, rd, qf, 0);
+    s[1] = mha_product<DP>(ks, rd, qf, 1);
+    if (k0 + KT - 1 > least) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          s[n][v] = k0 + n * 32 + mha_key(v, half) <= last ? s[n][v] : -INFINITY;
+    }
+    mha_softmax<2, DP / 32>(s, a.c, m, l, o);
+    mha_accumulate<DP>(o, vs, rd, s[0], 0);
+    mha_accumulate<DP>(o, vs, rd, s[1], 1);
+  }
+  l += __shfl_xor(l, 32, 64);
+  mha_store<DP>(a, it, r, m, l, o, half);
+}
+
+// ---- forward, at most 32 rows: the keys split over the waves --------------------------------------
+// One wave holds all rows; each of the NW waves takes every NW-th step of 32 keys through an LDS ring of its
+// own (no barrier in the loop), and the waves' results are joined at the end.  Bound by reading K and V.
+template <int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
+  constexpr int TILE = 32 * DP * 2;              // one matrix, 32 keys
+  constexpr int RING = 2 * 2 * TILE;             // K and V, two buffers, a wave
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[NW * RING];
+  __shared__ float sm_m[NW][32], sm_l[NW][32];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const MhaItem it = mha_item(a, blockIdx.x);
+  int t, h;
+  mha_token(a, it, col, &t, &h);
+  const bool ok = col < it.rows;
+  bf16x8_t qf[DP / 16];
+  mha_row_frags(qf, a.q + (int64_t)(it.q_start + t) * a.qt + (int64_t)h * a.qh, ok, a.D, half);
+  const int last = ok ? min(it.k1 - 1, t + it.shift) : -1;
+  int least = last;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) least = min(least, __shfl_xor(least, s, 64));
+  if (it.rows < 32) {          // columns without a row need no mask of their own: nothing of them is kept
+    least = 0x7fffffff;
+    for (int s = 0; s < it.rows; ++s) least = min(least, __shfl(last, s, 64));
+  }
+  least = __builtin_amdgcn_readfirstlane(least);
+  using Stage = MhaStage<DP, 32, 1>;
+  uint32_t koff[Stage::N], voff[Stage::N];
+  mha_offsets<DP, 32, 1>(koff, 0, lane, a.kt, a.D);
+  mha_offsets<DP, 32, 1>(voff, 0, lane, a.vt, a.Dv);
+  const MhaReads<DP> rd = mha_reads<DP>(lane);
+  const bf16_t* kb = a.k + (int64_t)it.hk * a.kh;
+  const bf16_t* vb = a.v + (int64_t)it.hk * a.vh;
+  const uint32_t lds = cg_lds_addr(smem) + wave * RING;
+  mha_lds_ptr sm = (mha_lds_ptr)smem + wave * RING;
+  auto stage = [&](int k0, int buf) {
+    mha_copy<DP, 32, 1>(koff, mha_rows<32>(kb, it.k_start + k0, it.Lk - k0, a.kt, a.D), lds + buf * 2 * TILE, 0);
+    mha_copy<DP, 32, 1>(voff, mha_rows<32>(vb, it.k_start + k0, it.Lk - k0, a.vt, a.Dv), lds + buf * 2 * TILE + TILE, 0);
+  };
+  f32x16_t o[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) o[i] = mha_zero();
+  float m = -INFINITY, l = 0.f;
+  const int first = it.k0 + wave * 32;
+  constexpr int INFLIGHT = 2 * Stage::N;         // copies of one step
+  if (first < it.k1) stage(first, 0);
+  int buf = 0;
+  for (int k0 = first; k0 < it.k1; k0 += NW * 32, buf ^= 1) {
+    // the other buffer was read in the last step: those reads have returned (their values were used)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (k0 + NW * 32 < it.k1) {
+      stage(k0 + NW * 32, buf ^ 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(INFLIGHT) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
+    f32x16_t s[1];
+    s[0] = mha_product<DP>(ks, rd, qf, 0);
+    if (k0 + 31 > least) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[0][v] = k0 + mha_key(v, half) <= last ? s[0][v] : -INFINITY;
+    }
+    mha_softmax<1, DP / 32>(s, a.c, m, l, o);
+    mha_accumulate<DP>(o, vs, rd, s[0], 0);
+  }
+  l += __shfl_xor(l, 32, 64);
+  if constexpr (NW > 1) {
+    if (half == 0) {
+      sm_m[wave][col] = m;
+      sm_l[wave][col] = l;
+    }
+    __syncthreads();                             // every wave is done with its ring, too
+    float top = sm_m[0][col];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) top = fmaxf(top, sm_m[w][col]);
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) total += sm_l[w][col] * mha_weight(sm_m[w][col], top);
+    const float mine = mha_weight(m, top);
+    // joined two waves at a time in a fixed order: wave w hands its scaled O to wave w - step
+    float* box = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[i][v] *= mine;
+#pragma unroll
+    for (int step = NW / 2; step > 0; step >>= 1) {
+      if (wave >= step && wave < 2 * step) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) box[((wave - step) * (DP / 32) * 16 + i * 16 + v) * 64 + lane] = o[i][v];
+      }
+      __syncthreads();
+      if (wave < step) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[i][v] += box[(wave * (DP / 32) * 16 + i * 16 + v) * 64 + lane];
+      }
+      __syncthreads();
+    }
+    if (wave != 0) return;
+    m = top;
+    l = total;
+  }
+  mha_store<DP>(a, it, col, m, l, o, half);
+}
+
+// ---- joins the partial results of a split item; one wave a row --------------------------------------
+// item {seq, hk, row0, rows here, parts, first unit, units a part}
+__global__ __launch_bounds__(256) void mha_join_kernel(MhaArgs a) {
+  const MhaItem it = mha_item(a, blockIdx.x);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int parts = it.k1;
+  const int64_t step = (int64_t)it.units * THIN_ROWS;
+  for (int i = blockIdx.y * 4 + wave; i < it.k0; i += gridDim.y * 4) {
+    const int64_t at = (int64_t)it.part * THIN_ROWS + i;
+    float top = -INFINITY;
+    for (int p = 0; p < parts; ++p) top = fmaxf(top, a.ws_ml[(at + p * step) * 2]);
+    float total = 0.f, acc[2] = {0.f, 0.f};
+    for (int p = 0; p < parts; ++p) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + (at + p * step) * 2);
+      const float w = mha_weight(ml.x, top);
+      total += ml.y * w;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (lane + 64 * j < a.Dv) acc[j] += a.ws_o[(at + p * step) * a.Dv + lane + 64 * j] * w;
+    }
+    int t, h;
+    mha_token(a, it, it.row0 + i, &t, &h);
+    const int64_t row = (int64_t)(it.q_start + t) * a.heads + h;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (lane + 64 * j < a.Dv) a.out[row * a.Dv + lane + 64 * j] = f2bf(acc[j] * inv);
+    if (a.lse && lane == 0)
+      a.lse[row] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * (1.f / LOG2E);
+  }
+}
+
+// ---- backward -----------------------------------------------------------------------------------
+// delta[row] = sum_d dout out; 16 lanes a row, 8 elements each
+__global__ __launch_bounds__(256) void mha_delta_kernel(const bf16_t* __restrict__ out,
+                                                        const bf16_t* __restrict__ dout, int64_t rows, int Dv,
+                                                        float* __restrict__ delta) {
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int d = (threadIdx.x & 15) * 8;
+  float s = 0.f;
+  if (row < rows && d < Dv) {
+    float x[8], y[8];
+    unpack8_bf16(*reinterpret_cast<const uint4*>(out + row * Dv + d), x);
+    unpack8_bf16(*reinterpret_cast<const uint4*>(dout + row * Dv + d), y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += x[j] * y[j];
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (row < rows && (threadIdx.x & 15) == 0) delta[row] = s;
+}
+
+// what the weights are rebuilt from, in exponents of two; a row that saw no key: +inf (weights 0)
+__device__ __forceinline__ float mha_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }
+
+// dQ: 128 rows x all keys; S^T and dP^T = V dO^T side by side, dQ^T += K^T dS^T
+template <int DP>
+__global__ __launch_bounds__(256, 2) void mha_bwd_q_kernel(MhaArgs a) {
+  constexpr int TILE = KT * DP * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const MhaItem it = mha_item(a, blockIdx.x);
+  const int r = it.row0 + wave * 32 + col;
+  int t, h;
+  mha_token(a, it, r, &t, &h);
+  const bool ok = r < it.rows;
+  const int64_t row = (int64_t)(it.q_start + t) * a.heads + h;
+  bf16x8_t qf[DP / 16], df[DP / 16];
+  mha_row_frags(qf, a.q + (int64_t)(it.q_start + t) * a.qt + (int64_t)h * a.qh, ok, a.D, half);
+  mha_row_frags(df, a.dout + row * a.Dv, ok, a.Dv, half);
+  const float lse2 = ok ? mha_lse2(a.lse_in[row]) : INFINITY;
+  const float delta = ok ? a.delta[row] : 0.f;
+  const int last = ok ? min(it.k1 - 1, t + it.shift) : -1;
+  int least = last, most = last;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    least = min(least, __shfl_xor(least, s, 64));
+    most = max(most, __shfl_xor(most, s, 64));
+  }
+  least = __builtin_amdgcn_readfirstlane(least);
+  most = __builtin_amdgcn_readfirstlane(most);
+  using Stage = MhaStage<DP, KT, 4>;
+  uint32_t koff[Stage::N], voff[Stage::N];
+  mha_offsets<DP, KT, 4>(koff, wave, lane, a.kt, a.D);
+  mha_offsets<DP, KT, 4>(voff, wave, lane, a.vt, a.Dv);
+  const MhaReads<DP> rd = mha_reads<DP>(lane);
+  const bf16_t* kb = a.k + (int64_t)it.hk * a.kh;
+  const bf16_t* vb = a.v + (int64_t)it.hk * a.vh;
+  const uint32_t lds = cg_lds_addr(smem);
+  mha_lds_ptr sm = (mha_lds_ptr)smem;
+  auto stage = [&](int k0, int buf) {
+    mha_copy<DP, KT, 4>(koff, mha_rows<KT>(kb, it.k_start + k0, it.Lk - k0, a.kt, a.D), lds + buf * 2 * TILE, wave);
+    mha_copy<DP, KT, 4>(voff, mha_rows<KT>(vb, it.k_start + k0, it.Lk - k0, a.vt, a.Dv), lds + buf * 2 * TILE + TILE, wave);
+  };
+  f32x16_t dq[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) dq[i] = mha_zero();
+  if (it.k0 < it.k1) stage(it.k0, 0);
+  int buf = 0;
+  for (int k0 = it.k0; k0 < it.k1; k0 += KT, buf ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (k0 + KT < it.k1) stage(k0 + KT, buf ^ 1);
+    if (k0 > most) continue;
+    mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      f32x16_t s = mha_product<DP>(ks, rd, qf, n);
+      const f32x16_t dp = mha_product<DP>(vs, rd, df, n);
+      const bool masked = k0 + n * 32 + 31 > least;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c, -lse2));
+        p *= dp[v] - delta;
+        if (masked) p = k0 + n * 32 + mha_key(v, half) <= last ? p : 0.f;
+        s[v] = p;
+      }
+      mha_accumulate<DP>(dq, ks, rd, s, n);
+    }
+  }
+  if (!ok) return;
+  bf16_t* dst = a.dq + row * a.D;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = i * 32 + g * 8 + 4 * half;
+      if (d < a.D) {
+        const float w[4] = {dq[i][4 * g] * a.scale, dq[i][4 * g + 1] * a.scale, dq[i][4 * g + 2] * a.scale, dq[i][4 * g + 3] * a.scale};
+        *reinterpret_cast<uint2*>(dst + d) = pack4_bf16(w);
+      }
+    }
+}
+
+// dK, dV: 128 keys x the rows that see them.  S[row][key] = Q K^T and dP = dO V^T with the keys in the lanes'
+// columns; dV^T += dO^T P, dK^T += Q^T dS.  Item {seq, hk, key0, first row, end row}.
+template <int DP>
+__global__ __launch_bounds__(256, 1) void mha_bwd_kv_kernel(MhaArgs a) {
+  constexpr int TILE = KT * DP * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][KT];   // [buffer][lse, delta][row]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const MhaItem it = mha_item(a, blockIdx.x);
+  const int key = it.row0 + wave * 32 + col;
+  const bool ok = key < it.Lk;
+  bf16x8_t kf[DP / 16], vf[DP / 16];
+  mha_row_frags(kf, a.k + (int64_t)(it.k_start + key) * a.kt + (int64_t)it.hk * a.kh, ok, a.D, half);
+  mha_row_frags(vf, a.v + (int64_t)(it.k_start + key) * a.vt + (int64_t)it.hk * a.vh, ok, a.Dv, half);
+  // first row that sees this key; rows of the wave's first and last key for skipping and masking
+  auto first_row = [&](int k) { return a.causal ? max(0, k - it.shift) * a.G : 0; };
+  const int mine = first_row(key);
+  const int wave_first = first_row(it.row0 + wave * 32), wave_all = first_row(it.row0 + wave * 32 + 31);
+  const bool some = it.row0 + wave * 32 < it.Lk;
+  const int rb = it.k0, re = it.k1;
+  using Stage = MhaStage<DP, KT, 4>;
+  const MhaReads<DP> rd = mha_reads<DP>(lane);
+  const bf16_t* qb = a.q + (int64_t)it.hk * a.G * a.qh;
+  const bf16_t* db = a.dout + (int64_t)it.hk * a.G * a.Dv;
+  const uint32_t lds = cg_lds_addr(smem);
+  mha_lds_ptr sm = (mha_lds_ptr)smem;
+  const int64_t dt = (int64_t)a.heads * a.Dv;
+  auto stage = [&](int r0, int buf) {
+    // rows r0 .. r0 + 63 gathered by (token, head) relative to the first one's token
+    const int t0 = __builtin_amdgcn_readfirstlane((int)fdiv((uint32_t)r0, a.dG));
+    const cg_i32x4_t qr = cg_make_rsrc(qb + (int64_t)(it.q_start + t0) * a.qt, 0x7fffffffu);
+    const cg_i32x4_t dr = cg_make_rsrc(db + (int64_t)(it.q_start + t0) * dt, 0x7fffffffu);
+#pragma unroll
+    for (int n = 0; n < Stage::N; ++n) {
+      int i, c;
+      Stage::place(n, wave, lane, &i, &c);
+      const int r = r0 + i;
+      const int t = (int)fdiv((uint32_t)r, a.dG), g = r - t * a.G;
+      const bool in = r < re;
+      const uint32_t at = lds + buf * 2 * TILE + (uint32_t)(n * 4 + wave) * 1024u;
+      cg_dma16_asm(qr, in && c < a.D ? (uint32_t)(t - t0) * (uint32_t)(a.qt * 2) + (uint32_t)g * (uint32_t)(a.qh * 2) + c * 2 : OUTSIDE, 0u, at);
+      cg_dma16_asm(dr, in && c < a.Dv ? (uint32_t)(t - t0) * (uint32_t)(dt * 2) + (uint32_t)g * (uint32_t)(a.Dv * 2) + c * 2 : OUTSIDE, 0u, at + TILE);
+    }
+  };
+  f32x16_t dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) {
+    dk[i] = mha_zero();
+    dv[i] = mha_zero();
+  }
+
+  // wave 0 / 1 carry the statistics of the next tile: one row a lane
+  auto stat_load = [&](int r0) {
+    const int r = r0 + lane;
+    if (wave > 1) return 0.f;
+    if (r >= re) return wave == 0 ? INFINITY : 0.f;
+    const int t = (int)fdiv((uint32_t)r, a.dG), g = r - t * a.G;
+    const int64_t row = (int64_t)(it.q_start + t) * a.heads + it.hk * a.G + g;
+    return wave == 0 ? mha_lse2(a.lse_in[row]) : a.delta[row];
+  };
+  float next = 0.f;
+  if (rb < re) {
+    next = stat_load(rb);
+    stage(rb, 0);
+  }
+  int buf = 0;
+  for (int r0 = rb; r0 < re; r0 += KT, buf ^= 1) {
+    if (wave < 2) stat[buf][wave][lane] = next;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (r0 + KT < re) {
+      next = stat_load(r0 + KT);
+      stage(r0 + KT, buf ^ 1);
+    }
+    if (!some) continue;
+    mha_lds_ptr qs = sm + buf * 2 * TILE, ds = qs + TILE;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int rs = r0 + n * 32;
+      if (rs + 31 < wave_first || rs >= re) continue;
+      f32x16_t s = mha_product<DP>(qs, rd, kf, n);
+      f32x16_t dp = mha_product<DP>(ds, rd, vf, n);
+      const bool masked = rs < wave_all;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 ls = *reinterpret_cast<const float4*>(&stat[buf][0][n * 32 + 8 * g + 4 * half]);
+        const float4 de = *reinterpret_cast<const float4*>(&stat[buf][1][n * 32 + 8 * g + 4 * half]);
+        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dev[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int v = 4 * g + j;
+          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c, -lsv[j]));
+          float x = p * (dp[v] - dev[j]);
+          if (masked) {
+            const bool see = rs + mha_key(v, half) >= mine;
+            p = see ? p : 0.f;
+            x = see ? x : 0.f;
+          }
+          s[v] = p;
+          dp[v] = x;
+        }
+      }
+      mha_accumulate<DP>(dv, ds, rd, s, n);
+      mha_accumulate<DP>(dk, qs, rd, dp, n);
+    }
+  }
+  if (!ok) return;
+  bf16_t* dkp = a.dk + ((int64_t)(it.k_start + key) * a.kv_heads + it.hk) * a.D;
+  bf16_t* dvp = a.dv + ((int64_t)(it.k_start + key) * a.kv_heads + it.hk) * a.Dv;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = i * 32 + g * 8 + 4 * half;
+      const float w[4] = {dk[i][4 * g] * a.scale, dk[i][4 * g + 1] * a.scale, dk[i][4 * g + 2] * a.scale, dk[i][4 * g + 3] * a.scale};
+      const float u[4] = {dv[i][4 * g], dv[i][4 * g + 1], dv[i][4 * g + 2], dv[i][4 * g + 3]};
+      if (d < a.D) *reinterpret_cast<uint2*>(dkp + d) = pack4_bf16(w);
+      if (d < a.Dv) *reinterpret_cast<uint2*>(dvp + d) = pack4_bf16(u);
+    }
+}
+
+// ---- the plan ------------------------------------------------------------------------------------
+struct Work {
+  int32_t v[8];
+  int64_t cost;
+  int32_t unit;      // (sequence, key head): what shares K and V
+};
+
+// Longest first, and the tiles of one unit on one XCD (blocks go to the XCDs in turn) so that its keys stay in
+// that XCD's L2: units are given to the least loaded XCD, with fewer units than XCDs each has several of them.
+void mha_deal(std::vector<Work>* items, int units) {
+  constexpr int X = 8;
+  std::vector<Work>& w = *items;
+  if (w.empty()) return;
+  std::vector<int64_t> unit_cost(units, 0);
+  for (const Work& i : w) unit_cost[i.unit] += i.cost;
+  std::vector<int32_t> order(units);
+  for (int u = 0; u < units; ++u) order[u] = u;
+  std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return unit_cost[a] > unit_cost[b]; });
+  int live = 0;
+  while (live < units && unit_cost[order[live]] > 0) ++live;
+  if (live == 0) live = units;
+  std::vector<int32_t> first(units, 0), count(units, 1), next(units, 0);
+  if (live >= X) {
+    int64_t load[X] = {0};
+    for (int i = 0; i < units; ++i) {
+      int best = 0;
+      for (int x = 1; x < X; ++x)
+        if (load[x] < load[best]) best = x;
+      first[order[i]] = best;
+      load[best] += unit_cost[order[i]] + 1;
+    }
+  } else {
+    for (int i = 0; i < units; ++i) {
+      first[order[i]] = i % live;
+      count[order[i]] = (X - 1 - i % live) / live + 1;     // XCDs first, first + live, ...
+    }
+  }
+  std::stable_sort(w.begin(), w.end(), [](const Work& a, const Work& b) { return a.cost > b.cost; });
+  std::vector<Work> queue[X];
+  for (const Work& i : w) {
+    const int u = i.unit;
+    queue[live >= X ? first[u] : first[u] + live * (next[u]++ % count[u])].push_back(i);
+  }
+  size_t at[X] = {0};
+  for (size_t n = 0; n < w.size(); ++n) {
+    int x = (int)(n % X);
+    if (at[x] >= queue[x].size()) {            // an empty one helps where most is left
+      for (int y = 0; y < X; ++y)
+        if (queue[y].size() - at[y] > queue[x].size() - at[x]) x = y;
+    }
+    w[n] = queue[x][at[x]++];
+  }
+}
+
+// Blocks that a launch should have at least: 2 resident a CU, 256 CUs.  A launch with fewer is split over the
+// keys, in parts of no less than SPLIT_MIN keys (a part costs its fp32 result: written and read once).
+constexpr int64_t TILE_BLOCKS = 512, THIN_BLOCKS = 1024;
+constexpr int SPLIT_MIN = 256, THIN_SPLIT_MIN = 512;
+constexpr int THIN1_KEYS = 128;     // up to so many keys one wave does a thin item alone
+
+void mha_split(std::vector<Work>* items, int64_t blocks, int step, int least, int units_a_part, int G,
+               const int32_t* q_len, std::vector<Work>* joins, int64_t* parts) {
+  int64_t all = 0;
+  for (const Work& w : *items) all += (w.v[4] + step - 1) / step;
+  if ((int64_t)items->size() >= blocks || all == 0) return;
+  const int64_t chunk = std::max<int64_t>(least / step, (all + blocks - 1) / blocks);
+  std::vector<Work> out;
+  for (Work& w : *items) {
+    const int64_t steps = (w.v[4] + step - 1) / step;
+    const int64_t n = (steps + chunk - 1) / chunk;
+    if (n <= 1) {
+      out.push_back(w);
+      continue;
+    }
+    Work j = w;
+    j.v[3] = (int32_t)std::min<int64_t>((int64_t)32 * units_a_part, (int64_t)q_len[w.v[0]] * G - w.v[2]);
+    j.v[5] = (int32_t)*parts;
+    j.v[6] = units_a_part;
+    const int32_t end = w.v[4];
+    int32_t made = 0;
+    for (int64_t i = 0; i < n; ++i) {
+      Work p = w;
+      p.v[3] = (int32_t)(steps * i / n) * step;
+      p.v[4] = (int32_t)std::min<int64_t>(end, steps * (i + 1) / n * step);
+      p.v[5] = (int32_t)*parts;
+      p.cost = p.v[4] - p.v[3] + 64;
+      *parts += units_a_part;
+      out.push_back(p);
+      ++made;
+    }
+    j.v[4] = made;
+    joins->push_back(j);
+  }
+  items->swap(out);
+}
+
+int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start, const int32_t* k_len,
+             int B, int heads, int kv_heads, int causal, int32_t* data, int64_t capacity, cgAttentionPlan* info) {
+  const int G = heads / kv_heads;
+  std::vector<Work> tiles, thin4, thin1, joins, dq, dkv;
+  cgAttentionPlan p = {};
+  for (int b = 0; b < B; ++b) {
+    const int64_t Lq = q_len[b], Lk = k_len[b], rows = Lq * G, shift = Lk - Lq;
+    if (Lq > 0) p.max_q_row = std::max<int32_t>(p.max_q_row, (int32_t)(q_start[b] + Lq));
+    if (Lk > 0) p.max_k_row = std::max<int32_t>(p.max_k_row, (int32_t)(k_start[b] + Lk));
+    auto keys_of = [&](int64_t end_row) {     // keys that the rows below end_row see
+      if (!causal) return Lk;
+      return std::min(Lk, std::max<int64_t>(0, (end_row - 1) / G + shift + 1));
+    };
+    for (int h = 0; h < kv_heads; ++h) {
+      const int32_t unit = b * kv_heads + h;
+      for (int64_t r = 0; r < rows; r += ROW_TILE) {
+        const int64_t keys = keys_of(std::min(rows, r + ROW_TILE));
+        Work w = {{b, h, (int32_t)r, 0, (int32_t)keys, -1, 0, 0}, keys + 64, unit};
+        dq.push_back(w);
+        if (rows > THIN_ROWS) tiles.push_back(w);
+        else (keys <= THIN1_KEYS ? thin1 : thin4).push_back(w);
+      }
+      for (int64_t k = 0; k < Lk; k += KEY_TILE) {
+        const int64_t from = causal ? std::min(rows, std::max<int64_t>(0, k - shift) * G) : 0;
+        dkv.push_back(Work{{b, h, (int32_t)k, (int32_t)from, (int32_t)rows, -1, 0, 0}, rows - from + 64, unit});
+      }
+    }
+  }
+  int64_t parts = 0;
+  mha_split(&tiles, TILE_BLOCKS, KT, SPLIT_MIN, ROW_TILE / 32, G, q_len, &joins, &parts);
+  mha_split(&thin4, THIN_BLOCKS, 32, THIN_SPLIT_MIN, 1, G, q_len, &joins, &parts);
+  if (parts > 0x7fffffff) CG_FAIL(CG_ERR_UNSUPPORTED, "cg_host_attention_plan: too many partial results");
+  const int units = B * kv_heads;
+  std::vector<Work>* lists[6] = {&tiles, &thin4, &thin1, &joins, &dq, &dkv};
+  int64_t ints = 4 * (int64_t)B;
+  for (auto* l : lists) ints += 8 * (int64_t)l->size();
+  if (ints > 0x7fffffff) CG_FAIL(CG_ERR_UNSUPPORTED, "cg_host_attention_plan: too many work items");
+  p.ints = ints;
+  p.parts = parts;
+  p.sequences = B;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.causal = causal ? 1 : 0;
+  p.tiles = (int32_t)tiles.size();
+  p.thin4 = (int32_t)thin4.size();
+  p.thin1 = (int32_t)thin1.size();
+  p.joins = (int32_t)joins.size();
+  p.dq_tiles = (int32_t)dq.size();
+  p.dkv_tiles = (int32_t)dkv.size();
+  *info = p;
+  if (!data) return CG_OK;
+  if (capacity < ints) CG_FAIL(CG_ERR_WORKSPACE, "cg_host_attention_plan: %lld ints of %lld", (long long)capacity, (long long)ints);
+  for (int b = 0; b < B; ++b) {
+    const int32_t s[4] = {q_start[b], q_len[b], k_start[b], k_len[b]};
+    memcpy(data + 4 * (int64_t)b, s, sizeof(s));
+  }
+  int32_t* at = data + 4 * (int64_t)B;
+  for (auto* l : lists) {
+    if (l != &joins) mha_deal(l, units);
+    for (const Work& w : *l) {
+      memcpy(at, w.v, sizeof(w.v));
+      at += 8;
+    }
+  }
+  return CG_OK;
+}
+
+int mha_check(const char* name, const cgAttentionInput* in, const cgAttentionPlan* p, const int32_t* data, MhaArgs* a) {
+  if (!in || !p || !data) CG_FAIL(CG_ERR_BAD_ARG, "%s: null input or plan", name);
+  if (p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->ints < 1)
+    CG_FAIL(CG_ERR_BAD_ARG, "%s: not a plan of cg_host_attention_plan", name);
+  if (in->D < 8 || in->D > 128 || in->D % 8 || in->Dv < 8 || in->Dv > 128 || in->Dv % 8)
+    CG_FAIL(CG_ERR_UNSUPPORTED, "%s: head widths %d and %d (multiples of 8, at most 128)", name, in->D, in->Dv);
+  if (!(in->scale > 0.f) || in->scale > 3.0e38f) CG_FAIL(CG_ERR_BAD_ARG, "%s: scale has to be positive and finite", name);
+  if (in->q_rows < p->max_q_row || in->k_rows < p->max_k_row)
+    CG_FAIL(CG_ERR_BAD_ARG, "%s: %d query and %d key rows, the plan's sequences need %d and %d", name, in->q_rows,
+            in->k_rows, p->max_q_row, p->max_k_row);
+  const int64_t G = p->heads / p->kv_heads;
+  const int64_t st[6] = {in->q_stride_t, in->q_stride_h, in->k_stride_t, in->k_stride_h, in->v_stride_t, in->v_stride_h};
+  for (int i = 0; i < 6; ++i)
+    if (st[i] < 0 || st[i] % 8) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: strides have to be multiples of 8 elements", name);
+  const void* ptr[3] = {in->q, in->k, in->v};
+  for (int i = 0; i < 3; ++i) {
+    // (no keys at all: K and V may be null, no work item reads them)
+    if (!ptr[i] && (i == 0 ? p->max_q_row : p->max_k_row) > 0) CG_FAIL(CG_ERR_BAD_ARG, "%s: null tensor", name);
+    if ((uintptr_t)ptr[i] % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: tensors have to be 16-byte aligned", name);
+  }
+  // a tile's byte offsets are 32-bit (its base is 64-bit): 64 rows, and the shared heads of one
+  if ((int64_t)KT * 2 * std::max(std::max(st[0], st[2]), st[4]) + 2 * G * st[1] >= 0x7fffff00ll ||
+      (int64_t)KT * 2 * p->heads * 128 >= 0x3fffff00ll)
+    CG_FAIL(CG_ERR_UNSUPPORTED, "%s: strides too large", name);
+  a->q = (const bf16_t*)in->q;
+  a->k = (const bf16_t*)in->k;
+  a->v = (const bf16_t*)in->v;
+  a->qt = st[0]; a->qh = st[1]; a->kt = st[2]; a->kh = st[3]; a->vt = st[4]; a->vh = st[5];
+  a->seqs = (const int4*)data;
+  a->heads = p->heads;
+  a->kv_heads = p->kv_heads;
+  a->G = (int)G;
+  a->dG = make_fastdiv((uint32_t)G);
+  a->D = in->D;
+  a->Dv = in->Dv;
+  a->causal = p->causal;
+  a->scale = in->scale;
+  a->c = in->scale * LOG2E;
+  return CG_OK;
+}
+
+// item lists behind the sequences
+const int4* mha_list(const cgAttentionPlan* p, const int32_t* data, int which) {
+  const int64_t n[6] = {p->tiles, p->thin4, p->thin1, p->joins, p->dq_tiles, p->dkv_tiles};
+  int64_t at = 4 * (int64_t)p->sequences;
+  for (int i = 0; i < which; ++i) at += 8 * n[i];
+  return (const int4*)(data + at);
+}
+
+// padded head width: both matrices of a tile have it
+int mha_width(int D, int Dv) { return ((D > Dv ? D : Dv) + 31) / 32 * 32; }
+
+}  // namespace
+
+#define MHA_LAUNCH(dp, kernel, grid, block, st, args)                          \
+  switch (dp) {                                                                \
+    case 32: kernel(32)<<<grid, block, 0, st>>>(args); break;                  \
+    case 64: kernel(64)<<<grid, block, 0, st>>>(args); break;                  \
+    case 96: kernel(96)<<<grid, block, 0, st>>>(args); break;                  \
+    default: kernel(128)<<<grid, block, 0, st>>>(args); break;                 \
+  }
+#define MHA_FWD(dp) mha_fwd_kernel<dp>
+#define MHA_THIN4(dp) mha_thin_kernel<dp, 4>
+#define MHA_THIN1(dp) mha_thin_kernel<dp, 1>
+#define MHA_BWD_Q(dp) mha_bwd_q_kernel<dp>
+#define MHA_BWD_KV(dp) mha_bwd_kv_kernel<dp>
+
+extern "C" int cg_host_attention_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start,
+                                      const int32_t* k_len, int sequences, int heads, int kv_heads, int causal,
+                                      int32_t* data_host, int64_t capacity, cgAttentionPlan* info) {
+  const char* name = "cg_host_attention_plan";
+  if (!q_start || !q_len || !k_start || !k_len || !info) CG_FAIL(CG_ERR_BAD_ARG, "%s: null argument", name);
+  if (sequences < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 4096)
+    CG_FAIL(CG_ERR_BAD_ARG, "%s: %d sequences, %d heads over %d", name, sequences, heads, kv_heads);
+  const int64_t G = heads / kv_heads;
+  if ((int64_t)sequences * kv_heads > 0x3fffffff) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: too many sequences", name);
+  for (int b = 0; b < sequences; ++b) {
+    if (q_start[b] < 0 || q_len[b] < 0 || k_start[b] < 0 || k_len[b] < 0)
+      CG_FAIL(CG_ERR_BAD_ARG, "%s: sequence %d has a negative start or length", name, b);
+    if ((int64_t)q_len[b] * G > 0x3fffffff || (int64_t)q_start[b] + q_len[b] > 0x3fffffff ||
+        (int64_t)k_start[b] + k_len[b] > 0x3fffffff)
+      CG_FAIL(CG_ERR_UNSUPPORTED, "%s: sequence %d is too long", name, b);
+  }
+  try {
+    return mha_plan(q_start, q_len, k_start, k_len, sequences, heads, kv_heads, causal, data_host, capacity, info);
+  } catch (const std::bad_alloc&) {
+    CG_FAIL(CG_ERR_WORKSPACE, "%s: out of host memory", name);
+  } catch (...) {
+    CG_FAIL(CG_ERR_BAD_ARG, "%s: failed", name);
+  }
+}
+
+extern "C" size_t cg_packed_attention_fwd_workspace_bytes(const cgAttentionPlan* plan, int Dv) {
+  if (!plan || Dv < 1) return 0;
+  return (size_t)plan->parts * THIN_ROWS * ((size_t)Dv + 2) * sizeof(float);
+}
+
+extern "C" int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAttentionPlan* plan, const int32_t* data,
+                                       void* out, float* lse, void* ws, size_t ws_bytes, cgStream stream) {
+  const char* name = "cg_packed_attention_fwd";
+  MhaArgs a = {};
+  const int rc = mha_check(name, in, plan, data, &a);
+  if (rc) return rc;
+  if (plan->max_q_row == 0) return CG_OK;
+  if (!out) CG_FAIL(CG_ERR_BAD_ARG, "%s: null output", name);
+  if ((uintptr_t)out % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: tensors have to be 16-byte aligned", name);
+  if (plan->parts > 0 && (!ws || ws_bytes < cg_packed_attention_fwd_workspace_bytes(plan, in->Dv)))
+    CG_FAIL(CG_ERR_WORKSPACE, "%s: workspace of %zu bytes", name, ws_bytes);
+  a.out = (bf16_t*)out;
+  a.lse = lse;
+  a.ws_o = (float*)ws;
+  a.ws_ml = a.ws_o + plan->parts * THIN_ROWS * (int64_t)in->Dv;
+  const hipStream_t st = (hipStream_t)stream;
+  const int dp = mha_width(in->D, in->Dv);
+  if (plan->tiles) {
+    a.items = mha_list(plan, data, 0);
+    MHA_LAUNCH(dp, MHA_FWD, plan->tiles, 256, st, a);
+    CG_CHECK_LAUNCH(name);
+  }
+  if (plan->thin4) {
+    a.items = mha_list(plan, data, 1);
+    MHA_LAUNCH(dp, MHA_THIN4, plan->thin4, 256, st, a);
+    CG_CHECK_LAUNCH(name);
+  }
+  if (plan->thin1) {
+    a.items = mha_list(plan, data, 2);
+    MHA_LAUNCH(dp, MHA_THIN1, plan->thin1, 64, st, a);
+    CG_CHECK_LAUNCH(name);
+  }
+  if (plan->joins) {
+    a.items = mha_list(plan, data, 3);
+    mha_join_kernel<<<dim3(plan->joins, 8), 256, 0, st>>>(a);
+    CG_CHECK_LAUNCH(name);
+  }
+  return CG_OK;
+}
+
+extern "C" size_t cg_packed_attention_bwd_workspace_bytes(const cgAttentionPlan* plan, int q_rows) {
+  if (!plan || q_rows < 1) return 0;
+  return (size_t)q_rows * plan->heads * sizeof(float);
+}
+
+extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAttentionPlan* plan, const int32_t* data,
+                                       const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                                       void* dv, void* ws, size_t ws_bytes, cgStream stream) {
+  const char* name = "cg_packed_attention_bwd";
+  MhaArgs a = {};
+  const int rc = mha_check(name, in, plan, data, &a);
+  if (rc) return rc;
+  if (plan->max_q_row > 0) {
+    if (!out || !lse || !dout || !dq) CG_FAIL(CG_ERR_BAD_ARG, "%s: null tensor", name);
+    if (!ws || ws_bytes < cg_packed_attention_bwd_workspace_bytes(plan, in->q_rows))
+      CG_FAIL(CG_ERR_WORKSPACE, "%s: workspace of %zu bytes", name, ws_bytes);
+  }
+  if (plan->max_k_row > 0 && (!dk || !dv)) CG_FAIL(CG_ERR_BAD_ARG, "%s: null gradient", name);
+  const void* ptr[5] = {out, dout, dq, dk, dv};
+  for (const void* p : ptr)
+    if ((uintptr_t)p % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: tensors have to be 16-byte aligned", name);
+  a.o_in = (const bf16_t*)out;
+  a.lse_in = lse;
+  a.dout = (const bf16_t*)dout;
+  a.dq = (bf16_t*)dq;
+  a.dk = (bf16_t*)dk;
+  a.dv = (bf16_t*)dv;
+  a.delta = (const float*)ws;
+  const hipStream_t st = (hipStream_t)stream;
+  const int dp = mha_width(in->D, in->Dv);
+  if (plan->max_q_row > 0) {
+    const int64_t rows = (int64_t)in->q_rows * plan->heads;
+    if (rows > (int64_t)0x7fffffff * 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: too many rows", name);
+    mha_delta_kernel<<<(uint32_t)((rows + 15) / 16), 256, 0, st>>>(a.o_in, a.dout, rows, a.Dv, (float*)ws);
+    CG_CHECK_LAUNCH(name);
+  }
+  if (plan->dq_tiles) {
+    a.items = mha_list(plan, data, 4);
+    MHA_LAUNCH(dp, MHA_BWD_Q, plan->dq_tiles, 256, st, a);
+    CG_CHECK_LAUNCH(name);
+  }
+  if (plan->dkv_tiles) {
+    a.items = mha_list(plan, data, 5);
+    MHA_LAUNCH(dp, MHA_BWD_KV, plan->dkv_tiles, 256, st, a);
+    CG_CHECK_LAUNCH(name);
+  }
+  return CG_OK;
+}

@@ -60,6 +60,32 @@ class ConvFusion(ctypes.Structure):
                 ("bn_stat_group", ctypes.c_int32)]
 
 
+class HeadRows(ctypes.Structure):
+    """Mirror of cgHeadRows."""
+    _fields_ = [("x", vp), ("stride_t", c_i64), ("stride_h", c_i64), ("heads", ctypes.c_int32),
+                ("gain", vp)]
+
+
+class Rotation(ctypes.Structure):
+    """Mirror of cgRotation."""
+    _fields_ = [("positions", vp), ("freq", vp), ("amplitude", c_f32), ("axes", ctypes.c_int32),
+                ("rot", ctypes.c_int32), ("interleaved", ctypes.c_int32)]
+
+
+class AttentionPlanInfo(ctypes.Structure):
+    """Mirror of cgAttentionPlan."""
+    _fields_ = [("ints", c_i64), ("parts", c_i64)] + [(n, ctypes.c_int32) for n in (
+        "sequences", "heads", "kv_heads", "causal", "tiles", "thin4", "thin1", "joins", "dq_tiles",
+        "dkv_tiles", "small", "max_q_row", "max_k_row")]
+
+
+class AttentionInput(ctypes.Structure):
+    """Mirror of cgAttentionInput."""
+    _fields_ = [("q", vp), ("k", vp), ("v", vp)] + [(n, c_i64) for n in (
+        "q_stride_t", "q_stride_h", "k_stride_t", "k_stride_h", "v_stride_t", "v_stride_h")] + [
+            (n, ctypes.c_int32) for n in ("q_rows", "k_rows", "D", "Dv")] + [("scale", c_f32)]
+
+
 ADAM_CHUNK = 16384
 GP = ctypes.POINTER(ConvGeom)
 
@@ -170,6 +196,16 @@ SIGNATURES = {
     "cg_attention_bwd_workspace_bytes": (c_sz, [c_int, c_int, c_int, c_int, c_int]),
     "cg_attention_bwd": (c_int, [vp, vp, vp, vp, vp, vp, c_int, c_int, c_int, c_int, c_int, vp,
                                  vp, vp, vp, c_sz, vp]),
+    "cg_rotary": (c_int, [vp, c_int, c_int, c_int, vp, c_int, vp, vp]),
+    "cg_qk_norm_rotary_fwd": (c_int, [vp, vp, c_int, c_int, c_int, c_f32, vp, vp, vp, vp]),
+    "cg_qk_norm_rotary_bwd_workspace_bytes": (c_sz, [c_int, c_int]),
+    "cg_qk_norm_rotary_bwd": (c_int, [vp, vp, vp, vp, c_int, c_int, c_int, c_f32, vp, vp, vp, vp, vp, vp,
+                                      c_sz, vp]),
+    "cg_host_attention_plan": (c_int, [vp, vp, vp, vp, c_int, c_int, c_int, c_int, vp, c_i64, vp]),
+    "cg_packed_attention_fwd_workspace_bytes": (c_sz, [vp, c_int]),
+    "cg_packed_attention_fwd": (c_int, [vp, vp, vp, vp, vp, vp, c_sz, vp]),
+    "cg_packed_attention_bwd_workspace_bytes": (c_sz, [vp, c_int]),
+    "cg_packed_attention_bwd": (c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, c_sz, vp]),
     "cg_gan_loss": (c_int, [c_int, vp, c_int, vp, vp, vp, vp]),
     "cg_softmax_xent_eps": (c_int, [vp, vp, c_int, c_int, c_f32, vp, vp, vp]),
     "cg_s3gan_labels": (c_int, [vp, vp, c_int, c_int, c_int, vp, vp, vp]),

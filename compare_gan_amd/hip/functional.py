@@ -1006,6 +1006,81 @@ class AttentionFn(torch.autograd.Function):
     return K.attention_bwd(theta, phi, g, out, lse, _bf16(dout))
 
 
+class RotaryFn(torch.autograd.Function):
+  """Rotary positions (K.rotary); the adjoint turns by the negative angles."""
+
+  @staticmethod
+  def forward(ctx, x, positions, table):
+    ctx.save_for_backward(positions)
+    ctx.table = table
+    return K.rotary(x, positions, table)
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, dy):
+    (positions,) = ctx.saved_tensors
+    return K.rotary(dy, positions, ctx.table, inverse=True), None, None
+
+
+def rotary(x, positions, table):
+  """x [T, heads, D] (bf16 / fp32) with rotary positions (int32 [T] or [T, axes]) of a K.RotaryTable applied
+  to the first table.rotary_dim entries of every head; differentiable in x."""
+  return RotaryFn.apply(x, positions, table)
+
+
+class QkNormRotaryFn(torch.autograd.Function):
+  """RMS norm of every head of q and k, gains, rotation: one launch each way (K.qk_norm_rotary)."""
+
+  @staticmethod
+  def forward(ctx, q, k, q_gain, k_gain, positions, table, eps):
+    q_out, k_out = K.qk_norm_rotary(q, k, q_gain, k_gain, positions, table, eps)
+    ctx.save_for_backward(q, k, q_gain, k_gain, positions)
+    ctx.table, ctx.eps = table, eps
+    return q_out, k_out
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, dq_out, dk_out):
+    q, k, q_gain, k_gain, positions = ctx.saved_tensors
+    dq, dk, dqg, dkg = K.qk_norm_rotary_bwd(q, k, q_gain, k_gain, positions, ctx.table, dq_out.contiguous(),
+                                            dk_out.contiguous(), ctx.eps)
+    return dq, dk, dqg, dkg, None, None, None
+
+
+def qk_norm_rotary(q, k, q_gain, k_gain, positions=None, table=None, eps=1e-6):
+  """Queries [T, heads, D] and keys [T, kv_heads, D] of an attention block: RMS norm over every head times
+  a gain (fp32 [D] or None), then the rotation by `positions` (none without a table); differentiable in q, k
+  and the gains."""
+  return QkNormRotaryFn.apply(q, k, q_gain, k_gain, positions, table, eps)
+
+
+class PackedAttentionFn(torch.autograd.Function):
+  """Softmax attention with grouped heads over packed sequences (K.packed_attention_fwd / _bwd)."""
+
+  @staticmethod
+  def forward(ctx, q, k, v, plan, scale):
+    wanted = any(ctx.needs_input_grad[:3])
+    out, lse = K.packed_attention_fwd(q, k, v, plan, scale, want_lse=wanted)
+    if wanted:
+      ctx.save_for_backward(q, k, v, out, lse)
+      ctx.plan, ctx.scale = plan, scale
+    return out
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, dout):
+    q, k, v, out, lse = ctx.saved_tensors
+    dq, dk, dv = K.packed_attention_bwd(q, k, v, ctx.plan, out, lse, _bf16(dout), ctx.scale)
+    return dq, dk, dv, None, None
+
+
+def packed_attention(q, k, v, plan, scale=None):
+  """softmax(scale q k^T) v over the sequences of a K.AttentionPlan (q [rows, heads, D], k [rows, kv_heads, D],
+  v [rows, kv_heads, Dv], bf16); differentiable in q, k and v.  Rows outside every sequence give zeros and
+  get zero gradients."""
+  return PackedAttentionFn.apply(q, k, v, plan, scale)
+
+
 class ScaleWeightFn(torch.autograd.Function):
   """w_eff = sigma * w for a trainable device scalar sigma: `x + sigma * conv(a, w)`
   (arch_ops.py:755-758) runs as conv(a, sigma * w) with x as the convolution's residual -- no pass

@@ -2,12 +2,15 @@
 workspace allocation on the current torch HIP stream.  No arithmetic happens in Python/torch here;
 torch only owns the device memory and the stream."""
 import ctypes
+import math
 import os
 
+import numpy as np
 import torch
 
 from compare_gan_amd.hip import _lib
-from compare_gan_amd.hip._lib import ConvGeom, WgradItem, check
+from compare_gan_amd.hip._lib import (AttentionInput, AttentionPlanInfo, ConvGeom, HeadRows, Rotation,
+                                       WgradItem, check)
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -1080,6 +1083,353 @@ def attention_bwd(theta, phi, g, out, lse, dout):
                                  Dk, Dv, _p(dtheta), _p(dphi), _p(dg), _p(ws), ws.numel(),
                                  _stream()), "cg_attention_bwd")
     return dtheta, dphi, dg
+
+
+# ------------------------------------------------------------------------------------------------
+# multi-head attention on packed rows
+# ------------------------------------------------------------------------------------------------
+HEAD_TYPES = {BF16: 0, F32: 1}
+
+
+class RotaryTable(object):
+    """Frequencies of a rotary position encoding: pair i of the first `rotary_dim` entries of a head is
+    turned by position * f_i, f_i = base^(-i / n), n = rotary_dim / 2 / axes pairs an axis (pair i
+    belongs to axis i // n; axes = 2 for the row and column of a map).
+
+    layout   : "half" pairs (i, rotary_dim / 2 + i), "interleaved" pairs (2 i, 2 i + 1).
+    scaling  : for positions beyond the `original_length` the frequencies were learnt on, by `factor`:
+               "linear"  f / factor;
+               "ntk"     base * factor^(n / (n - 1)) in place of base (the fastest pair stays, the slowest
+                         is divided by factor);
+               "yarn"    pairs that turn more than 32 times over original_length stay, those that turn
+                         less than once are divided by factor, linear in the number of turns between
+                         (NTK by parts); the turned part is scaled by 0.1 ln(factor) + 1.
+    The table lives on `device` (fp64, turns a position) and is made once; it is read-only afterwards."""
+
+    SCALINGS = ("none", "linear", "ntk", "yarn")
+
+    def __init__(self, rotary_dim, layout="half", base=10000.0, scaling="none", factor=1.0,
+                 original_length=4096, axes=1, device="cuda"):
+        rotary_dim, axes = int(rotary_dim), int(axes)
+        if layout not in ("half", "interleaved"):
+            raise ValueError("layout must be 'half' or 'interleaved', got %r" % (layout,))
+        if scaling not in self.SCALINGS:
+            raise ValueError("scaling must be one of %s, got %r" % (", ".join(self.SCALINGS), scaling))
+        if axes < 1 or rotary_dim < 2 or rotary_dim % (2 * axes):
+            raise ValueError("rotary_dim must be a positive multiple of 2 * axes, got %d for %d axes" % (
+                rotary_dim, axes))
+        if not (base > 0.0 and math.isfinite(base)):
+            raise ValueError("base must be positive and finite, got %r" % (base,))
+        if not (factor >= 1.0 and math.isfinite(factor)):
+            raise ValueError("factor must be finite and at least 1, got %r" % (factor,))
+        if original_length < 1:
+            raise ValueError("original_length must be positive, got %r" % (original_length,))
+        n = rotary_dim // 2 // axes
+        self.amplitude = 1.0
+        if scaling == "ntk" and n > 1:
+            base = base * factor ** (n / (n - 1.0))
+        turns = []
+        for i in range(n):
+            f = base ** (-float(i) / n)
+            if scaling == "linear":
+                f /= factor
+            elif scaling == "yarn":
+                keep = (original_length * f / (2 * math.pi) - 1.0) / 31.0
+                keep = min(1.0, max(0.0, keep))
+                f = f * keep + f / factor * (1.0 - keep)
+            turns.append(f / (2 * math.pi))
+        if scaling == "yarn":
+            self.amplitude = 0.1 * math.log(factor) + 1.0
+        self.rotary_dim, self.axes, self.layout = rotary_dim, axes, layout
+        self.freq = torch.tensor(turns * axes, dtype=F64, device=device)
+        _ready_on_every_stream(self.freq)
+
+    def struct(self, positions):
+        return Rotation(_p(positions), _p(self.freq), self.amplitude, self.axes, self.rotary_dim,
+                        1 if self.layout == "interleaved" else 0)
+
+
+def _ready_on_every_stream(t):
+    """Constants (tables, plans) are used on any stream: wait for their upload once, when they are made."""
+    if t.is_cuda:
+        torch.cuda.current_stream(t.device).synchronize()
+
+
+def _req_heads(t, name, like=None):
+    """[T, heads, D] with the D entries of a head contiguous (other strides free)."""
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise ValueError("%s must be a tensor on the GPU (no CPU fallback exists)" % name)
+    if t.dim() != 3:
+        raise ValueError("%s must be [rows, heads, width], got %d dimensions" % (name, t.dim()))
+    if like is not None:
+        if t.device != like.device:
+            raise ValueError("%s is on %s, the other tensors on %s" % (name, t.device, like.device))
+        if t.dtype != like.dtype:
+            raise ValueError("%s must be %s, got %s" % (name, like.dtype, t.dtype))
+
+
+def _head_inner(t):
+    """`t` with its last dimension contiguous (a copy only where it is not)."""
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _head_rows(t, gain=None):
+    # a stride of a dimension of one entry means nothing: 0 keeps the alignment rules out of it
+    st = t.stride(0) if t.shape[0] > 1 else 0
+    sh = t.stride(1) if t.shape[1] > 1 else 0
+    return HeadRows(_p(t), st, sh, t.shape[1], _p(gain))
+
+
+def _rotary_args(x, positions, table):
+    """Checks positions against `x`; returns them contiguous."""
+    if not isinstance(table, RotaryTable):
+        raise ValueError("table must be a RotaryTable")
+    if not torch.is_tensor(positions) or not positions.is_cuda or positions.dtype != torch.int32:
+        raise ValueError("positions must be an int32 tensor on the GPU")
+    want = (x.shape[0],) if table.axes == 1 else (x.shape[0], table.axes)
+    if tuple(positions.shape) != want and not (table.axes == 1 and
+                                               tuple(positions.shape) == (x.shape[0], 1)):
+        raise ValueError("positions must be %s for %d axes, got %s" % (
+            list(want), table.axes, list(positions.shape)))
+    if positions.device != x.device or table.freq.device != x.device:
+        raise ValueError("positions, table and tensors must be on one device")
+    if table.rotary_dim > x.shape[2]:
+        raise ValueError("rotary_dim %d exceeds the head width %d" % (table.rotary_dim, x.shape[2]))
+    return positions.contiguous()
+
+
+def _req_width(x, name):
+    if x.dtype not in HEAD_TYPES:
+        raise ValueError("%s must be bfloat16 or float32, got %s" % (name, x.dtype))
+    if x.shape[1] < 1 or x.shape[2] < 2 or x.shape[2] % 2 or x.shape[2] > 256:
+        raise ValueError("%s: heads of even width up to 256 expected, got %s" % (name, list(x.shape)))
+
+
+def rotary(x, positions, table, inverse=False):
+    """x [T, heads, D] (bf16 / fp32) with the first table.rotary_dim entries of every head turned by the
+    angles of `positions` (int32 [T] or [T, axes]); inverse: the adjoint.  Returns a dense tensor."""
+    _req_heads(x, "x")
+    _req_width(x, "x")
+    positions = _rotary_args(x, positions, table)
+    x = _head_inner(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        check(lib().cg_rotary(ctypes.byref(_head_rows(x)), x.shape[0], x.shape[2], HEAD_TYPES[x.dtype],
+                              ctypes.byref(table.struct(positions)), 1 if inverse else 0, _p(y), _stream()),
+              "cg_rotary")
+    return y
+
+
+def _qk_args(q, k, q_gain, k_gain, positions, table, eps):
+    _req_heads(q, "q")
+    _req_width(q, "q")
+    _req_heads(k, "k", q)
+    _req_width(k, "k")
+    if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError("q %s and k %s must agree in rows and width" % (list(q.shape), list(k.shape)))
+    for g, nm in ((q_gain, "q_gain"), (k_gain, "k_gain")):
+        if g is not None:
+            _req(g, F32, nm)
+            if tuple(g.shape) != (q.shape[2],) or g.device != q.device:
+                raise ValueError("%s must be [%d] on %s" % (nm, q.shape[2], q.device))
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError("eps must be finite and not negative, got %r" % (eps,))
+    if (positions is None) != (table is None):
+        raise ValueError("positions and table come together")
+    return None if table is None else _rotary_args(q, positions, table)
+
+
+def qk_norm_rotary(q, k, q_gain, k_gain, positions, table, eps=1e-6):
+    """RMS norm of every head of q [T, heads, D] and k [T, kv_heads, D] over its D entries, times the gains
+    (fp32 [D] or None), then the rotation (positions = table = None: none), in one launch."""
+    positions = _qk_args(q, k, q_gain, k_gain, positions, table, eps)
+    q, k = _head_inner(q), _head_inner(k)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    rot = None if table is None else ctypes.byref(table.struct(positions))
+    with torch.cuda.device(q.device):
+        check(lib().cg_qk_norm_rotary_fwd(
+            ctypes.byref(_head_rows(q, q_gain)), ctypes.byref(_head_rows(k, k_gain)), q.shape[0], q.shape[2],
+            HEAD_TYPES[q.dtype], eps, rot, _p(q_out), _p(k_out), _stream()), "cg_qk_norm_rotary_fwd")
+    return q_out, k_out
+
+
+def qk_norm_rotary_bwd(q, k, q_gain, k_gain, positions, table, dq_out, dk_out, eps=1e-6):
+    """Gradients of qk_norm_rotary: dq, dk (dense, the inputs' type), dq_gain, dk_gain (fp32 [D], None
+    where the gain is None)."""
+    positions = _qk_args(q, k, q_gain, k_gain, positions, table, eps)
+    _req(dq_out, q.dtype, "dq_out")
+    _req(dk_out, q.dtype, "dk_out")
+    if dq_out.shape != q.shape or dk_out.shape != k.shape or dq_out.device != q.device or dk_out.device != q.device:
+        raise ValueError("dq_out and dk_out must have the shapes and the device of q and k")
+    q, k = _head_inner(q), _head_inner(k)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dqg = None if q_gain is None else torch.empty_like(q_gain)
+    dkg = None if k_gain is None else torch.empty_like(k_gain)
+    ws = _ws(lib().cg_qk_norm_rotary_bwd_workspace_bytes(q.shape[0], q.shape[2]), q)
+    rot = None if table is None else ctypes.byref(table.struct(positions))
+    with torch.cuda.device(q.device):
+        check(lib().cg_qk_norm_rotary_bwd(
+            ctypes.byref(_head_rows(q, q_gain)), ctypes.byref(_head_rows(k, k_gain)), _p(dq_out), _p(dk_out),
+            q.shape[0], q.shape[2], HEAD_TYPES[q.dtype], eps, rot, _p(dq), _p(dk), _p(dqg), _p(dkg), _p(ws),
+            ws.numel(), _stream()), "cg_qk_norm_rotary_bwd")
+    return dq, dk, dqg, dkg
+
+
+class AttentionPlan(object):
+    """What packed_attention does for given lengths, worked out once on the host
+    (cg_host_attention_plan) and kept on `device`.
+
+    q_lengths / k_lengths : rows of every sequence (k_lengths None: the same; zeros allowed).
+    q_starts / k_starts   : first row of every sequence (None: one behind the other); sequences must not
+                            overlap.  Rows between them belong to nobody -- a padded batch or a cache with
+                            room is [sequences * capacity, heads, D] with starts at multiples of capacity.
+    heads, kv_heads       : query head h reads key head h // (heads / kv_heads).
+    causal                : row i of a sequence sees its keys 0 .. i + k_length - q_length (the last row
+                            sees all of them; rows in front of the first key see none and give 0)."""
+
+    def __init__(self, q_lengths, k_lengths=None, heads=1, kv_heads=None, causal=False, q_starts=None,
+                 k_starts=None, device="cuda"):
+        heads = int(heads)
+        kv_heads = heads if kv_heads is None else int(kv_heads)
+        if heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise ValueError("heads (%d) must be a positive multiple of kv_heads (%d)" % (heads, kv_heads))
+        q_starts, q_lengths = _sequences(q_starts, q_lengths, "q")
+        k_starts, k_lengths = _sequences(k_starts, q_lengths if k_lengths is None else k_lengths, "k")
+        if len(q_lengths) != len(k_lengths):
+            raise ValueError("%d query and %d key sequences" % (len(q_lengths), len(k_lengths)))
+        self.heads, self.kv_heads, self.causal = heads, kv_heads, bool(causal)
+        args = [a.ctypes.data for a in (q_starts, q_lengths, k_starts, k_lengths)]
+        tail = (len(q_lengths), heads, kv_heads, 1 if causal else 0)
+        self.info = AttentionPlanInfo()
+        check(lib().cg_host_attention_plan(*args, *tail, None, 0, ctypes.byref(self.info)),
+              "cg_host_attention_plan")
+        self.host = np.empty(self.info.ints, dtype=np.int32)
+        check(lib().cg_host_attention_plan(*args, *tail, self.host.ctypes.data, self.info.ints,
+                                           ctypes.byref(self.info)), "cg_host_attention_plan")
+        self.q_rows, self.k_rows = self.info.max_q_row, self.info.max_k_row
+        # rows of sequences = all rows up to the last one: outputs need no zeros in between
+        self.q_dense = int(q_lengths.sum(dtype=np.int64)) == self.q_rows
+        self.k_dense = int(k_lengths.sum(dtype=np.int64)) == self.k_rows
+        self.device = torch.device(device)
+        self.data = torch.from_numpy(self.host).to(self.device)
+        _ready_on_every_stream(self.data)
+
+
+def _sequences(starts, lengths, name):
+    """(starts, lengths) as int32 arrays; refuses negative and overlapping sequences."""
+    lengths = np.asarray(lengths, dtype=np.int64).reshape(-1)
+    if lengths.size < 1:
+        raise ValueError("%s_lengths must name at least one sequence" % name)
+    if starts is None:
+        starts = np.concatenate(([0], np.cumsum(lengths)[:-1]))
+    starts = np.asarray(starts, dtype=np.int64).reshape(-1)
+    if starts.size != lengths.size:
+        raise ValueError("%s_starts names %d sequences, %s_lengths %d" % (name, starts.size, name, lengths.size))
+    if (lengths < 0).any() or (starts < 0).any() or (starts + lengths >= 2 ** 30).any():
+        raise ValueError("%s: starts and lengths must be in [0, 2^30)" % name)
+    live = lengths > 0
+    order = np.argsort(starts[live], kind="stable")
+    s, e = starts[live][order], (starts + lengths)[live][order]
+    if (s[1:] < e[:-1]).any():
+        raise ValueError("%s: sequences must not overlap" % name)
+    return np.ascontiguousarray(starts, dtype=np.int32), np.ascontiguousarray(lengths, dtype=np.int32)
+
+
+def _attention_operand(t):
+    """`t` as the kernels read it: entries of a head contiguous, rows and heads at multiples of 16 bytes
+    (a dense copy where it is not)."""
+    st = [t.stride(i) for i in (0, 1) if t.shape[i] > 1]
+    if t.stride(-1) != 1 or any(x % 8 for x in st) or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _attention_input(q, k, v, plan, scale):
+    if not isinstance(plan, AttentionPlan):
+        raise ValueError("plan must be an AttentionPlan")
+    _req_heads(q, "q")
+    if q.dtype != BF16:
+        raise ValueError("q must be %s, got %s" % (BF16, q.dtype))
+    _req_heads(k, "k", q)
+    _req_heads(v, "v", q)
+    if plan.data.device != q.device:
+        raise ValueError("the plan is on %s, the tensors on %s" % (plan.data.device, q.device))
+    if q.shape[1] != plan.heads or k.shape[1] != plan.kv_heads or v.shape[1] != plan.kv_heads:
+        raise ValueError("the plan is for %d heads over %d, got q %s, k %s, v %s" % (
+            plan.heads, plan.kv_heads, list(q.shape), list(k.shape), list(v.shape)))
+    if k.shape[2] != q.shape[2] or v.shape[0] != k.shape[0]:
+        raise ValueError("q %s, k %s and v %s do not fit together" % (list(q.shape), list(k.shape), list(v.shape)))
+    for w in (q.shape[2], v.shape[2]):
+        if w < 8 or w > 128 or w % 8:
+            raise ValueError("head widths must be multiples of 8 up to 128, got %d" % w)
+    if q.shape[0] < plan.q_rows or k.shape[0] < plan.k_rows:
+        raise ValueError("the plan's sequences end at query row %d and key row %d, got q %s and k %s" % (
+            plan.q_rows, plan.k_rows, list(q.shape), list(k.shape)))
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError("scale must be positive and finite, got %r" % (scale,))
+    return scale
+
+
+def _attention_struct(q, k, v, scale):
+    r = [_head_rows(t) for t in (q, k, v)]
+    return AttentionInput(r[0].x, r[1].x, r[2].x, r[0].stride_t, r[0].stride_h, r[1].stride_t, r[1].stride_h,
+                          r[2].stride_t, r[2].stride_h, q.shape[0], k.shape[0], q.shape[2], v.shape[2], scale)
+
+
+def _rows_out(shape, dense, used, device, dtype=BF16):
+    """An output whose rows outside every sequence are zero."""
+    if dense and used == shape[0]:
+        return torch.empty(shape, dtype=dtype, device=device)
+    return torch.zeros(shape, dtype=dtype, device=device)
+
+
+def packed_attention_fwd(q, k, v, plan, scale=None, want_lse=True, out=None):
+    """softmax(scale q k^T) v over the plan's sequences: q [rows, heads, D], k [rows, kv_heads, D],
+    v [rows, kv_heads, Dv] bf16 -> out [rows, heads, Dv] bf16, lse [rows, heads] fp32 (or None).
+    scale: 1 / sqrt(D) by default.  Rows of q outside every sequence give zeros -- or keep what `out`, if
+    given (dense), holds there."""
+    scale = _attention_input(q, k, v, plan, scale)
+    q, k, v = _attention_operand(q), _attention_operand(k), _attention_operand(v)
+    shape = (q.shape[0], q.shape[1], v.shape[2])
+    if out is None:
+        out = _rows_out(shape, plan.q_dense, plan.q_rows, q.device)
+    else:
+        _req(out, BF16, "out")
+        if tuple(out.shape) != shape or out.device != q.device or out.data_ptr() % 16:
+            raise ValueError("out must be %s on %s, 16-byte aligned" % (list(shape), q.device))
+    lse = torch.empty(shape[:2], dtype=F32, device=q.device) if want_lse else None
+    nbytes = lib().cg_packed_attention_fwd_workspace_bytes(ctypes.byref(plan.info), shape[2])
+    ws = _ws(nbytes, q) if nbytes else None
+    arg = _attention_struct(q, k, v, scale)
+    with torch.cuda.device(q.device):
+        check(lib().cg_packed_attention_fwd(ctypes.byref(arg), ctypes.byref(plan.info), _p(plan.data), _p(out),
+                                            _p(lse), _p(ws), nbytes, _stream()), "cg_packed_attention_fwd")
+    return out, lse
+
+
+def packed_attention_bwd(q, k, v, plan, out, lse, dout, scale=None):
+    """Gradients of packed_attention_fwd: dq, dk, dv, dense bf16 with zeros outside every sequence."""
+    scale = _attention_input(q, k, v, plan, scale)
+    q, k, v = _attention_operand(q), _attention_operand(k), _attention_operand(v)
+    shape = (q.shape[0], q.shape[1], v.shape[2])
+    for t, nm, dt, shp in ((out, "out", BF16, shape), (dout, "dout", BF16, shape), (lse, "lse", F32, shape[:2])):
+        _req(t, dt, nm)
+        if tuple(t.shape) != shp or t.device != q.device:
+            raise ValueError("%s must be %s on %s" % (nm, list(shp), q.device))
+    out, dout = _attention_operand(out), _attention_operand(dout)
+    dq = _rows_out(q.shape, plan.q_dense, plan.q_rows, q.device)
+    dk = _rows_out(k.shape, plan.k_dense, plan.k_rows, q.device)
+    dv = _rows_out(v.shape, plan.k_dense, plan.k_rows, q.device)
+    ws = _ws(lib().cg_packed_attention_bwd_workspace_bytes(ctypes.byref(plan.info), q.shape[0]), q)
+    arg = _attention_struct(q, k, v, scale)
+    with torch.cuda.device(q.device):
+        check(lib().cg_packed_attention_bwd(ctypes.byref(arg), ctypes.byref(plan.info), _p(plan.data), _p(out),
+                                            _p(lse), _p(dout), _p(dq), _p(dk), _p(dv), _p(ws), ws.numel(),
+                                            _stream()), "cg_packed_attention_bwd")
+    return dq, dk, dv
 
 
 # ------------------------------------------------------------------------------------------------

@@ -554,6 +554,82 @@ int cg_attention_bwd(const void* theta, const void* phi, const void* g, const vo
                      cgStream stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Multi-head attention on packed rows (what a block with several heads needs around the single-head
+ * core above, arch_ops.py:709-758 of the reference): rotary positions, the RMS norm of every head of the
+ * queries and keys with the rotation in the same pass, and softmax attention with grouped heads over
+ * sequences of different lengths.
+ * ------------------------------------------------------------------------------------------ */
+/* [T, heads, D] rows: strides in elements, the D entries of a head contiguous; gain [D] fp32 or NULL. */
+typedef struct {
+  const void* x;
+  int64_t stride_t, stride_h;
+  int32_t heads;
+  const float* gain;
+} cgHeadRows;
+/* positions [T, axes] int32; freq [rot / 2] fp64, in TURNS a position; pair i belongs to axis
+ * i / (rot / 2 / axes).  interleaved: pairs (2i, 2i + 1), else (i, rot / 2 + i).  Entries >= rot of a head
+ * are copied.  amplitude scales the turned part. */
+typedef struct {
+  const int32_t* positions;
+  const double* freq;
+  float amplitude;
+  int32_t axes, rot, interleaved;
+} cgRotation;
+/* dtype 0: bf16, 1: fp32.  D even, at most 256.  y [T, heads, D] contiguous.  inverse != 0: the adjoint
+ * (turns by -angle).  x->gain is not used. */
+int cg_rotary(const cgHeadRows* x, int T, int D, int dtype, const cgRotation* rot, int inverse, void* y,
+              cgStream stream);
+/* y = rotate(x * rsqrt(mean_d x^2 + eps) * gain) for the heads of q and of k; rot NULL: no rotation. */
+int cg_qk_norm_rotary_fwd(const cgHeadRows* q, const cgHeadRows* k, int T, int D, int dtype, float eps,
+                          const cgRotation* rot, void* q_out, void* k_out, cgStream stream);
+/* Gradients of the same: dq_out / dk_out contiguous; dq / dk contiguous out; dq_gain / dk_gain [D] fp32 or
+ * NULL (summed in a fixed order). */
+size_t cg_qk_norm_rotary_bwd_workspace_bytes(int T, int D);
+int cg_qk_norm_rotary_bwd(const cgHeadRows* q, const cgHeadRows* k, const void* dq_out, const void* dk_out,
+                          int T, int D, int dtype, float eps, const cgRotation* rot, void* dq, void* dk,
+                          float* dq_gain, float* dk_gain, void* ws, size_t ws_bytes, cgStream stream);
+
+/* What one packed attention does, worked out on the host from the lengths alone: sequence b has q_len[b]
+ * query rows from row q_start[b] on and k_len[b] key rows from k_start[b] on; `heads` query heads share
+ * `kv_heads` key heads (head h uses key head h / (heads / kv_heads)).  causal: query i of a sequence sees
+ * its keys 0 .. i + k_len - q_len.  The plan is a list of work items for every kernel, ordered by cost and
+ * dealt to the 8 XCDs so that the tiles of one key head share an L2; few rows against many keys are
+ * split over the keys.
+ * cg_host_attention_plan fills `info` and, if data_host is not NULL, `info->ints` int32 there; the caller
+ * copies them to the device and hands that copy and `info` to the kernels. */
+typedef struct {
+  int64_t ints;                       /* size of the plan in int32 */
+  int64_t parts;                      /* partial results: workspace of the forward pass */
+  int32_t sequences, heads, kv_heads, causal;
+  int32_t tiles, thin4, thin1, joins; /* forward work items of each form */
+  int32_t dq_tiles, dkv_tiles, small; /* backward work items of each form */
+  int32_t max_q_row, max_k_row;       /* rows that the tensors must have at least */
+} cgAttentionPlan;
+int cg_host_attention_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start,
+                           const int32_t* k_len, int sequences, int heads, int kv_heads, int causal,
+                           int32_t* data_host, int64_t capacity, cgAttentionPlan* info);
+/* q [q_rows, heads, D], k [k_rows, kv_heads, D], v [k_rows, kv_heads, Dv] bf16, strides in elements, heads
+ * contiguous inside; D and Dv multiples of 8, at most 128; scale > 0.  out [q_rows, heads, Dv] contiguous,
+ * lse [q_rows, heads] fp32 (NULL: not wanted).  Rows that see no key: out 0, lse -inf.  Rows that belong to
+ * no sequence are left as they were. */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  int32_t q_rows, k_rows, D, Dv;
+  float scale;
+} cgAttentionInput;
+size_t cg_packed_attention_fwd_workspace_bytes(const cgAttentionPlan* plan, int Dv);
+int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAttentionPlan* plan, const int32_t* data,
+                            void* out, float* lse, void* ws, size_t ws_bytes, cgStream stream);
+/* Gradients: out, lse of the forward pass, dout [q_rows, heads, Dv] contiguous; dq [q_rows, heads, D],
+ * dk [k_rows, kv_heads, D], dv [k_rows, kv_heads, Dv] contiguous bf16, every row of a sequence written
+ * (the shared heads of a key head summed inside, no atomics). */
+size_t cg_packed_attention_bwd_workspace_bytes(const cgAttentionPlan* plan, int q_rows);
+int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAttentionPlan* plan, const int32_t* data,
+                            const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                            void* dv, void* ws, size_t ws_bytes, cgStream stream);
+
+/* ------------------------------------------------------------------------------------------
  * Losses (gans/loss_lib.py:53-148) and WGAN-GP (gans/penalty_lib.py:59-82).
  * kind: 0 non_saturating, 1 wasserstein, 2 least_squares, 3 hinge.
  * logits fp32 [2B] = real (first B) then fake (last B) (modular_gan.py:657-661).

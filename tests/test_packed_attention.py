@@ -1,0 +1,220 @@
+"""Rotary tables, plans and refusals of the packed attention operators (no GPU)."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from compare_gan_amd.hip import _lib
+from compare_gan_amd.hip import functional as Fn
+from compare_gan_amd.hip import kernels as K
+
+
+# -- frequencies ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("rot,axes", [(2, 1), (4, 2), (64, 1), (64, 2), (36, 3)])
+@pytest.mark.parametrize("scaling,factor", [("none", 1.0), ("linear", 8.0), ("ntk", 4.0), ("yarn", 16.0)])
+def test_rotary_table(rot, axes, scaling, factor):
+  t = K.RotaryTable(rot, base=10000.0, scaling=scaling, factor=factor, original_length=2048, axes=axes,
+                    device="cpu")
+  assert t.freq.dtype == torch.float64 and t.freq.shape == (rot // 2,)
+  n = rot // 2 // axes
+  f = t.freq.numpy() * 2 * math.pi
+  for a in range(1, axes):
+    np.testing.assert_array_equal(f[:n], f[a * n:(a + 1) * n])
+  plain = 10000.0 ** (-np.arange(n) / n)
+  if scaling == "none":
+    np.testing.assert_allclose(f[:n], plain, rtol=1e-14)
+  elif scaling == "linear":
+    np.testing.assert_allclose(f[:n], plain / factor, rtol=1e-14)
+  elif scaling == "ntk":      # the fastest pair stays, the slowest is divided by the factor
+    assert f[0] == pytest.approx(1.0, rel=1e-14)
+    if n > 1:
+      assert f[n - 1] == pytest.approx(plain[-1] / factor, rel=1e-12)
+  else:
+    turns = 2048 * plain / (2 * math.pi)
+    for i in range(n):
+      if turns[i] >= 32:
+        assert f[i] == pytest.approx(plain[i], rel=1e-14)
+      elif turns[i] <= 1:
+        assert f[i] == pytest.approx(plain[i] / factor, rel=1e-14)
+      else:
+        assert plain[i] / factor < f[i] < plain[i]
+  assert t.amplitude == (0.1 * math.log(factor) + 1.0 if scaling == "yarn" else 1.0)
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=6, axes=2),
+                                dict(rotary_dim=8, layout="pairs"), dict(rotary_dim=8, scaling="log"),
+                                dict(rotary_dim=8, base=0.0), dict(rotary_dim=8, base=float("nan")),
+                                dict(rotary_dim=8, scaling="linear", factor=0.5),
+                                dict(rotary_dim=8, factor=float("inf")), dict(rotary_dim=8, axes=0),
+                                dict(rotary_dim=8, original_length=0)])
+def test_rotary_table_refusals(kw):
+  with pytest.raises(ValueError):
+    K.RotaryTable(device="cpu", **kw)
+
+
+# -- plans ---------------------------------------------------------------------------------------
+def _lists(plan):
+  i = plan.info
+  at = 4 * i.sequences
+  out = {"seqs": plan.host[:at].reshape(-1, 4)}
+  for name in ("tiles", "thin4", "thin1", "joins", "dq_tiles", "dkv_tiles"):
+    n = getattr(i, name)
+    out[name] = plan.host[at:at + 8 * n].reshape(n, 8)
+    at += 8 * n
+  assert at == i.ints
+  return out
+
+
+PLANS = [
+    ("one token", [1], None, 1, 1, False, None),
+    ("ragged", [2047, 1, 0, 5000, 333, 64, 129], None, 8, 2, True, None),
+    ("maps", [256] * 40, None, 3, 3, False, None),
+    ("new tokens", [1] * 5, [1, 8192, 0, 777, 40000], 32, 8, True, 40000),
+    ("few rows, many keys", [200], [70001], 2, 1, False, None),
+    ("queries in front of the keys", [100, 40], [30, 0], 4, 4, True, None),
+    ("odd heads", [33, 65, 31], [64, 1, 300], 15, 3, True, 512),
+    ("one row a head, 40 shared", [1], [3000], 40, 1, False, None),
+]
+
+
+@pytest.mark.parametrize("case", PLANS, ids=[c[0] for c in PLANS])
+def test_plan_covers_every_row_and_key_once(case):
+  _, q, k, heads, kv_heads, causal, capacity = case
+  kk = q if k is None else k
+  starts = None if capacity is None else [i * capacity for i in range(len(kk))]
+  plan = K.AttentionPlan(q, k, heads=heads, kv_heads=kv_heads, causal=causal, k_starts=starts, device="cpu")
+  p, g = _lists(plan), heads // kv_heads
+  assert p["seqs"][:, 1].tolist() == list(q) and p["seqs"][:, 3].tolist() == list(kk)
+  assert plan.q_rows == sum(q) and plan.q_dense
+  assert plan.k_rows == max([s + n for s, n in zip(p["seqs"][:, 2].tolist(), kk) if n] + [0])
+
+  def seen(b, token):            # keys of a token
+    return max(0, min(kk[b], token + kk[b] - q[b] + 1)) if causal else kk[b]
+
+  used = set()
+  pieces = {}
+  for name, tile, step in (("tiles", 128, 64), ("thin4", 32, 32), ("thin1", 32, 32)):
+    for b, h, row0, k0, k1, part, _, _ in p[name].tolist():
+      rows = q[b] * g
+      assert 0 <= h < kv_heads and row0 % tile == 0 and row0 < rows and (rows > 32) == (name == "tiles")
+      assert 0 <= k0 <= k1 <= kk[b] and k0 % step == 0
+      pieces.setdefault((b, h, row0), []).append((k0, k1, part))
+      if part >= 0:
+        units = tile // 32
+        assert not used & set(range(part, part + units))
+        used |= set(range(part, part + units))
+  assert len(used) == plan.info.parts and (not used or max(used) == plan.info.parts - 1)
+  joins = {(b, h, r): (n, parts, unit, units) for b, h, r, n, parts, unit, units, _ in p["joins"].tolist()}
+  for b, n in enumerate(q):
+    for h in range(kv_heads):
+      tile = 128 if n * g > 32 else 32
+      for r in range(0, n * g, tile):
+        got = sorted(pieces.pop((b, h, r)))
+        end = seen(b, (min(r + tile, n * g) - 1) // g)
+        assert got[0][0] == 0 and got[-1][1] == end
+        assert all(x[1] == y[0] for x, y in zip(got, got[1:]))
+        if len(got) == 1:
+          assert got[0][2] == -1 and (b, h, r) not in joins
+        else:
+          rows, parts, unit, units = joins.pop((b, h, r))
+          assert rows == min(tile, n * g - r) and units == tile // 32
+          assert [x[2] for x in got] == [unit + i * units for i in range(parts)]
+  assert not pieces and not joins
+  dq = sorted((b, h, r, k1) for b, h, r, _, k1, _, _, _ in p["dq_tiles"].tolist())
+  assert dq == sorted((b, h, r, seen(b, (min(r + 128, n * g) - 1) // g)) for b, n in enumerate(q)
+                      for h in range(kv_heads) for r in range(0, n * g, 128))
+  want = []
+  for b, n in enumerate(kk):
+    for h in range(kv_heads):
+      for key in range(0, n, 128):
+        first = 0
+        while first < q[b] and seen(b, first) <= key:
+          first += 1
+        want.append((b, h, key, first * g, q[b] * g))
+  assert sorted((b, h, r, a, e) for b, h, r, a, e, _, _, _ in p["dkv_tiles"].tolist()) == sorted(want)
+
+
+def test_plan_spreads_few_rows_over_the_chip():
+  plan = K.AttentionPlan([1] * 4, [50000] * 4, heads=8, kv_heads=2, causal=True, device="cpu")
+  p = _lists(plan)
+  assert len(p["thin4"]) >= 512 and len(p["joins"]) == 8
+  assert max(k1 - k0 for _, _, _, k0, k1, _, _, _ in p["thin4"].tolist()) <= 1024
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q_lengths=[]), dict(q_lengths=[-1]), dict(q_lengths=[4], k_lengths=[4, 4]),
+    dict(q_lengths=[4], heads=3, kv_heads=2), dict(q_lengths=[4], heads=0),
+    dict(q_lengths=[4, 4], q_starts=[0, 2]), dict(q_lengths=[4, 4], q_starts=[0]),
+    dict(q_lengths=[4, 4], k_starts=[3, 0]), dict(q_lengths=[4], k_starts=[-1]),
+    dict(q_lengths=[2 ** 30]), dict(q_lengths=[2 ** 40]), dict(q_lengths=[4], heads=8192)])
+def test_plan_refusals(kw):
+  with pytest.raises((ValueError, _lib.CgamdError)):
+    K.AttentionPlan(device="cpu", **kw)
+
+
+def test_plan_entry_point_refuses_without_throwing():
+  lib = _lib.load()
+  info = _lib.AttentionPlanInfo()
+  one = np.ones(1, np.int32)
+  p = one.ctypes.data
+  assert lib.cg_host_attention_plan(None, p, p, p, 1, 1, 1, 0, None, 0, ctypes.byref(info)) == -1
+  assert lib.cg_host_attention_plan(p, p, p, p, 0, 1, 1, 0, None, 0, ctypes.byref(info)) == -1
+  assert lib.cg_host_attention_plan(p, p, p, p, 1, 3, 2, 0, None, 0, ctypes.byref(info)) == -1
+  assert lib.cg_host_attention_plan(p, p, p, p, 1, 1, 1, 0, p, 1, ctypes.byref(info)) == -4
+  neg = -one
+  assert lib.cg_host_attention_plan(p, neg.ctypes.data, p, p, 1, 1, 1, 0, None, 0, ctypes.byref(info)) == -1
+
+
+def test_entry_points_refuse_without_a_launch():
+  """Pointers that are never followed: every refusal comes before the first launch."""
+  lib = _lib.load()
+  fake = 4096
+  plan = K.AttentionPlan([4], heads=2, kv_heads=1, device="cpu")
+  info = ctypes.byref(plan.info)
+
+  def call(entry, **kw):
+    f = dict(q=fake, k=fake, v=fake, q_stride_t=128, q_stride_h=64, k_stride_t=64, k_stride_h=64,
+             v_stride_t=64, v_stride_h=64, q_rows=4, k_rows=4, D=64, Dv=64, scale=1.0)
+    f.update(kw)
+    arg = ctypes.byref(_lib.AttentionInput(*[f[n] for n, _ in _lib.AttentionInput._fields_]))
+    if entry == "fwd":
+      return lib.cg_packed_attention_fwd(arg, info, fake, None, None, None, 0, None)
+    return lib.cg_packed_attention_bwd(arg, info, fake, fake, fake, fake, fake, fake, fake, None, 0, None)
+  for entry in ("fwd", "bwd"):
+    assert call(entry, D=60) == -2 and call(entry, Dv=136) == -2 and call(entry, D=0) == -2
+    assert call(entry, scale=0.0) == -1 and call(entry, scale=float("nan")) == -1
+    assert call(entry, scale=float("inf")) == -1
+    assert call(entry, q_rows=3) == -1 and call(entry, k_rows=3) == -1
+    assert call(entry, k_stride_t=63) == -2 and call(entry, q_stride_t=-8) == -2
+    assert call(entry, v=fake + 8) == -2 and call(entry, q=None) == -1
+    assert call(entry, k_stride_t=2 ** 26) == -2
+  assert call("fwd") == -1          # no output
+  assert call("bwd") == -4          # no workspace
+  rows = _lib.HeadRows(fake, 64, 64, 1, None)
+  r = ctypes.byref(rows)
+  rot = _lib.Rotation(fake, fake, 1.0, 1, 64, 0)
+  wide = _lib.Rotation(fake, fake, 1.0, 2, 66, 0)
+  assert lib.cg_rotary(r, 1, 63, 0, ctypes.byref(rot), 0, fake, None) == -2
+  assert lib.cg_rotary(r, 1, 258, 0, ctypes.byref(rot), 0, fake, None) == -2
+  assert lib.cg_rotary(r, 1, 64, 2, ctypes.byref(rot), 0, fake, None) == -2
+  assert lib.cg_rotary(r, 1, 64, 0, ctypes.byref(wide), 0, fake, None) == -1
+  assert lib.cg_rotary(r, 1, 64, 0, None, 0, fake, None) == -1
+  assert lib.cg_rotary(r, 1, 64, 0, ctypes.byref(rot), 0, None, None) == -1
+  assert lib.cg_qk_norm_rotary_fwd(r, None, 1, 64, 0, 1e-6, None, fake, fake, None) == -1
+  assert lib.cg_qk_norm_rotary_fwd(r, r, 1, 64, 0, -1.0, None, fake, fake, None) == -1
+  assert lib.cg_qk_norm_rotary_bwd(r, r, fake, fake, 1, 64, 0, 1e-6, None, fake, fake, fake, fake, None, 0,
+                                   None) == -4
+
+
+def test_operators_refuse_host_tensors():
+  x = torch.zeros(2, 1, 8)
+  pos = torch.zeros(2, dtype=torch.int32)
+  table = K.RotaryTable(8, device="cpu")
+  with pytest.raises(ValueError, match="GPU"):
+    Fn.rotary(x, pos, table)
+  with pytest.raises(ValueError, match="GPU"):
+    Fn.qk_norm_rotary(x, x, None, None, pos, table)
+  with pytest.raises(ValueError, match="GPU"):
+    Fn.packed_attention(x.bfloat16(), x.bfloat16(), x.bfloat16(), K.AttentionPlan([2], device="cpu"))

@@ -1,0 +1,648 @@
+"""Rotary positions, norms of queries and keys with the rotation, and packed attention on the GPU, against
+plain implementations in 64 bits.
+
+Tolerances count roundings.  A value rounded to bf16 is off by at most half a step, HB = 2^-8 of itself, to fp32 by HF =
+2^-24.  Attention: the weights P enter the matrix instruction in bf16, so |out - exact| <= HB sum_j P_j |v_j| (weights)
++ HB |out| (the result), plus the weights' own relative error rp: a score is a fp32 sum of D products, off by at most
+D HF sum |q k| scale, and the exponential and the sum of the weights add some 2^-20.  Backward likewise, with the error
+of delta = sum dout out (out was rounded) and of dS on its way into the matrix instruction.
+"""
+import math
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HB, HF = 2.0 ** -8, 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def K(dev):
+  from compare_gan_amd.hip import kernels
+  return kernels
+
+
+@pytest.fixture(scope="module")
+def Fn(dev):
+  from compare_gan_amd.hip import functional
+  return functional
+
+
+def within(got, want, tol, what):
+  got = got.double().cpu()
+  bad = ~((got - want).abs() <= tol)
+  if bad.any():
+    i = tuple(int(x) for x in bad.nonzero()[0])
+    ratio = ((got - want).abs() / tol).nan_to_num(float("inf")).max()
+    raise AssertionError("%s: %d of %d off, first at %s: %r, exact %r, tolerance %r (worst ratio %.3g)" % (
+        what, int(bad.sum()), got.numel(), i, float(got[i]), float(want[i]), float(tol[i]), ratio))
+
+
+def normal(gen, shape, dtype=torch.bfloat16):
+  return torch.randn(shape, generator=gen).to(dtype)
+
+
+# ------------------------------------------------------------------------------------------------
+# rotation and norm
+# ------------------------------------------------------------------------------------------------
+def exact_turn(x, positions, table, inverse=False):
+  """x fp64 [T, H, D] on the CPU; also the sum of the magnitudes that meet in every entry."""
+  rot, n = table.rotary_dim, table.rotary_dim // 2 // table.axes
+  f = table.freq.cpu() * 2 * math.pi
+  pos = positions.cpu().double().reshape(x.shape[0], -1)
+  angle = torch.cat([pos[:, a:a + 1] * f[a * n:(a + 1) * n] for a in range(table.axes)], 1)[:, None]
+  c, s = torch.cos(angle) * table.amplitude, torch.sin(angle) * table.amplitude * (-1 if inverse else 1)
+  half = table.layout == "half"
+  a = x[..., :rot // 2] if half else x[..., 0:rot:2]
+  b = x[..., rot // 2:rot] if half else x[..., 1:rot:2]
+  y, mag = x.clone(), x.abs()
+  both = (a.abs() + b.abs()) * table.amplitude
+  if half:
+    y[..., :rot // 2], y[..., rot // 2:rot] = a * c - b * s, a * s + b * c
+    mag[..., :rot // 2], mag[..., rot // 2:rot] = both, both
+  else:
+    y[..., 0:rot:2], y[..., 1:rot:2] = a * c - b * s, a * s + b * c
+    mag[..., 0:rot:2], mag[..., 1:rot:2] = both, both
+  return y, mag
+
+
+def half_step(dtype):
+  return HB if dtype == torch.bfloat16 else HF
+
+
+# a turned entry: the angle (reduced in 64 bits, then fp32: half a step of half a turn = 2^-25 turns, 2 pi 2^-25 < 2^-22
+# rad), cosine / sine (fp32 library: 2 steps; bf16 data: the hardware's, taken as good to 2^-16), three fp32 roundings
+def turn_error(dtype):
+  return 2.0 ** -15 if dtype == torch.bfloat16 else 2.0 ** -22 + 2 * 2.0 ** -23 + 3 * HF
+
+
+ROTARY = [
+    # T, H, D, rot, layout, axes, scaling, dtype
+    (1, 1, 2, 2, "half", 1, "none", torch.float32),
+    (1, 3, 64, 64, "half", 1, "none", torch.bfloat16),
+    (7, 8, 64, 32, "interleaved", 1, "linear", torch.bfloat16),
+    (130, 5, 80, 40, "half", 1, "yarn", torch.float32),
+    (65, 2, 18, 10, "interleaved", 1, "ntk", torch.float32),
+    (33, 3, 36, 36, "half", 3, "none", torch.bfloat16),
+    (1000, 4, 128, 128, "half", 2, "yarn", torch.bfloat16),
+    (19, 2, 256, 256, "half", 1, "none", torch.bfloat16),
+    (19, 3, 254, 254, "interleaved", 1, "none", torch.float32),
+    (5, 17, 16, 16, "half", 1, "none", torch.bfloat16),
+    (4099, 1, 96, 48, "interleaved", 2, "none", torch.bfloat16),
+]
+
+
+def positions_of(gen, t, axes, far):
+  return torch.randint(-far // 8, far, (t, axes) if axes > 1 else (t,), generator=gen, dtype=torch.int32).cuda()
+
+
+@pytest.mark.parametrize("case", ROTARY, ids=[str(i) for i in range(len(ROTARY))])
+def test_rotary(K, Fn, case):
+  t, h, d, rot, layout, axes, scaling, dtype = case
+  gen = torch.Generator().manual_seed(t + h + d)
+  table = K.RotaryTable(rot, layout=layout, scaling=scaling, factor=4.0, axes=axes)
+  pos = positions_of(gen, t, axes, 1 << 20)
+  x = normal(gen, (t, h, d), dtype).cuda().requires_grad_(True)
+  y = Fn.rotary(x, pos, table)
+  want, mag = exact_turn(x.detach().double().cpu(), pos, table)
+  assert y.dtype == dtype and y.shape == x.shape
+  within(y, want, half_step(dtype) * want.abs() + turn_error(dtype) * mag + 1e-30, "y")
+  assert torch.equal(y[..., rot:], x[..., rot:])
+  dy = normal(gen, (t, h, d), dtype).cuda()
+  (dx,) = torch.autograd.grad(y, (x,), dy)
+  want, mag = exact_turn(dy.double().cpu(), pos, table, inverse=True)
+  within(dx, want, half_step(dtype) * want.abs() + turn_error(dtype) * mag + 1e-30, "dx")
+
+
+def exact_norm(x, gain, eps):
+  inv = 1.0 / torch.sqrt(x.square().mean(-1, keepdim=True) + eps)
+  return x * inv * (1.0 if gain is None else gain)
+
+
+QK = [
+    # T, H, Hk, D, rot, layout, axes, dtype, merged, gains
+    (1, 1, 1, 2, 2, "half", 1, torch.float32, False, True),
+    (3, 4, 1, 64, 64, "half", 1, torch.bfloat16, False, True),
+    (300, 6, 6, 32, 32, "half", 2, torch.bfloat16, False, True),
+    (1009, 12, 4, 72, 36, "interleaved", 1, torch.bfloat16, True, True),
+    (77, 3, 1, 50, 22, "half", 1, torch.float32, True, True),
+    (40, 2, 2, 256, 128, "interleaved", 1, torch.bfloat16, False, False),
+    (40, 2, 1, 250, 250, "half", 1, torch.float32, False, True),
+    (2500, 8, 2, 128, 128, "half", 1, torch.bfloat16, True, True),
+    (64, 5, 5, 16, 0, "half", 1, torch.bfloat16, False, True),
+]
+
+
+@pytest.mark.parametrize("case", QK, ids=[str(i) for i in range(len(QK))])
+def test_qk_norm_rotary(K, Fn, case):
+  t, h, hk, d, rot, layout, axes, dtype, merged, gains = case
+  gen = torch.Generator().manual_seed(t + h + d)
+  table = K.RotaryTable(rot, layout=layout, axes=axes) if rot else None
+  pos = positions_of(gen, t, axes, 100000) if rot else None
+  whole = normal(gen, (t, h + 2 * hk, d), dtype)
+  whole[0] = 0.0                                   # a head of zeros: eps carries the norm
+  whole = whole.cuda()
+  q, k = whole[:, :h], whole[:, h:h + hk]
+  if not merged:
+    q, k = q.contiguous(), k.contiguous()
+  q, k = q.detach().requires_grad_(True), k.detach().requires_grad_(True)
+  qg = (1 + 0.3 * normal(gen, (d,), torch.float32)).cuda().requires_grad_(True) if gains else None
+  kg = (1 + 0.3 * normal(gen, (d,), torch.float32)).cuda().requires_grad_(True) if gains else None
+  eps = 1e-6
+  qo, ko = Fn.qk_norm_rotary(q, k, qg, kg, pos, table, eps=eps)
+  dqo, dko = normal(gen, q.shape, dtype).cuda(), normal(gen, k.shape, dtype).cuda()
+  wanted = [x for x in (q, k, qg, kg) if x is not None]
+  grads = torch.autograd.grad((qo, ko), wanted, (dqo, dko))
+  te = turn_error(dtype)
+  for x, g, y, dy, dx, dg in ((q, qg, qo, dqo, grads[0], grads[2] if gains else None),
+                              (k, kg, ko, dko, grads[1], grads[3] if gains else None)):
+    x64, g64 = x.detach().double().cpu(), (g.detach().double().cpu() if gains else None)
+    n64 = exact_norm(x64, g64, eps)
+    # sum of d squares, square root, divide, two products: (d + 5) fp32 roundings at most, before the turn
+    rn = (d + 5) * HF
+    want, mag = exact_turn(n64, pos, table) if rot else (n64, n64.abs())
+    within(y, want, half_step(dtype) * want.abs() + (te + rn) * mag + 1e-30, "y")
+    gy = dy.double().cpu()
+    gr, gmag = exact_turn(gy, pos, table, inverse=True) if rot else (gy, gy.abs())
+    inv = 1.0 / torch.sqrt(x64.square().mean(-1, keepdim=True) + eps)
+    unit = x64 * inv
+    gg = gr * (g64 if gains else 1.0)
+    ggm = gmag * (g64.abs() if gains else 1.0)
+    want = inv * (gg - unit * (gg * unit).mean(-1, keepdim=True))
+    size = inv * (ggm + unit.abs() * (ggm * unit.abs()).mean(-1, keepdim=True))
+    within(dx, want, half_step(dtype) * want.abs() + (te + 3 * rn) * size + 1e-30, "dx")
+    if gains:
+      # a fp32 sum of T heads terms in a tree of partial sums: at most (T heads) roundings of the running sum; the
+      # partials of a block and the blocks' join keep it far below, the bound used is the square root of that
+      rows = t * x.shape[1]
+      size = (gmag * unit.abs()).sum((0, 1))
+      within(dg, (gr * unit).sum((0, 1)), (te + 3 * rn + math.sqrt(rows) * HF) * size + 1e-30, "dgain")
+
+
+def test_rotation_on_strided_views(K, Fn):
+  """Heads and rows at any stride; a transposed head width is copied; unaligned starts take the narrow loads."""
+  gen = torch.Generator().manual_seed(5)
+  table = K.RotaryTable(32)
+  big = normal(gen, (9, 40, 70)).cuda()
+  for x in (big[:, 3:17:2, 1:65], big[::2, :5, 6:70], big[:, :, :64].transpose(0, 1), big[:, :, 2:66],
+            normal(gen, (6, 64, 7)).cuda().transpose(1, 2), normal(gen, (1, 1, 64)).cuda().expand(4, 3, 64)):
+    pos = positions_of(gen, x.shape[0], 1, 5000)
+    want, mag = exact_turn(x.double().cpu(), pos, table)
+    y = Fn.rotary(x, pos, table)
+    assert y.is_contiguous()
+    within(y, want, HB * want.abs() + turn_error(torch.bfloat16) * mag + 1e-30, "strided")
+
+
+def test_rotation_of_nothing(K, Fn):
+  table = K.RotaryTable(16)
+  none = torch.empty((0,), dtype=torch.int32, device="cuda")
+  x = torch.empty((0, 2, 16), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+  assert Fn.rotary(x, none, table).shape == (0, 2, 16)
+  g = torch.ones(16, device="cuda", requires_grad=True)
+  q, k = Fn.qk_norm_rotary(x, x, g, g, none, table)
+  dx, dg = torch.autograd.grad((q, k), (x, g), (torch.empty_like(q), torch.empty_like(k)))
+  assert dx.shape == (0, 2, 16) and torch.equal(dg, torch.zeros_like(dg))
+
+
+def test_rotation_refusals(K, Fn):
+  table, pos = K.RotaryTable(16, axes=2), torch.zeros((4, 2), dtype=torch.int32, device="cuda")
+  x = torch.zeros((4, 2, 32), dtype=torch.bfloat16, device="cuda")
+  assert Fn.rotary(x, pos, table).shape == x.shape
+  for bad in (dict(x=x.half()), dict(x=x[0]), dict(x=x[..., :31]), dict(positions=pos.long()), dict(positions=pos[:3]),
+              dict(positions=pos[:, 0]), dict(positions=pos.cpu()), dict(table=None), dict(x=x[..., :8]),
+              dict(x=torch.zeros((4, 2, 258), dtype=torch.bfloat16, device="cuda"))):
+    with pytest.raises(ValueError):
+      Fn.rotary(**dict(dict(x=x, positions=pos, table=table), **bad))
+  g = torch.ones(32, device="cuda")
+  good = dict(q=x, k=x, q_gain=g, k_gain=None, positions=pos, table=table)
+  Fn.qk_norm_rotary(**good)
+  for bad in (dict(k=x.float()), dict(k=x[:3]), dict(k=x[..., :16]), dict(q_gain=g[:16]), dict(q_gain=g.double()),
+              dict(positions=None), dict(eps=-1.0), dict(eps=float("nan"))):
+    with pytest.raises(ValueError):
+      Fn.qk_norm_rotary(**dict(good, **bad))
+
+
+# ------------------------------------------------------------------------------------------------
+# attention
+# ------------------------------------------------------------------------------------------------
+def exact_attention(q, k, v, dout, seqs, heads, kv_heads, causal, scale):
+  """fp64 on the CPU: outputs, gradients and their tolerances (None entries of dout: forward only)."""
+  q, k, v = q.double().cpu(), k.double().cpu(), v.double().cpu()
+  g, d = heads // kv_heads, q.shape[2]
+  out = torch.zeros(q.shape[0], heads, v.shape[2], dtype=torch.float64)
+  tout = torch.full_like(out, 1e-30)
+  res = {"out": (out, tout)}
+  if dout is not None:
+    dout = dout.double().cpu()
+    for name, t in (("dq", q), ("dk", k), ("dv", v)):
+      res[name] = (torch.zeros_like(t), torch.zeros_like(t))
+  for q0, lq, k0, lk in seqs:
+    if lq == 0 or lk == 0:
+      continue
+    see = torch.ones(lq, lk, dtype=torch.bool)
+    if causal:
+      see = torch.arange(lk)[None] <= torch.arange(lq)[:, None] + (lk - lq)
+    for h in range(heads):
+      a, b, c = q[q0:q0 + lq, h], k[k0:k0 + lk, h // g], v[k0:k0 + lk, h // g]
+      s = (a @ b.t() * scale).masked_fill(~see, -math.inf)
+      top = s.amax(-1, keepdim=True)
+      p = torch.exp(s - torch.where(top == -math.inf, torch.zeros_like(top), top))
+      p = p / p.sum(-1, keepdim=True).clamp_min(1e-300)
+      o = p @ c
+      rp = 2 * scale * d * HF * float((a.abs() @ b.abs().t()).max()) + 2.0 ** -20
+      to = (HB + rp) * (p @ c.abs()) + HB * o.abs()
+      out[q0:q0 + lq, h] = o
+      tout[q0:q0 + lq, h] += to
+      if dout is None:
+        continue
+      e = dout[q0:q0 + lq, h]
+      dp = e @ c.t()
+      delta = (e * o).sum(-1, keepdim=True)
+      ds = p * (dp - delta)
+      # dP is a fp32 sum of Dv products; delta meets the rounded out; dS is rounded once
+      tds = (HB + rp) * ds.abs() + p * ((e.abs() * to).sum(-1, keepdim=True) +
+                                        (v.shape[2] * HF + rp) * (e.abs() @ c.abs().t()))
+      res["dv"][0][k0:k0 + lk, h // g] += p.t() @ e
+      res["dv"][1][k0:k0 + lk, h // g] += (HB + rp) * (p.t() @ e.abs())
+      res["dq"][0][q0:q0 + lq, h] += ds @ b * scale
+      res["dq"][1][q0:q0 + lq, h] += tds @ b.abs() * scale
+      res["dk"][0][k0:k0 + lk, h // g] += ds.t() @ a * scale
+      res["dk"][1][k0:k0 + lk, h // g] += tds.t() @ a.abs() * scale
+  if dout is not None:
+    for name in ("dq", "dk", "dv"):
+      want, tol = res[name]
+      # the result's own rounding, and the fp32 sums behind the bf16 products
+      res[name] = (want, tol * (1 + 2.0 ** -6) + HB * want.abs() + 1e-30)
+  return res
+
+
+def run_attention(K, Fn, q_lengths, k_lengths, heads, kv_heads, d, dv, causal, grad, seed=0, q_starts=None, k_starts=None,
+                  scale=None, spread=1.0, rows=None):
+  gen = torch.Generator().manual_seed(seed)
+  plan = K.AttentionPlan(q_lengths, k_lengths, heads=heads, kv_heads=kv_heads, causal=causal, q_starts=q_starts,
+                         k_starts=k_starts)
+  kl = list(q_lengths) if k_lengths is None else list(k_lengths)
+  q0 = list(q_starts) if q_starts else [sum(q_lengths[:i]) for i in range(len(q_lengths))]
+  k0 = list(k_starts) if k_starts else [sum(kl[:i]) for i in range(len(kl))]
+  nq, nk = rows or (plan.q_rows, plan.k_rows)
+  q = (spread * normal(gen, (nq, heads, d))).cuda().requires_grad_(grad)
+  k = (spread * normal(gen, (nk, kv_heads, d))).cuda().requires_grad_(grad)
+  v = normal(gen, (nk, kv_heads, dv)).cuda().requires_grad_(grad)
+  dout = normal(gen, (nq, heads, dv)).cuda() if grad else None
+  out = Fn.packed_attention(q, k, v, plan, scale)
+  got = {"out": out}
+  if grad:
+    got["dq"], got["dk"], got["dv"] = torch.autograd.grad(out, (q, k, v), dout)
+  want = exact_attention(q.detach(), k.detach(), v.detach(), dout, list(zip(q0, q_lengths, k0, kl)), heads, kv_heads,
+                         causal, 1.0 / math.sqrt(d) if scale is None else scale)
+  for name, (value, tol) in want.items():
+    within(got[name], value, tol, name)
+  return got, (q, k, v, dout, plan)
+
+
+ATTENTION = [
+    # q_lengths, k_lengths, heads, kv_heads, D, Dv, causal
+    ([1], None, 1, 1, 8, 8, False),
+    ([1], [1], 4, 1, 64, 64, True),
+    ([1], [2], 40, 1, 128, 128, True),
+    ([16] * 9, None, 3, 3, 64, 64, False),
+    ([32], [33], 1, 1, 32, 32, False),
+    ([33], [32], 1, 1, 32, 32, True),
+    ([64, 1, 0, 63, 65], None, 4, 2, 64, 64, True),
+    ([127, 129, 128], None, 2, 1, 128, 128, True),
+    ([127, 129, 128], None, 2, 1, 128, 128, False),
+    ([100], [40], 3, 1, 96, 64, True),              # rows in front of the keys see nothing
+    ([40], [300], 6, 2, 64, 128, True),
+    ([5, 0, 7, 9], [0, 6, 200, 1], 5, 5, 40, 72, False),
+    ([300, 257], None, 5, 1, 8, 120, True),
+    ([513], None, 2, 2, 104, 104, False),
+    ([1000], [1100], 1, 1, 128, 128, True),
+    ([7], [1900], 3, 1, 64, 64, True),
+]
+
+
+@pytest.mark.parametrize("case", ATTENTION, ids=[str(i) for i in range(len(ATTENTION))])
+def test_packed_attention(K, Fn, case):
+  run_attention(K, Fn, *case, grad=True, seed=len(case[0]) + case[4])
+
+
+NEW_TOKENS = [
+    # k_lengths, heads, kv_heads, D, Dv, capacity
+    ([1, 513, 0, 4097], 8, 2, 128, 128, 5000),
+    ([129, 128], 32, 1, 64, 64, 129),
+    ([20000], 8, 8, 128, 128, 20000),
+    ([9001, 3], 12, 4, 96, 32, 9001),
+    ([70000], 1, 1, 32, 32, 70000),
+    ([3001], 66, 2, 64, 64, 3001),                  # 33 shared heads: more than one wave's rows
+]
+
+
+@pytest.mark.parametrize("case", NEW_TOKENS, ids=[str(i) for i in range(len(NEW_TOKENS))])
+def test_new_tokens_against_a_cache(K, Fn, case):
+  k, heads, kv_heads, d, dv, capacity = case
+  n = len(k)
+  run_attention(K, Fn, [1] * n, k, heads, kv_heads, d, dv, True, False, k_starts=[i * capacity for i in range(n)],
+                rows=(n, n * capacity))
+
+
+def test_split_over_keys_with_many_rows(K, Fn):
+  """Few tiles of 128 rows against many keys: partial results joined; with gradients."""
+  run_attention(K, Fn, [70], [5000], 2, 1, 64, 64, True, True)
+  run_attention(K, Fn, [300, 3], [3000, 2000], 1, 1, 128, 96, False, True)
+
+
+@pytest.mark.parametrize("spread", [0.0, 8.0])
+def test_flat_and_sharp_scores(K, Fn, spread):
+  """All scores equal, and scores so far apart that the reference exponent is raised again and again."""
+  run_attention(K, Fn, [150], [400], 2, 2, 64, 64, False, spread == 0.0, spread=spread)
+
+
+def test_scale(K, Fn):
+  run_attention(K, Fn, [90], None, 2, 1, 32, 32, True, True, scale=0.7)
+  run_attention(K, Fn, [90], None, 2, 1, 32, 32, True, True, scale=1e-3)
+
+
+def test_rising_scores_raise_the_reference(K, Fn):
+  """Every tile's maximum passes the last one's by far: the accumulators are rescaled in every tile."""
+  d, n = 64, 512
+  k = torch.zeros(n, 1, d)
+  k[:, 0, 0] = torch.arange(n) / 4.0
+  q = torch.zeros(130, 1, d)
+  q[:, 0, 0] = torch.linspace(-8, 8, 130)
+  v = normal(torch.Generator().manual_seed(1), (n, 1, d))
+  q, k = q.bfloat16(), k.bfloat16()
+  plan = K.AttentionPlan([130], [n], heads=1)
+  got = Fn.packed_attention(q.cuda(), k.cuda(), v.cuda(), plan, 1.0)
+  want = exact_attention(q, k, v, None, [(0, 130, 0, n)], 1, 1, False, 1.0)["out"]
+  within(got, want[0], want[1], "out")
+
+
+def test_padded_batch_and_rows_of_nobody(K, Fn):
+  """Starts with room between the sequences, filled with NaN: nothing of it is read into a result; rows of nobody
+  give zeros and get zero gradients, and keep what a given output holds."""
+  cap, lens, heads = 96, [50, 0, 96, 7], 2
+  starts = [i * cap for i in range(4)]
+  plan = K.AttentionPlan(lens, heads=heads, causal=True, q_starts=starts, k_starts=starts)
+  gen = torch.Generator().manual_seed(3)
+  rows = 4 * cap + 5
+  mine = torch.zeros(rows, dtype=torch.bool)
+  for s, n in zip(starts, lens):
+    mine[s:s + n] = True
+  data = []
+  for _ in range(4):
+    x = normal(gen, (rows, heads, 64))
+    x[~mine] = float("nan")
+    data.append(x.cuda())
+  q, k, v, dout = data
+  for x in (q, k, v):
+    x.requires_grad_(True)
+  out = Fn.packed_attention(q, k, v, plan)
+  got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), dout)), out=out)
+  clean = [x.detach().nan_to_num(0.0) for x in data]
+  want = exact_attention(*clean, list(zip(starts, lens, starts, lens)), heads, heads, True, 0.125)
+  for name, (value, tol) in want.items():
+    within(got[name], value, tol, name)
+    assert torch.equal(got[name][~mine], torch.zeros_like(got[name][~mine]))
+  kept = torch.full((rows, heads, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+  K.packed_attention_fwd(q.detach(), k.detach(), v.detach(), plan, out=kept)
+  assert torch.equal(kept[~mine], torch.full_like(kept[~mine], 3.0))
+  within(kept[mine], want["out"][0][mine], want["out"][1][mine], "kept")
+
+
+def test_strided_and_merged_inputs(K, Fn):
+  """q, k, v as views of one projection, broadcast heads, odd strides (copied), gradients of the views."""
+  gen = torch.Generator().manual_seed(4)
+  lens, seqs = [70, 33], [(0, 70, 0, 70), (70, 33, 70, 33)]
+  plan = K.AttentionPlan(lens, heads=4, kv_heads=2, causal=True)
+  merged = normal(gen, (103, 8, 64)).cuda().requires_grad_(True)
+  q, k, v = merged[:, :4], merged[:, 4:6], merged[:, 6:]
+  dout = normal(gen, (103, 4, 64)).cuda()
+  out = Fn.packed_attention(q, k, v, plan)
+  (dm,) = torch.autograd.grad(out, (merged,), dout)
+  want = exact_attention(q.detach(), k.detach(), v.detach(), dout, seqs, 4, 2, True, 0.125)
+  within(out, *want["out"], "out")
+  for name, got in (("dq", dm[:, :4]), ("dk", dm[:, 4:6]), ("dv", dm[:, 6:])):
+    within(got, *want[name], name)
+  # one key head shown to all by a stride of zero, odd row strides, a transposed width
+  one = normal(gen, (103, 1, 64)).cuda()
+  odd = normal(gen, (103, 4, 67)).cuda()[..., 1:65]
+  turned = normal(gen, (103, 64, 2)).cuda().transpose(1, 2)
+  out = Fn.packed_attention(odd, one.expand(103, 2, 64), turned, plan)
+  want = exact_attention(odd, one.expand(103, 2, 64), turned, None, seqs, 4, 2, True, 0.125)
+  within(out, *want["out"], "strided")
+
+
+def test_no_keys_at_all(K, Fn):
+  plan = K.AttentionPlan([3, 2], [0, 0], heads=2)
+  q = torch.ones((5, 2, 16), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+  k = torch.ones((0, 2, 16), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+  out = Fn.packed_attention(q, k, k, plan)
+  assert torch.equal(out, torch.zeros_like(out))
+  dq, dk = torch.autograd.grad(out, (q, k), torch.ones_like(out))
+  assert torch.equal(dq, torch.zeros_like(dq)) and dk.shape == k.shape
+  plan = K.AttentionPlan([0], [4], heads=2)
+  q0 = torch.ones((0, 2, 16), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+  k4 = torch.ones((4, 2, 16), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+  out = Fn.packed_attention(q0, k4, k4, plan)
+  dk = torch.autograd.grad(out, (k4,), torch.ones_like(out))[0]
+  assert out.shape == (0, 2, 16) and torch.equal(dk, torch.zeros_like(dk))
+
+
+def test_statistics_of_rows(K):
+  gen = torch.Generator().manual_seed(6)
+  q, k = normal(gen, (40, 1, 32)), normal(gen, (20, 1, 32))
+  plan = K.AttentionPlan([40], [20], causal=True)
+  out, lse = K.packed_attention_fwd(q.cuda(), k.cuda(), k.cuda(), plan)
+  s = q[:, 0].double() @ k[:, 0].double().t() / math.sqrt(32)
+  s = s.masked_fill(torch.arange(20)[None] > torch.arange(40)[:, None] - 20, -math.inf)
+  want = torch.logsumexp(s, -1)
+  assert (lse[:20, 0] == -math.inf).all() and (out[:20] == 0).all()
+  assert ((lse[20:, 0].cpu() - want[20:]).abs() < 1e-5).all()
+  assert K.packed_attention_fwd(q.cuda(), k.cuda(), k.cuda(), plan, want_lse=False)[1] is None
+
+
+def test_infinite_and_missing_values_stay_in_their_rows(K, Fn):
+  """A NaN in a query, and an infinite one, reach that row only; NaN in a key's row reach every row that sees it."""
+  gen = torch.Generator().manual_seed(7)
+  q, k, v = (normal(gen, (200, 1, 64)).cuda() for _ in range(3))
+  plan = K.AttentionPlan([200])
+  clean = Fn.packed_attention(q, k, v, plan)
+  q[17, 0, 3] = float("nan")
+  q[90, 0, 5] = float("inf")
+  got = Fn.packed_attention(q, k, v, plan)
+  rest = torch.ones(200, dtype=torch.bool)
+  rest[[17, 90]] = False
+  assert torch.equal(got[rest], clean[rest])
+  assert got[17].isnan().all() and got[90].isnan().all()
+  k[3, 0, 0] = float("nan")
+  assert Fn.packed_attention(q, k, v, plan).isnan().all()
+
+
+def test_same_result_every_time(K, Fn):
+  """No atomics: two runs agree to the bit, alone and with another stream's call in between."""
+  gen = torch.Generator().manual_seed(8)
+  q, k, v = (normal(gen, (700, h, 64)).cuda().requires_grad_(True) for h in (4, 2, 2))
+  dout = normal(gen, (700, 4, 64)).cuda()
+  plan = K.AttentionPlan([300, 400], heads=4, kv_heads=2, causal=True)
+
+  def once():
+    out = Fn.packed_attention(q, k, v, plan)
+    return (out.detach(),) + torch.autograd.grad(out, (q, k, v), dout)
+  first = once()
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    other = once()
+  second = once()
+  torch.cuda.synchronize()
+  for a, b, c in zip(first, second, other):
+    assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_gradients_against_differences(K, Fn):
+  """d/de of sum(dout * out) along a random direction, taken from the kernels' own outputs at q, k, v +- e dir."""
+  gen = torch.Generator().manual_seed(9)
+  lens, heads, kv_heads, d = [60, 45], 4, 2, 64
+  plan = K.AttentionPlan(lens, heads=heads, kv_heads=kv_heads, causal=True)
+  n = sum(lens)
+  q, k, v = (normal(gen, (n, h, d)).cuda().requires_grad_(True) for h in (heads, kv_heads, kv_heads))
+  dout = normal(gen, (n, heads, d)).cuda()
+  grads = torch.autograd.grad(Fn.packed_attention(q, k, v, plan), (q, k, v), dout)
+  for i, x in enumerate((q, k, v)):
+    # along the gradient itself: the derivative is large against the rounding of the outputs
+    step = 0.5 * grads[i].float() / grads[i].float().abs().max()
+    up, down = ((x.detach().float() + s * step).bfloat16() for s in (1, -1))
+    args = [[y.detach() for y in (q, k, v)] for _ in range(2)]
+    args[0][i], args[1][i] = up, down
+    a, b = (Fn.packed_attention(*xs, plan).double() for xs in args)
+    change = float((dout.double() * (a - b)).sum())
+    want = float((grads[i].double() * (up.double() - down.double())).sum())
+    # third derivative: a step of at most 1/2 in values of size 1, softmax slopes of size 1: a few percent
+    assert abs(change - want) <= 0.05 * abs(want), (i, change, want)
+
+
+def test_attention_refusals(K, Fn):
+  plan = K.AttentionPlan([4], heads=2, kv_heads=1)
+  z = lambda *s, **kw: torch.zeros(s, dtype=kw.get("dtype", torch.bfloat16), device="cuda")
+  good = dict(q=z(4, 2, 16), k=z(4, 1, 16), v=z(4, 1, 24), plan=plan)
+  assert Fn.packed_attention(**good).shape == (4, 2, 24)
+  for bad in (dict(q=z(4, 2, 16, dtype=torch.float32)), dict(k=z(4, 1, 16, dtype=torch.half)), dict(q=z(4, 1, 16)),
+              dict(k=z(4, 2, 16)), dict(k=z(4, 1, 24)), dict(v=z(5, 1, 24)), dict(q=z(3, 2, 16)),
+              dict(k=z(3, 1, 16), v=z(3, 1, 16)), dict(q=z(4, 2, 12), k=z(4, 1, 12)), dict(v=z(4, 1, 136)),
+              dict(q=z(4, 32)), dict(plan=None), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+              dict(plan=K.AttentionPlan([4], heads=2, kv_heads=1, device="cpu")), dict(v=z(4, 1, 24).cpu())):
+    with pytest.raises(ValueError):
+      Fn.packed_attention(**dict(good, **bad))
+  with pytest.raises(ValueError):
+    K.packed_attention_fwd(out=z(4, 2, 16), **good)
+  out, lse = K.packed_attention_fwd(**good)
+  with pytest.raises(ValueError):
+    K.packed_attention_bwd(good["q"], good["k"], good["v"], plan, out, lse, z(4, 2, 16))
+  with pytest.raises(ValueError):
+    K.packed_attention_bwd(good["q"], good["k"], good["v"], plan, out, None, out)
+  q = z(4, 2, 16).requires_grad_(True)                # no second derivative: refused, not wrong
+  out = Fn.packed_attention(q, good["k"], good["v"], plan)
+  (dq,) = torch.autograd.grad(out.float().sum(), (q,), create_graph=True)
+  with pytest.raises(RuntimeError):
+    dq.float().sum().backward()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_drawn_sequences(K, Fn, seed):
+  rng = random.Random(seed)
+  n = rng.randint(1, 6)
+  q = [rng.choice((0, 1, 2, 31, 32, 33, 64, rng.randint(1, 400))) for _ in range(n)]
+  k = None if rng.random() < 0.4 else [rng.choice((0, 1, 63, 64, 65, rng.randint(1, 600))) for _ in range(n)]
+  kv_heads = rng.randint(1, 3)
+  heads = kv_heads * rng.randint(1, 4)
+  if not any(q):
+    q[0] = 1
+  run_attention(K, Fn, q, k, heads, kv_heads, 8 * rng.randint(1, 16), 8 * rng.randint(1, 16), rng.random() < 0.5, True,
+                seed=seed)
+
+
+# ------------------------------------------------------------------------------------------------
+# together
+# ------------------------------------------------------------------------------------------------
+def test_block_of_the_three(K, Fn):
+  """Projection rows -> norm + rotation -> attention, with gradients back to the projection and the gains, against
+  the chain in 64 bits; relative error of whole tensors (each stage rounds to bf16: three roundings of half a step
+  2^-8 each, uncorrelated over the sums)."""
+  gen = torch.Generator().manual_seed(11)
+  lens, heads, kv_heads, d = [64, 100, 1, 37], 4, 2, 64
+  n = sum(lens)
+  merged = normal(gen, (n, heads + 2 * kv_heads, d)).cuda().requires_grad_(True)
+  qg, kg = ((1 + 0.2 * normal(gen, (d,), torch.float32)).cuda().requires_grad_(True) for _ in range(2))
+  pos = torch.cat([torch.arange(x) for x in lens]).int().cuda()
+  table = K.RotaryTable(d)
+  plan = K.AttentionPlan(lens, heads=heads, kv_heads=kv_heads, causal=True)
+  q, k = Fn.qk_norm_rotary(merged[:, :heads], merged[:, heads:heads + kv_heads], qg, kg, pos, table)
+  out = Fn.packed_attention(q, k, merged[:, heads + kv_heads:], plan)
+  dout = normal(gen, out.shape).cuda()
+  got = (out,) + torch.autograd.grad(out, (merged, qg, kg), dout)
+  m = merged.detach().double().cpu().requires_grad_(True)
+  a, b = (x.detach().double().cpu().requires_grad_(True) for x in (qg, kg))
+  f = table.freq.cpu() * 2 * math.pi
+  angle = (pos.cpu().double()[:, None] * f)[:, None]
+  cos, sin = torch.cos(angle), torch.sin(angle)
+
+  def turn(x):
+    y, z = x[..., :d // 2], x[..., d // 2:]
+    return torch.cat((y * cos - z * sin, y * sin + z * cos), -1)
+  qq = turn(exact_norm(m[:, :heads], a, 1e-6))
+  kk = turn(exact_norm(m[:, heads:heads + kv_heads], b, 1e-6))
+  vv = m[:, heads + kv_heads:]
+  outs, at = [], 0
+  for x in lens:
+    part = []
+    for h in range(heads):
+      s = qq[at:at + x, h] @ kk[at:at + x, h // 2].t() / 8.0
+      s = s.masked_fill(torch.ones(x, x, dtype=torch.bool).triu(1), -math.inf)
+      part.append(torch.softmax(s, -1) @ vv[at:at + x, h // 2])
+    outs.append(torch.stack(part, 1))
+    at += x
+  o = torch.cat(outs)
+  want = (o,) + torch.autograd.grad(o, (m, a, b), dout.double().cpu())
+  for name, x, y in zip(("out", "dmerged", "dq_gain", "dk_gain"), got, want):
+    x, y = x.detach().double().cpu(), y.detach()
+    assert float((x - y).norm() / y.norm()) <= 3 * HB, name
+
+
+def test_captured_and_replayed(K, Fn):
+  """Forward and backward of the three in one graph (direct calls: no autograd inside the capture), replayed with new
+  inputs and eager work in between."""
+  gen = torch.Generator().manual_seed(12)
+  lens, heads, kv_heads, d = [1, 130, 70], 4, 1, 64
+  n = sum(lens)
+  plan = K.AttentionPlan(lens, [1, 900, 70], heads=heads, kv_heads=kv_heads, causal=True)
+  table = K.RotaryTable(d)
+  pos = torch.arange(n, dtype=torch.int32, device="cuda")
+  gain = torch.ones(d, device="cuda")
+  q, k = normal(gen, (n, heads, d)).cuda(), normal(gen, (n, kv_heads, d)).cuda()
+  cache_k, cache_v = (normal(gen, (971, kv_heads, d)).cuda() for _ in range(2))
+  dout = normal(gen, (n, heads, d)).cuda()
+
+  def step():
+    a, b = K.qk_norm_rotary(q, k, gain, gain, pos, table)
+    out, lse = K.packed_attention_fwd(a, cache_k, cache_v, plan)
+    grads = K.packed_attention_bwd(a, cache_k, cache_v, plan, out, lse, dout)
+    back = K.qk_norm_rotary_bwd(q, k, gain, gain, pos, table, grads[0], b)
+    return (out, K.rotary(b, pos, table)) + grads + back
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    step()
+  torch.cuda.current_stream().wait_stream(side)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    held = step()
+  for i in range(4):
+    q.copy_(normal(gen, q.shape))
+    cache_k.copy_(normal(gen, cache_k.shape))
+    want = [x.clone() for x in step()]
+    graph.replay()
+    torch.cuda.synchronize()
+    for x, y in zip(held, want):
+      assert torch.equal(x, y), i
