@@ -267,6 +267,19 @@ __device__ __forceinline__ void mha_token(const MhaArgs& a, const MhaItem& it, i
   *h = it.hk * a.G + (r - *t * a.G);
 }
 
+// a lane's row of an accumulator, fp32, to a partial result
+template <int DP>
+__device__ __forceinline__ void mha_store_part(float* dst, const f32x16_t (&o)[DP / 32], int width, int half) {
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = t * 32 + g * 8 + 4 * half;
+      if (d < width)
+        *reinterpret_cast<float4*>(dst + d) = make_float4(o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]);
+    }
+}
+
 // what a wave leaves behind: O^T in registers -> out, or a partial result
 template <int DP>
 __device__ __forceinline__ void mha_store(const MhaArgs& a, const MhaItem& it, int r, float m, float l,
@@ -274,15 +287,7 @@ __device__ __forceinline__ void mha_store(const MhaArgs& a, const MhaItem& it, i
   if (r >= it.rows) return;
   if (it.part >= 0) {
     const int64_t at = (int64_t)it.part * THIN_ROWS + (r - it.row0);
-    float* dst = a.ws_o + at * a.Dv;
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = t * 32 + g * 8 + 4 * half;
-        if (d < a.Dv)
-          *reinterpret_cast<float4*>(dst + d) = make_float4(o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]);
-      }
+    mha_store_part<DP>(a.ws_o + at * a.Dv, o, a.Dv, half);
     if (half == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m, l);
     return;
   }
@@ -587,7 +592,7 @@ __global__ __launch_bounds__(256, 2) void mha_bwd_q_kernel(MhaArgs a) {
     if (k0 + KT < it.k1) stage(k0 + KT, buf ^ 1);
     if (k0 > most) continue;
     mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
-#pragma unroll
+#pragma unroll 1
     for (int n = 0; n < 2; ++n) {
       f32x16_t s = mha_product<DP>(ks, rd, qf, n);
       const f32x16_t dp = mha_product<DP>(vs, rd, df, n);
@@ -603,6 +608,10 @@ __global__ __launch_bounds__(256, 2) void mha_bwd_q_kernel(MhaArgs a) {
     }
   }
   if (!ok) return;
+  if (it.part >= 0) {
+    mha_store_part<DP>(a.ws_o + ((int64_t)it.part * ROW_TILE + r - it.row0) * a.D, dq, a.D, half);
+    return;
+  }
   bf16_t* dst = a.dq + row * a.D;
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i)
@@ -619,7 +628,7 @@ __global__ __launch_bounds__(256, 2) void mha_bwd_q_kernel(MhaArgs a) {
 // dK, dV: 128 keys x the rows that see them.  S[row][key] = Q K^T and dP = dO V^T with the keys in the lanes'
 // columns; dV^T += dO^T P, dK^T += Q^T dS.  Item {seq, hk, key0, first row, end row}.
 template <int DP>
-__global__ __launch_bounds__(256, 1) void mha_bwd_kv_kernel(MhaArgs a) {
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaArgs a) {
   constexpr int TILE = KT * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
   __shared__ __attribute__((aligned(16))) float stat[2][2][KT];   // [buffer][lse, delta][row]
@@ -693,7 +702,7 @@ __global__ __launch_bounds__(256, 1) void mha_bwd_kv_kernel(MhaArgs a) {
     }
     if (!some) continue;
     mha_lds_ptr qs = sm + buf * 2 * TILE, ds = qs + TILE;
-#pragma unroll
+#pragma unroll 1
     for (int n = 0; n < 2; ++n) {
       const int rs = r0 + n * 32;
       if (rs + 31 < wave_first || rs >= re) continue;
@@ -724,6 +733,12 @@ __global__ __launch_bounds__(256, 1) void mha_bwd_kv_kernel(MhaArgs a) {
     }
   }
   if (!ok) return;
+  if (it.part >= 0) {
+    float* dst = a.ws_o + ((int64_t)it.part * KEY_TILE + key - it.row0) * (a.D + a.Dv);
+    mha_store_part<DP>(dst, dk, a.D, half);
+    mha_store_part<DP>(dst + a.D, dv, a.Dv, half);
+    return;
+  }
   bf16_t* dkp = a.dk + ((int64_t)(it.k_start + key) * a.kv_heads + it.hk) * a.D;
   bf16_t* dvp = a.dv + ((int64_t)(it.k_start + key) * a.kv_heads + it.hk) * a.Dv;
 #pragma unroll
@@ -736,6 +751,153 @@ __global__ __launch_bounds__(256, 1) void mha_bwd_kv_kernel(MhaArgs a) {
       if (d < a.D) *reinterpret_cast<uint2*>(dkp + d) = pack4_bf16(w);
       if (d < a.Dv) *reinterpret_cast<uint2*>(dvp + d) = pack4_bf16(u);
     }
+}
+
+// sums the partial gradients of a split item in their order: item {seq, hk, row0, rows here, parts, first part},
+// partial results [part][128][width]; dq: width D; dk and dv: D + Dv, the first D scaled
+template <bool KEYS>
+__global__ __launch_bounds__(256) void mha_join_grad_kernel(MhaArgs a) {
+  const MhaItem it = mha_item(a, blockIdx.x);
+  const int width = KEYS ? a.D + a.Dv : a.D, quads = width / 4;
+  const int64_t step = (int64_t)ROW_TILE * width;
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < it.k0 * quads; i += gridDim.y * 256) {
+    const int n = i / quads, d = (i - n * quads) * 4;
+    const float* src = a.ws_o + ((int64_t)it.part * ROW_TILE + n) * width + d;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < it.k1; ++p) {
+      const float4 x = *reinterpret_cast<const float4*>(src + p * step);
+      sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+    }
+    const float f = d < a.D ? a.scale : 1.f;
+    const float w[4] = {sum.x * f, sum.y * f, sum.z * f, sum.w * f};
+    bf16_t* dst;
+    if (KEYS) {
+      const int64_t row = (int64_t)(it.k_start + it.row0 + n) * a.kv_heads + it.hk;
+      dst = d < a.D ? a.dk + row * a.D + d : a.dv + row * a.Dv + (d - a.D);
+    } else {
+      int t, h;
+      mha_token(a, it, it.row0 + n, &t, &h);
+      dst = a.dq + ((int64_t)(it.q_start + t) * a.heads + h) * a.D + d;
+    }
+    *reinterpret_cast<uint2*>(dst) = pack4_bf16(w);
+  }
+}
+
+// All gradients of a sequence with at most 32 rows and 32 keys: one wave a key head, nothing but its own Q, K, V
+// and dO read.  The scores are formed both ways round (S^T for dQ, S for dK and dV); the softmax statistics and
+// delta = sum_k P dP come from the scores themselves, exact in fp32, and reach the other orientation by lane
+// exchanges.  Bound by latency: a launch of one wave workgroups, many a CU.
+template <int DP>
+__global__ __launch_bounds__(64) void mha_bwd_small_kernel(MhaArgs a) {
+  constexpr int TILE = 32 * DP * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[3 * TILE];   // K, Q, dO
+  const int lane = threadIdx.x, half = lane >> 5, col = lane & 31;
+  const MhaItem it = mha_item(a, blockIdx.x);
+  using Stage = MhaStage<DP, 32, 1>;
+  const MhaReads<DP> rd = mha_reads<DP>(lane);
+  const uint32_t lds = cg_lds_addr(smem);
+  mha_lds_ptr ks = (mha_lds_ptr)smem, qs = ks + TILE, ds = ks + 2 * TILE;
+  const int64_t dt = (int64_t)a.heads * a.Dv;
+  {
+    uint32_t koff[Stage::N];
+    mha_offsets<DP, 32, 1>(koff, 0, lane, a.kt, a.D);
+    mha_copy<DP, 32, 1>(koff, mha_rows<32>(a.k + (int64_t)it.hk * a.kh, it.k_start, it.Lk, a.kt, a.D), lds, 0);
+    const cg_i32x4_t qr = cg_make_rsrc(a.q + (int64_t)it.hk * a.G * a.qh + (int64_t)it.q_start * a.qt, 0x7fffffffu);
+    const cg_i32x4_t dr = cg_make_rsrc(a.dout + (int64_t)it.hk * a.G * a.Dv + (int64_t)it.q_start * dt, 0x7fffffffu);
+#pragma unroll
+    for (int n = 0; n < Stage::N; ++n) {
+      int r, c;
+      Stage::place(n, 0, lane, &r, &c);
+      const int t = (int)fdiv((uint32_t)r, a.dG), g = r - t * a.G;
+      // rows that see no key are left out: their dO may hold anything
+      const bool in = r < it.rows && t + it.shift >= 0;
+      cg_dma16_asm(qr, in && c < a.D ? (uint32_t)t * (uint32_t)(a.qt * 2) + (uint32_t)g * (uint32_t)(a.qh * 2) + c * 2 : OUTSIDE, 0u, lds + TILE + n * 1024u);
+      cg_dma16_asm(dr, in && c < a.Dv ? (uint32_t)t * (uint32_t)(dt * 2) + (uint32_t)g * (uint32_t)(a.Dv * 2) + c * 2 : OUTSIDE, 0u, lds + 2 * TILE + n * 1024u);
+    }
+  }
+  int t, h;
+  mha_token(a, it, col, &t, &h);
+  const bool row_ok = col < it.rows, key_ok = col < it.Lk;
+  bf16x8_t vf[DP / 16];
+  mha_row_frags(vf, a.v + (int64_t)(it.k_start + col) * a.vt + (int64_t)it.hk * a.vh, key_ok, a.Dv, half);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  bf16x8_t kf[DP / 16], qf[DP / 16], df[DP / 16];
+#pragma unroll
+  for (int kd = 0; kd < DP / 16; ++kd) {
+    kf[kd] = *(mha_frag_ptr)(ks + rd.row[kd]);
+    qf[kd] = *(mha_frag_ptr)(qs + rd.row[kd]);
+    df[kd] = *(mha_frag_ptr)(ds + rd.row[kd]);
+  }
+  auto product = [&](const bf16x8_t (&x)[DP / 16], const bf16x8_t (&y)[DP / 16]) {
+    f32x16_t s = mha_zero();
+#pragma unroll
+    for (int kd = 0; kd < DP / 16; ++kd) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[kd], y[kd], s, 0, 0, 0);
+    return s;
+  };
+  // rows in the lanes' columns: statistics, delta, dQ
+  f32x16_t s = product(kf, qf);
+  const f32x16_t dp = product(vf, df);
+  const int last = row_ok ? min(it.Lk - 1, t + it.shift) : -1;
+  float m = -INFINITY, l = 0.f, delta = 0.f;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    s[v] = mha_key(v, half) <= last ? s[v] * a.c : -INFINITY;
+    m = fmaxf(m, s[v]);
+  }
+  m = fmaxf(m, __shfl_xor(m, 32, 64));
+  if (m == -INFINITY) m = 0.f;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    s[v] = __builtin_amdgcn_exp2f(s[v] - m);
+    l += s[v];
+  }
+  l += __shfl_xor(l, 32, 64);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    s[v] *= inv;
+    delta += mha_key(v, half) <= last ? s[v] * dp[v] : 0.f;
+  }
+  delta += __shfl_xor(delta, 32, 64);
+#pragma unroll
+  for (int v = 0; v < 16; ++v) s[v] = mha_key(v, half) <= last ? s[v] * (dp[v] - delta) : 0.f;
+  f32x16_t acc[DP / 32];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) acc[i] = mha_zero();
+  };
+  auto store = [&](bf16_t* dst, float f, int width) {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = i * 32 + g * 8 + 4 * half;
+        const float w[4] = {acc[i][4 * g] * f, acc[i][4 * g + 1] * f, acc[i][4 * g + 2] * f, acc[i][4 * g + 3] * f};
+        if (d < width) *reinterpret_cast<uint2*>(dst + d) = pack4_bf16(w);
+      }
+  };
+  clear();
+  mha_accumulate<DP>(acc, ks, rd, s, 0);
+  if (row_ok) store(a.dq + ((int64_t)(it.q_start + t) * a.heads + h) * a.D, a.scale, a.D);
+  // keys in the lanes' columns: dK, dV
+  f32x16_t sk = product(qf, kf);
+  f32x16_t dk = product(df, vf);
+  const int mine = a.causal ? max(0, col - it.shift) * a.G : 0;    // first row that sees this key
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const int r = mha_key(v, half);
+    const float rm = __shfl(m, r, 64), ri = __shfl(inv, r, 64), rdelta = __shfl(delta, r, 64);
+    const bool see = key_ok && r >= mine && r < it.rows;
+    sk[v] = see ? __builtin_amdgcn_exp2f(__builtin_fmaf(sk[v], a.c, -rm)) * ri : 0.f;
+    dk[v] = see ? sk[v] * (dk[v] - rdelta) : 0.f;
+  }
+  const int64_t key = (int64_t)(it.k_start + col) * a.kv_heads + it.hk;
+  clear();
+  mha_accumulate<DP>(acc, ds, rd, sk, 0);
+  if (key_ok) store(a.dv + key * a.Dv, 1.f, a.Dv);
+  clear();
+  mha_accumulate<DP>(acc, qs, rd, dk, 0);
+  if (key_ok) store(a.dk + key * a.D, a.scale, a.D);
 }
 
 // ---- the plan ------------------------------------------------------------------------------------
@@ -792,44 +954,41 @@ void mha_deal(std::vector<Work>* items, int units) {
   }
 }
 
-// Blocks that a launch should have at least: 2 resident a CU, 256 CUs.  A launch with fewer is split over the
-// keys, in parts of no less than SPLIT_MIN keys (a part costs its fp32 result: written and read once).
-constexpr int64_t TILE_BLOCKS = 512, THIN_BLOCKS = 1024;
-constexpr int SPLIT_MIN = 256, THIN_SPLIT_MIN = 512;
+// A launch's items are split along the axis that they sum over (keys; rows for dK and dV) where one item is longer
+// than its share of the launch: the total over so many blocks (2 resident a CU, 256 CUs, a few rounds), but no part
+// below a length at which its fp32 result, written once and read once, is small against its own work.
+constexpr int64_t TILE_BLOCKS = 1024, THIN_BLOCKS = 1024;
+constexpr int TILE_SPLIT_MIN = 512, THIN_SPLIT_MIN = 512, GRAD_SPLIT_MIN = 1024;
 constexpr int THIN1_KEYS = 128;     // up to so many keys one wave does a thin item alone
 
-void mha_split(std::vector<Work>* items, int64_t blocks, int step, int least, int units_a_part, int G,
-               const int32_t* q_len, std::vector<Work>* joins, int64_t* parts) {
+void mha_split(std::vector<Work>* items, int64_t blocks, int step, int least, int tile, int units_a_part,
+               const std::vector<int64_t>& length, std::vector<Work>* joins, int64_t* parts) {
   int64_t all = 0;
-  for (const Work& w : *items) all += (w.v[4] + step - 1) / step;
-  if ((int64_t)items->size() >= blocks || all == 0) return;
-  const int64_t chunk = std::max<int64_t>(least / step, (all + blocks - 1) / blocks);
+  for (const Work& w : *items) all += w.v[4] - w.v[3];
+  const int64_t chunk = std::max<int64_t>(least, (all + blocks - 1) / blocks);
   std::vector<Work> out;
-  for (Work& w : *items) {
-    const int64_t steps = (w.v[4] + step - 1) / step;
-    const int64_t n = (steps + chunk - 1) / chunk;
+  for (const Work& w : *items) {
+    const int64_t len = w.v[4] - w.v[3], steps = (len + step - 1) / step;
+    const int64_t n = (len + chunk / 2) / chunk;
     if (n <= 1) {
       out.push_back(w);
       continue;
     }
     Work j = w;
-    j.v[3] = (int32_t)std::min<int64_t>((int64_t)32 * units_a_part, (int64_t)q_len[w.v[0]] * G - w.v[2]);
+    j.v[3] = (int32_t)std::min<int64_t>(tile, length[w.v[0]] - w.v[2]);
+    j.v[4] = (int32_t)n;
     j.v[5] = (int32_t)*parts;
     j.v[6] = units_a_part;
-    const int32_t end = w.v[4];
-    int32_t made = 0;
+    joins->push_back(j);
     for (int64_t i = 0; i < n; ++i) {
       Work p = w;
-      p.v[3] = (int32_t)(steps * i / n) * step;
-      p.v[4] = (int32_t)std::min<int64_t>(end, steps * (i + 1) / n * step);
+      p.v[3] = w.v[3] + (int32_t)(steps * i / n) * step;
+      p.v[4] = (int32_t)std::min<int64_t>(w.v[4], w.v[3] + steps * (i + 1) / n * step);
       p.v[5] = (int32_t)*parts;
       p.cost = p.v[4] - p.v[3] + 64;
       *parts += units_a_part;
       out.push_back(p);
-      ++made;
     }
-    j.v[4] = made;
-    joins->push_back(j);
   }
   items->swap(out);
 }
@@ -837,12 +996,15 @@ void mha_split(std::vector<Work>* items, int64_t blocks, int step, int least, in
 int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start, const int32_t* k_len,
              int B, int heads, int kv_heads, int causal, int32_t* data, int64_t capacity, cgAttentionPlan* info) {
   const int G = heads / kv_heads;
-  std::vector<Work> tiles, thin4, thin1, joins, dq, dkv;
+  std::vector<Work> tiles, thin4, thin1, joins, dq, dq_joins, dkv, dkv_joins, small;
+  std::vector<int64_t> all_rows(B), all_keys(B);
   cgAttentionPlan p = {};
   for (int b = 0; b < B; ++b) {
     const int64_t Lq = q_len[b], Lk = k_len[b], rows = Lq * G, shift = Lk - Lq;
     if (Lq > 0) p.max_q_row = std::max<int32_t>(p.max_q_row, (int32_t)(q_start[b] + Lq));
     if (Lk > 0) p.max_k_row = std::max<int32_t>(p.max_k_row, (int32_t)(k_start[b] + Lk));
+    all_rows[b] = rows;
+    all_keys[b] = Lk;
     auto keys_of = [&](int64_t end_row) {     // keys that the rows below end_row see
       if (!causal) return Lk;
       return std::min(Lk, std::max<int64_t>(0, (end_row - 1) / G + shift + 1));
@@ -852,9 +1014,13 @@ int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_star
       for (int64_t r = 0; r < rows; r += ROW_TILE) {
         const int64_t keys = keys_of(std::min(rows, r + ROW_TILE));
         Work w = {{b, h, (int32_t)r, 0, (int32_t)keys, -1, 0, 0}, keys + 64, unit};
-        dq.push_back(w);
+        if (rows > 32 || Lk > 32) dq.push_back(w);
         if (rows > THIN_ROWS) tiles.push_back(w);
         else (keys <= THIN1_KEYS ? thin1 : thin4).push_back(w);
+      }
+      if (rows <= 32 && Lk <= 32) {
+        if (rows > 0 || Lk > 0) small.push_back(Work{{b, h, 0, 0, (int32_t)Lk, -1, 0, 0}, 1, unit});
+        continue;
       }
       for (int64_t k = 0; k < Lk; k += KEY_TILE) {
         const int64_t from = causal ? std::min(rows, std::max<int64_t>(0, k - shift) * G) : 0;
@@ -862,12 +1028,14 @@ int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_star
       }
     }
   }
-  int64_t parts = 0;
-  mha_split(&tiles, TILE_BLOCKS, KT, SPLIT_MIN, ROW_TILE / 32, G, q_len, &joins, &parts);
-  mha_split(&thin4, THIN_BLOCKS, 32, THIN_SPLIT_MIN, 1, G, q_len, &joins, &parts);
-  if (parts > 0x7fffffff) CG_FAIL(CG_ERR_UNSUPPORTED, "cg_host_attention_plan: too many partial results");
+  int64_t parts = 0, dq_parts = 0, dkv_parts = 0;
+  mha_split(&tiles, TILE_BLOCKS, KT, TILE_SPLIT_MIN, ROW_TILE, ROW_TILE / 32, all_rows, &joins, &parts);
+  mha_split(&thin4, THIN_BLOCKS, 32, THIN_SPLIT_MIN, THIN_ROWS, 1, all_rows, &joins, &parts);
+  mha_split(&dq, TILE_BLOCKS, KT, GRAD_SPLIT_MIN, ROW_TILE, 1, all_rows, &dq_joins, &dq_parts);
+  mha_split(&dkv, TILE_BLOCKS, KT, GRAD_SPLIT_MIN, KEY_TILE, 1, all_keys, &dkv_joins, &dkv_parts);
+  if (parts > 0x7fffffff || dq_parts > 0x7fffffff || dkv_parts > 0x7fffffff) CG_FAIL(CG_ERR_UNSUPPORTED, "cg_host_attention_plan: too many partial results");
   const int units = B * kv_heads;
-  std::vector<Work>* lists[6] = {&tiles, &thin4, &thin1, &joins, &dq, &dkv};
+  std::vector<Work>* lists[9] = {&tiles, &thin4, &thin1, &joins, &dq, &dq_joins, &dkv, &dkv_joins, &small};
   int64_t ints = 4 * (int64_t)B;
   for (auto* l : lists) ints += 8 * (int64_t)l->size();
   if (ints > 0x7fffffff) CG_FAIL(CG_ERR_UNSUPPORTED, "cg_host_attention_plan: too many work items");
@@ -883,6 +1051,11 @@ int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_star
   p.joins = (int32_t)joins.size();
   p.dq_tiles = (int32_t)dq.size();
   p.dkv_tiles = (int32_t)dkv.size();
+  p.dq_joins = (int32_t)dq_joins.size();
+  p.dkv_joins = (int32_t)dkv_joins.size();
+  p.small = (int32_t)small.size();
+  p.dq_parts = dq_parts;
+  p.dkv_parts = dkv_parts;
   *info = p;
   if (!data) return CG_OK;
   if (capacity < ints) CG_FAIL(CG_ERR_WORKSPACE, "cg_host_attention_plan: %lld ints of %lld", (long long)capacity, (long long)ints);
@@ -892,7 +1065,7 @@ int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_star
   }
   int32_t* at = data + 4 * (int64_t)B;
   for (auto* l : lists) {
-    if (l != &joins) mha_deal(l, units);
+    if (l != &joins && l != &dq_joins && l != &dkv_joins) mha_deal(l, units);
     for (const Work& w : *l) {
       memcpy(at, w.v, sizeof(w.v));
       at += 8;
@@ -944,7 +1117,8 @@ int mha_check(const char* name, const cgAttentionInput* in, const cgAttentionPla
 
 // item lists behind the sequences
 const int4* mha_list(const cgAttentionPlan* p, const int32_t* data, int which) {
-  const int64_t n[6] = {p->tiles, p->thin4, p->thin1, p->joins, p->dq_tiles, p->dkv_tiles};
+  const int64_t n[9] = {p->tiles, p->thin4, p->thin1, p->joins, p->dq_tiles, p->dq_joins, p->dkv_tiles, p->dkv_joins,
+                        p->small};
   int64_t at = 4 * (int64_t)p->sequences;
   for (int i = 0; i < which; ++i) at += 8 * n[i];
   return (const int4*)(data + at);
@@ -967,6 +1141,7 @@ int mha_width(int D, int Dv) { return ((D > Dv ? D : Dv) + 31) / 32 * 32; }
 #define MHA_THIN1(dp) mha_thin_kernel<dp, 1>
 #define MHA_BWD_Q(dp) mha_bwd_q_kernel<dp>
 #define MHA_BWD_KV(dp) mha_bwd_kv_kernel<dp>
+#define MHA_BWD_SMALL(dp) mha_bwd_small_kernel<dp>
 
 extern "C" int cg_host_attention_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start,
                                       const int32_t* k_len, int sequences, int heads, int kv_heads, int causal,
@@ -1038,9 +1213,15 @@ extern "C" int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAtten
   return CG_OK;
 }
 
-extern "C" size_t cg_packed_attention_bwd_workspace_bytes(const cgAttentionPlan* plan, int q_rows) {
-  if (!plan || q_rows < 1) return 0;
-  return (size_t)q_rows * plan->heads * sizeof(float);
+// workspace: delta [q_rows, heads], then the partial results of dq, then (the same memory) of dk and dv
+static int64_t mha_delta_bytes(const cgAttentionPlan* p, int q_rows) {
+  return ((int64_t)q_rows * p->heads * (int64_t)sizeof(float) + 255) / 256 * 256;
+}
+
+extern "C" size_t cg_packed_attention_bwd_workspace_bytes(const cgAttentionPlan* plan, int q_rows, int D, int Dv) {
+  if (!plan || q_rows < 1 || D < 1 || Dv < 1) return 0;
+  const int64_t a = plan->dq_parts * D, b = plan->dkv_parts * (D + Dv);
+  return (size_t)(mha_delta_bytes(plan, q_rows) + (a > b ? a : b) * ROW_TILE * (int64_t)sizeof(float));
 }
 
 extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAttentionPlan* plan, const int32_t* data,
@@ -1052,11 +1233,11 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   if (rc) return rc;
   if (plan->max_q_row > 0) {
     if (!out || !lse || !dout || !dq) CG_FAIL(CG_ERR_BAD_ARG, "%s: null tensor", name);
-    if (!ws || ws_bytes < cg_packed_attention_bwd_workspace_bytes(plan, in->q_rows))
+    if (!ws || ws_bytes < cg_packed_attention_bwd_workspace_bytes(plan, in->q_rows, in->D, in->Dv))
       CG_FAIL(CG_ERR_WORKSPACE, "%s: workspace of %zu bytes", name, ws_bytes);
   }
   if (plan->max_k_row > 0 && (!dk || !dv)) CG_FAIL(CG_ERR_BAD_ARG, "%s: null gradient", name);
-  const void* ptr[5] = {out, dout, dq, dk, dv};
+  const void* ptr[6] = {out, dout, dq, dk, dv, ws};
   for (const void* p : ptr)
     if ((uintptr_t)p % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: tensors have to be 16-byte aligned", name);
   a.o_in = (const bf16_t*)out;
@@ -1066,22 +1247,36 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   a.dk = (bf16_t*)dk;
   a.dv = (bf16_t*)dv;
   a.delta = (const float*)ws;
+  if (plan->max_q_row > 0) a.ws_o = (float*)((char*)ws + mha_delta_bytes(plan, in->q_rows));
   const hipStream_t st = (hipStream_t)stream;
   const int dp = mha_width(in->D, in->Dv);
-  if (plan->max_q_row > 0) {
+  if (plan->dq_tiles) {
     const int64_t rows = (int64_t)in->q_rows * plan->heads;
     if (rows > (int64_t)0x7fffffff * 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: too many rows", name);
     mha_delta_kernel<<<(uint32_t)((rows + 15) / 16), 256, 0, st>>>(a.o_in, a.dout, rows, a.Dv, (float*)ws);
     CG_CHECK_LAUNCH(name);
-  }
-  if (plan->dq_tiles) {
     a.items = mha_list(plan, data, 4);
     MHA_LAUNCH(dp, MHA_BWD_Q, plan->dq_tiles, 256, st, a);
     CG_CHECK_LAUNCH(name);
   }
-  if (plan->dkv_tiles) {
+  if (plan->dq_joins) {
     a.items = mha_list(plan, data, 5);
+    mha_join_grad_kernel<false><<<dim3(plan->dq_joins, 4), 256, 0, st>>>(a);
+    CG_CHECK_LAUNCH(name);
+  }
+  if (plan->dkv_tiles) {
+    a.items = mha_list(plan, data, 6);
     MHA_LAUNCH(dp, MHA_BWD_KV, plan->dkv_tiles, 256, st, a);
+    CG_CHECK_LAUNCH(name);
+  }
+  if (plan->dkv_joins) {
+    a.items = mha_list(plan, data, 7);
+    mha_join_grad_kernel<true><<<dim3(plan->dkv_joins, 4), 256, 0, st>>>(a);
+    CG_CHECK_LAUNCH(name);
+  }
+  if (plan->small) {
+    a.items = mha_list(plan, data, 8);
+    MHA_LAUNCH(dp, MHA_BWD_SMALL, plan->small, 64, st, a);
     CG_CHECK_LAUNCH(name);
   }
   return CG_OK;

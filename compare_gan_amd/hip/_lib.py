@@ -74,9 +74,9 @@ class Rotation(ctypes.Structure):
 
 class AttentionPlanInfo(ctypes.Structure):
     """Mirror of cgAttentionPlan."""
-    _fields_ = [("ints", c_i64), ("parts", c_i64)] + [(n, ctypes.c_int32) for n in (
+    _fields_ = [(n, c_i64) for n in ("ints", "parts", "dq_parts", "dkv_parts")] + [(n, ctypes.c_int32) for n in (
         "sequences", "heads", "kv_heads", "causal", "tiles", "thin4", "thin1", "joins", "dq_tiles",
-        "dkv_tiles", "small", "max_q_row", "max_k_row")]
+        "dq_joins", "dkv_tiles", "dkv_joins", "small", "max_q_row", "max_k_row")]
 
 
 class AttentionInput(ctypes.Structure):
@@ -204,7 +204,7 @@ SIGNATURES = {
     "cg_host_attention_plan": (c_int, [vp, vp, vp, vp, c_int, c_int, c_int, c_int, vp, c_i64, vp]),
     "cg_packed_attention_fwd_workspace_bytes": (c_sz, [vp, c_int]),
     "cg_packed_attention_fwd": (c_int, [vp, vp, vp, vp, vp, vp, c_sz, vp]),
-    "cg_packed_attention_bwd_workspace_bytes": (c_sz, [vp, c_int]),
+    "cg_packed_attention_bwd_workspace_bytes": (c_sz, [vp, c_int, c_int, c_int]),
     "cg_packed_attention_bwd": (c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, c_sz, vp]),
     "cg_gan_loss": (c_int, [c_int, vp, c_int, vp, vp, vp, vp]),
     "cg_softmax_xent_eps": (c_int, [vp, vp, c_int, c_int, c_f32, vp, vp, vp]),

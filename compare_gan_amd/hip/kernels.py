@@ -1423,7 +1423,8 @@ def packed_attention_bwd(q, k, v, plan, out, lse, dout, scale=None):
     dq = _rows_out(q.shape, plan.q_dense, plan.q_rows, q.device)
     dk = _rows_out(k.shape, plan.k_dense, plan.k_rows, q.device)
     dv = _rows_out(v.shape, plan.k_dense, plan.k_rows, q.device)
-    ws = _ws(lib().cg_packed_attention_bwd_workspace_bytes(ctypes.byref(plan.info), q.shape[0]), q)
+    ws = _ws(lib().cg_packed_attention_bwd_workspace_bytes(ctypes.byref(plan.info), q.shape[0], q.shape[2],
+                                                           v.shape[2]), q)
     arg = _attention_struct(q, k, v, scale)
     with torch.cuda.device(q.device):
         check(lib().cg_packed_attention_bwd(ctypes.byref(arg), ctypes.byref(plan.info), _p(plan.data), _p(out),

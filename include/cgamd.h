@@ -599,10 +599,10 @@ int cg_qk_norm_rotary_bwd(const cgHeadRows* q, const cgHeadRows* k, const void* 
  * copies them to the device and hands that copy and `info` to the kernels. */
 typedef struct {
   int64_t ints;                       /* size of the plan in int32 */
-  int64_t parts;                      /* partial results: workspace of the forward pass */
+  int64_t parts, dq_parts, dkv_parts; /* partial results: workspaces of the forward and backward pass */
   int32_t sequences, heads, kv_heads, causal;
   int32_t tiles, thin4, thin1, joins; /* forward work items of each form */
-  int32_t dq_tiles, dkv_tiles, small; /* backward work items of each form */
+  int32_t dq_tiles, dq_joins, dkv_tiles, dkv_joins, small;   /* backward work items of each form */
   int32_t max_q_row, max_k_row;       /* rows that the tensors must have at least */
 } cgAttentionPlan;
 int cg_host_attention_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start,
@@ -624,7 +624,7 @@ int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAttentionPlan* p
 /* Gradients: out, lse of the forward pass, dout [q_rows, heads, Dv] contiguous; dq [q_rows, heads, D],
  * dk [k_rows, kv_heads, D], dv [k_rows, kv_heads, Dv] contiguous bf16, every row of a sequence written
  * (the shared heads of a key head summed inside, no atomics). */
-size_t cg_packed_attention_bwd_workspace_bytes(const cgAttentionPlan* plan, int q_rows);
+size_t cg_packed_attention_bwd_workspace_bytes(const cgAttentionPlan* plan, int q_rows, int D, int Dv);
 int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAttentionPlan* plan, const int32_t* data,
                             const void* out, const float* lse, const void* dout, void* dq, void* dk,
                             void* dv, void* ws, size_t ws_bytes, cgStream stream);

@@ -59,7 +59,7 @@ def _lists(plan):
   i = plan.info
   at = 4 * i.sequences
   out = {"seqs": plan.host[:at].reshape(-1, 4)}
-  for name in ("tiles", "thin4", "thin1", "joins", "dq_tiles", "dkv_tiles"):
+  for name in ("tiles", "thin4", "thin1", "joins", "dq_tiles", "dq_joins", "dkv_tiles", "dkv_joins", "small"):
     n = getattr(i, name)
     out[name] = plan.host[at:at + 8 * n].reshape(n, 8)
     at += 8 * n
@@ -122,18 +122,43 @@ def test_plan_covers_every_row_and_key_once(case):
           assert rows == min(tile, n * g - r) and units == tile // 32
           assert [x[2] for x in got] == [unit + i * units for i in range(parts)]
   assert not pieces and not joins
-  dq = sorted((b, h, r, k1) for b, h, r, _, k1, _, _, _ in p["dq_tiles"].tolist())
-  assert dq == sorted((b, h, r, seen(b, (min(r + 128, n * g) - 1) // g)) for b, n in enumerate(q)
-                      for h in range(kv_heads) for r in range(0, n * g, 128))
-  want = []
-  for b, n in enumerate(kk):
+  # gradients: sequences that fit one wave as a whole, the others in tiles whose parts follow one another
+  alone = sorted((b, h) for b, h, _, _, k1, _, _, _ in p["small"].tolist())
+  fits = lambda b: q[b] * g <= 32 and kk[b] <= 32
+  assert alone == sorted((b, h) for b in range(len(q)) for h in range(kv_heads) if fits(b) and (q[b] or kk[b]))
+  want_q, want_k = {}, {}
+  for b in range(len(q)):
     for h in range(kv_heads):
-      for key in range(0, n, 128):
+      if fits(b):
+        continue
+      for r in range(0, q[b] * g, 128):
+        want_q[(b, h, r)] = (0, seen(b, (min(r + 128, q[b] * g) - 1) // g), min(128, q[b] * g - r))
+      for key in range(0, kk[b], 128):
         first = 0
         while first < q[b] and seen(b, first) <= key:
           first += 1
-        want.append((b, h, key, first * g, q[b] * g))
-  assert sorted((b, h, r, a, e) for b, h, r, a, e, _, _, _ in p["dkv_tiles"].tolist()) == sorted(want)
+        want_k[(b, h, key)] = (first * g, q[b] * g, min(128, kk[b] - key))
+  for tiles, joins, want, total in (("dq_tiles", "dq_joins", want_q, plan.info.dq_parts),
+                                    ("dkv_tiles", "dkv_joins", want_k, plan.info.dkv_parts)):
+    pieces, joined = {}, {}
+    for b, h, at, x0, x1, part, _, _ in p[tiles].tolist():
+      pieces.setdefault((b, h, at), []).append((x0, x1, part))
+    for b, h, at, n, parts, first, _, _ in p[joins].tolist():
+      joined[(b, h, at)] = (n, parts, first)
+    assert sorted(pieces) == sorted(want)
+    numbers = []
+    for key, got in pieces.items():
+      got.sort()
+      start, end, n = want[key]
+      assert got[0][0] == start and got[-1][1] == end and all(x[1] == y[0] for x, y in zip(got, got[1:]))
+      if len(got) == 1:
+        assert got[0][2] == -1 and key not in joined
+      else:
+        first = joined[key][2]
+        assert joined.pop(key) == (n, len(got), first)
+        assert [x[2] for x in got] == list(range(first, first + len(got)))
+        numbers += [x[2] for x in got]
+    assert not joined and sorted(numbers) == list(range(total))
 
 
 def test_plan_spreads_few_rows_over_the_chip():
