@@ -4,13 +4,13 @@ torch only owns the device memory and the stream."""
 import ctypes
 import math
 import os
+import struct
 
 import numpy as np
 import torch
 
 from compare_gan_amd.hip import _lib
-from compare_gan_amd.hip._lib import (AttentionInput, AttentionPlanInfo, ConvGeom, HeadRows, Rotation,
-                                       WgradItem, check)
+from compare_gan_amd.hip._lib import AttentionPlanInfo, ConvGeom, WgradItem, check
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -1089,6 +1089,31 @@ def attention_bwd(theta, phi, g, out, lse, dout):
 # multi-head attention on packed rows
 # ------------------------------------------------------------------------------------------------
 HEAD_TYPES = {BF16: 0, F32: 1}
+# cgHeadRows, cgRotation and cgAttentionInput as bytes (native layout): these calls may last a few
+# microseconds, which a ctypes structure's construction is not small against
+_HEAD_ROWS = struct.Struct("@PqqiP0q")
+_ROTATION = struct.Struct("@PPfiii0q")
+_ATTENTION_INPUT = struct.Struct("@PPPqqqqqqiiiif0q")
+
+
+class _On(object):
+    """Launches on `t`'s device and its current stream (`stream`), whichever device is current."""
+
+    __slots__ = ("stream", "_ctx")
+
+    def __init__(self, t):
+        index = t.get_device()
+        self._ctx = None if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+        self.stream = torch._C._cuda_getCurrentRawStream(index)
+
+    def __enter__(self):
+        if self._ctx is not None:
+            self._ctx.__enter__()
+        return self.stream
+
+    def __exit__(self, *exc):
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
 
 
 class RotaryTable(object):
@@ -1142,11 +1167,12 @@ class RotaryTable(object):
             self.amplitude = 0.1 * math.log(factor) + 1.0
         self.rotary_dim, self.axes, self.layout = rotary_dim, axes, layout
         self.freq = torch.tensor(turns * axes, dtype=F64, device=device)
+        self._tail = (self.freq.data_ptr(), self.amplitude, axes, rotary_dim, 1 if layout == "interleaved" else 0)
         _ready_on_every_stream(self.freq)
 
-    def struct(self, positions):
-        return Rotation(_p(positions), _p(self.freq), self.amplitude, self.axes, self.rotary_dim,
-                        1 if self.layout == "interleaved" else 0)
+    def packed(self, positions):
+        """cgRotation for `positions` (its bytes)."""
+        return _ROTATION.pack(positions.data_ptr(), *self._tail)
 
 
 def _ready_on_every_stream(t):
@@ -1173,11 +1199,22 @@ def _head_inner(t):
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _row_strides(t):
+    """Strides of rows and heads; of a dimension of one entry it means nothing: 0 keeps the alignment
+    rules out of it."""
+    rows, heads, _ = t.shape
+    st, sh, _ = t.stride()
+    return st if rows > 1 else 0, sh if heads > 1 else 0
+
+
 def _head_rows(t, gain=None):
-    # a stride of a dimension of one entry means nothing: 0 keeps the alignment rules out of it
-    st = t.stride(0) if t.shape[0] > 1 else 0
-    sh = t.stride(1) if t.shape[1] > 1 else 0
-    return HeadRows(_p(t), st, sh, t.shape[1], _p(gain))
+    """cgHeadRows of `t` (its bytes)."""
+    st, sh = _row_strides(t)
+    return _HEAD_ROWS.pack(t.data_ptr(), st, sh, t.shape[1], 0 if gain is None else gain.data_ptr())
+
+
+def _dense_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _rotary_args(x, positions, table):
@@ -1187,8 +1224,7 @@ def _rotary_args(x, positions, table):
     if not torch.is_tensor(positions) or not positions.is_cuda or positions.dtype != torch.int32:
         raise ValueError("positions must be an int32 tensor on the GPU")
     want = (x.shape[0],) if table.axes == 1 else (x.shape[0], table.axes)
-    if tuple(positions.shape) != want and not (table.axes == 1 and
-                                               tuple(positions.shape) == (x.shape[0], 1)):
+    if positions.shape != want and positions.shape != (x.shape[0], table.axes):
         raise ValueError("positions must be %s for %d axes, got %s" % (
             list(want), table.axes, list(positions.shape)))
     if positions.device != x.device or table.freq.device != x.device:
@@ -1212,11 +1248,11 @@ def rotary(x, positions, table, inverse=False):
     _req_width(x, "x")
     positions = _rotary_args(x, positions, table)
     x = _head_inner(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        check(lib().cg_rotary(ctypes.byref(_head_rows(x)), x.shape[0], x.shape[2], HEAD_TYPES[x.dtype],
-                              ctypes.byref(table.struct(positions)), 1 if inverse else 0, _p(y), _stream()),
-              "cg_rotary")
+    rows, _, width = x.shape
+    y = _dense_like(x)
+    with _On(x) as stream:
+        check(lib().cg_rotary(_head_rows(x), rows, width, HEAD_TYPES[x.dtype], table.packed(positions),
+                              1 if inverse else 0, y.data_ptr(), stream), "cg_rotary")
     return y
 
 
@@ -1244,13 +1280,13 @@ def qk_norm_rotary(q, k, q_gain, k_gain, positions, table, eps=1e-6):
     (fp32 [D] or None), then the rotation (positions = table = None: none), in one launch."""
     positions = _qk_args(q, k, q_gain, k_gain, positions, table, eps)
     q, k = _head_inner(q), _head_inner(k)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    rot = None if table is None else ctypes.byref(table.struct(positions))
-    with torch.cuda.device(q.device):
+    rows, _, width = q.shape
+    q_out, k_out = _dense_like(q), _dense_like(k)
+    rot = None if table is None else table.packed(positions)
+    with _On(q) as stream:
         check(lib().cg_qk_norm_rotary_fwd(
-            ctypes.byref(_head_rows(q, q_gain)), ctypes.byref(_head_rows(k, k_gain)), q.shape[0], q.shape[2],
-            HEAD_TYPES[q.dtype], eps, rot, _p(q_out), _p(k_out), _stream()), "cg_qk_norm_rotary_fwd")
+            _head_rows(q, q_gain), _head_rows(k, k_gain), rows, width, HEAD_TYPES[q.dtype], eps, rot,
+            q_out.data_ptr(), k_out.data_ptr(), stream), "cg_qk_norm_rotary_fwd")
     return q_out, k_out
 
 
@@ -1263,17 +1299,17 @@ def qk_norm_rotary_bwd(q, k, q_gain, k_gain, positions, table, dq_out, dk_out, e
     if dq_out.shape != q.shape or dk_out.shape != k.shape or dq_out.device != q.device or dk_out.device != q.device:
         raise ValueError("dq_out and dk_out must have the shapes and the device of q and k")
     q, k = _head_inner(q), _head_inner(k)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    rows, _, width = q.shape
+    dq, dk = _dense_like(q), _dense_like(k)
     dqg = None if q_gain is None else torch.empty_like(q_gain)
     dkg = None if k_gain is None else torch.empty_like(k_gain)
-    ws = _ws(lib().cg_qk_norm_rotary_bwd_workspace_bytes(q.shape[0], q.shape[2]), q)
-    rot = None if table is None else ctypes.byref(table.struct(positions))
-    with torch.cuda.device(q.device):
+    ws = _ws(lib().cg_qk_norm_rotary_bwd_workspace_bytes(rows, width), q)
+    rot = None if table is None else table.packed(positions)
+    with _On(q) as stream:
         check(lib().cg_qk_norm_rotary_bwd(
-            ctypes.byref(_head_rows(q, q_gain)), ctypes.byref(_head_rows(k, k_gain)), _p(dq_out), _p(dk_out),
-            q.shape[0], q.shape[2], HEAD_TYPES[q.dtype], eps, rot, _p(dq), _p(dk), _p(dqg), _p(dkg), _p(ws),
-            ws.numel(), _stream()), "cg_qk_norm_rotary_bwd")
+            _head_rows(q, q_gain), _head_rows(k, k_gain), dq_out.data_ptr(), dk_out.data_ptr(), rows, width,
+            HEAD_TYPES[q.dtype], eps, rot, dq.data_ptr(), dk.data_ptr(), _p(dqg), _p(dkg), ws.data_ptr(),
+            ws.numel(), stream), "cg_qk_norm_rotary_bwd")
     return dq, dk, dqg, dkg
 
 
@@ -1303,6 +1339,7 @@ class AttentionPlan(object):
         args = [a.ctypes.data for a in (q_starts, q_lengths, k_starts, k_lengths)]
         tail = (len(q_lengths), heads, kv_heads, 1 if causal else 0)
         self.info = AttentionPlanInfo()
+        self.ref = ctypes.byref(self.info)
         check(lib().cg_host_attention_plan(*args, *tail, None, 0, ctypes.byref(self.info)),
               "cg_host_attention_plan")
         self.host = np.empty(self.info.ints, dtype=np.int32)
@@ -1340,8 +1377,8 @@ def _sequences(starts, lengths, name):
 def _attention_operand(t):
     """`t` as the kernels read it: entries of a head contiguous, rows and heads at multiples of 16 bytes
     (a dense copy where it is not)."""
-    st = [t.stride(i) for i in (0, 1) if t.shape[i] > 1]
-    if t.stride(-1) != 1 or any(x % 8 for x in st) or t.data_ptr() % 16:
+    st, sh = _row_strides(t)
+    if t.stride(2) != 1 or st % 8 or sh % 8 or t.data_ptr() % 16:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -1373,10 +1410,10 @@ def _attention_input(q, k, v, plan, scale):
     return scale
 
 
-def _attention_struct(q, k, v, scale):
-    r = [_head_rows(t) for t in (q, k, v)]
-    return AttentionInput(r[0].x, r[1].x, r[2].x, r[0].stride_t, r[0].stride_h, r[1].stride_t, r[1].stride_h,
-                          r[2].stride_t, r[2].stride_h, q.shape[0], k.shape[0], q.shape[2], v.shape[2], scale)
+def _attention_packed(q, k, v, scale):
+    """cgAttentionInput (its bytes)."""
+    return _ATTENTION_INPUT.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *_row_strides(q), *_row_strides(k),
+                                 *_row_strides(v), q.shape[0], k.shape[0], q.shape[2], v.shape[2], scale)
 
 
 def _rows_out(shape, dense, used, device, dtype=BF16):
@@ -1401,12 +1438,14 @@ def packed_attention_fwd(q, k, v, plan, scale=None, want_lse=True, out=None):
         if tuple(out.shape) != shape or out.device != q.device or out.data_ptr() % 16:
             raise ValueError("out must be %s on %s, 16-byte aligned" % (list(shape), q.device))
     lse = torch.empty(shape[:2], dtype=F32, device=q.device) if want_lse else None
-    nbytes = lib().cg_packed_attention_fwd_workspace_bytes(ctypes.byref(plan.info), shape[2])
-    ws = _ws(nbytes, q) if nbytes else None
-    arg = _attention_struct(q, k, v, scale)
-    with torch.cuda.device(q.device):
-        check(lib().cg_packed_attention_fwd(ctypes.byref(arg), ctypes.byref(plan.info), _p(plan.data), _p(out),
-                                            _p(lse), _p(ws), nbytes, _stream()), "cg_packed_attention_fwd")
+    nbytes, ws = 0, None
+    if plan.info.parts:
+        nbytes = lib().cg_packed_attention_fwd_workspace_bytes(plan.ref, shape[2])
+        ws = _ws(nbytes, q)
+    with _On(q) as stream:
+        check(lib().cg_packed_attention_fwd(_attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(),
+                                            out.data_ptr(), _p(lse), _p(ws), nbytes, stream),
+              "cg_packed_attention_fwd")
     return out, lse
 
 
@@ -1423,13 +1462,12 @@ def packed_attention_bwd(q, k, v, plan, out, lse, dout, scale=None):
     dq = _rows_out(q.shape, plan.q_dense, plan.q_rows, q.device)
     dk = _rows_out(k.shape, plan.k_dense, plan.k_rows, q.device)
     dv = _rows_out(v.shape, plan.k_dense, plan.k_rows, q.device)
-    ws = _ws(lib().cg_packed_attention_bwd_workspace_bytes(ctypes.byref(plan.info), q.shape[0], q.shape[2],
-                                                           v.shape[2]), q)
-    arg = _attention_struct(q, k, v, scale)
-    with torch.cuda.device(q.device):
-        check(lib().cg_packed_attention_bwd(ctypes.byref(arg), ctypes.byref(plan.info), _p(plan.data), _p(out),
-                                            _p(lse), _p(dout), _p(dq), _p(dk), _p(dv), _p(ws), ws.numel(),
-                                            _stream()), "cg_packed_attention_bwd")
+    ws = _ws(lib().cg_packed_attention_bwd_workspace_bytes(plan.ref, q.shape[0], q.shape[2], v.shape[2]), q)
+    with _On(q) as stream:
+        check(lib().cg_packed_attention_bwd(
+            _attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel(), stream),
+            "cg_packed_attention_bwd")
     return dq, dk, dv
 
 

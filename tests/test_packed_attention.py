@@ -243,3 +243,16 @@ def test_operators_refuse_host_tensors():
     Fn.qk_norm_rotary(x, x, None, None, pos, table)
   with pytest.raises(ValueError, match="GPU"):
     Fn.packed_attention(x.bfloat16(), x.bfloat16(), x.bfloat16(), K.AttentionPlan([2], device="cpu"))
+
+
+def test_packed_structures_have_the_declared_layout():
+  rows = torch.zeros(200).as_strided((3, 2, 8), (40, 16, 1))
+  raw = _lib.HeadRows.from_buffer_copy(K._head_rows(rows, rows))
+  assert (raw.x, raw.stride_t, raw.stride_h, raw.heads, raw.gain) == (rows.data_ptr(), 40, 16, 2, rows.data_ptr())
+  table = K.RotaryTable(8, scaling="yarn", factor=2.0, axes=2, layout="interleaved", device="cpu")
+  raw = _lib.Rotation.from_buffer_copy(table.packed(rows))
+  assert (raw.positions, raw.freq, raw.axes, raw.rot, raw.interleaved) == (
+      rows.data_ptr(), table.freq.data_ptr(), 2, 8, 1)
+  assert raw.amplitude == pytest.approx(table.amplitude, rel=1e-7)
+  raw = _lib.AttentionInput.from_buffer_copy(K._attention_packed(rows, rows[:2], rows[:1], 0.5))
+  assert [getattr(raw, n) for n, _ in raw._fields_] == [rows.data_ptr()] * 3 + [40, 16, 40, 16, 0, 16, 3, 2, 8, 8, 0.5]
