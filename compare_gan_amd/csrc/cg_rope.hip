@@ -35,9 +35,9 @@ struct RopeArgs {
   const double* freq;
   float* partial;    // [blocks][2][D] gain gradients
   float amplitude, eps, inv_d, sign;
-  int T, D, rot, pairs, per_axis, axes, interleaved;
+  int T, D, rot, pairs, slots, per_axis, axes, interleaved;   // slots: pairs + identities behind them
   int tb, lanes, lanes_log, units, pair_units, chunks;
-  FastDiv dpairs, dper;
+  FastDiv dslots, dper;
 };
 
 template <typename T, int VP>
@@ -105,11 +105,13 @@ __device__ __forceinline__ float2 turn_cos_sin(float turns) {
   }
 }
 
-constexpr int ROPE_LDS_FLOATS = 8192;   // 32 KiB: cosines and sines, then the gain partials
+// 16 KiB: cosines and sines, then the gain partials (rows of a block x D <= 256 lanes x 16 elements); eight blocks a
+// CU, so that the angles of one are formed while others move data
+constexpr int ROPE_LDS_FLOATS = 4096;
 
 // UPL: units (2 VP elements) a lane holds
 template <typename T, int VP, int UPL, bool NORM, bool BWD>
-__global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
+__global__ __launch_bounds__(256, NORM && VP == 8 ? 3 : BWD ? 4 : 6) void rope_kernel(RopeArgs a) {
   __shared__ __attribute__((aligned(16))) float lds[ROPE_LDS_FLOATS];
   float2* cs = reinterpret_cast<float2*>(lds);
   constexpr int E = 2 * VP * UPL;
@@ -143,8 +145,12 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     const int t0 = chunk * a.tb;
     const int nt = min(a.tb, a.T - t0);
     __syncthreads();      // the previous chunk's angles are no longer read
-    for (int i = threadIdx.x; i < nt * a.pairs; i += 256) {
-      const int tok = fdiv(i, a.dpairs), pair = i - tok * a.pairs;
+    for (int i = threadIdx.x; i < nt * a.slots; i += 256) {
+      const int tok = fdiv(i, a.dslots), pair = i - tok * a.slots;
+      if (pair >= a.pairs) {
+        cs[i] = make_float2(1.f, 0.f);
+        continue;
+      }
       const int axis = fdiv(pair, a.dper);
       const double turns = (double)a.positions[(int64_t)(t0 + tok) * a.axes + axis] * a.freq[pair];
       const float2 v = turn_cos_sin<T>((float)(turns - rint(turns)));
@@ -204,7 +210,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 #pragma unroll
           for (int u = 0; u < UPL; ++u) {
             if (!pair_unit[u]) continue;
-            const float2* c = cs + tok * a.pairs + cs_at[u];
+            const float2* c = cs + tok * a.slots + cs_at[u];
 #pragma unroll
             for (int j = 0; j < VP; ++j) {
               const float2 q = c[j];
@@ -297,20 +303,26 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
   }
 }
 
-// dgain[s][d] = sum over blocks of partial[block][s][d]; 64 columns a workgroup, 16 rows of threads
+// dgain[s][d] = sum over blocks of partial[block][s][d]; 16 columns a workgroup, 64 rows of threads, four loads in
+// flight each
 __global__ __launch_bounds__(1024) void rope_gain_kernel(const float* __restrict__ partial, int blocks, int D,
                                                          float* __restrict__ dq, float* __restrict__ dk) {
-  __shared__ float lds[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
-  float sum = 0.f;
+  __shared__ float lds[64][17];
+  const int c = threadIdx.x & 15, col = blockIdx.x * 16 + c, part = threadIdx.x >> 4;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
   if (col < 2 * D)
-    for (int b = part; b < blocks; b += 16) sum += partial[(int64_t)b * 2 * D + col];
-  lds[part][threadIdx.x & 63] = sum;
+    for (int b = part; b < blocks; b += 256) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (b + 64 * j < blocks) sum[j] += partial[(int64_t)(b + 64 * j) * 2 * D + col];
+    }
+  lds[part][c] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
   __syncthreads();
   if (part == 0 && col < 2 * D) {
-    for (int p = 1; p < 16; ++p) sum += lds[p][threadIdx.x & 63];
+    float all = 0.f;
+    for (int p = 0; p < 64; ++p) all += lds[p][c];
     float* out = col < D ? dq : dk;
-    if (out) out[col < D ? col : col - D] = sum;
+    if (out) out[col < D ? col : col - D] = all;
   }
 }
 
@@ -349,19 +361,22 @@ int rope_plan(RopeArgs* a, const cgRotation* rot, int T, int D, int esize, bool 
   a->positions = rot ? rot->positions : nullptr;
   a->freq = rot ? rot->freq : nullptr;
   a->amplitude = rot ? rot->amplitude : 1.f;
-  a->dpairs = make_fastdiv(a->pairs > 0 ? a->pairs : 1);
   a->dper = make_fastdiv(a->per_axis);
-  int vp = 8;
+  // 16-byte loads; the backward pass of bf16 data takes 8-byte ones: with 16 elements a lane it has 188 registers and
+  // two waves a SIMD (65 536 tokens, 12 heads of 32: 51 us, with 8 elements 38)
+  int vp = bwd || esize == 4 ? 4 : 8;
   for (; vp > 1; vp >>= 1) {
-    bool ok = a->pairs % vp == 0 && (D - a->rot) % (2 * vp) == 0;
-    const int bytes = vp * esize > 16 ? 16 : vp * esize;
-    const int v = bytes / esize;
+    // interleaved pairs lie one behind the other: a unit may hold the last pairs and the first copied entries (turned
+    // by the identity); with halves the two parts of a unit have to end together
+    bool ok = D % (2 * vp) == 0 && (a->interleaved || (a->pairs % vp == 0 && (D - a->rot) % (2 * vp) == 0));
     for (int s = 0; s < a->ntensors; ++s)
-      ok = ok && aligned_for(a->t[s].x, a->t[s].st, a->t[s].sh, v, esize) &&
-           (uintptr_t)a->t[s].out % bytes == 0 && (uintptr_t)a->t[s].dy % bytes == 0;
+      ok = ok && aligned_for(a->t[s].x, a->t[s].st, a->t[s].sh, vp, esize) &&
+           (uintptr_t)a->t[s].out % (vp * esize) == 0 && (uintptr_t)a->t[s].dy % (vp * esize) == 0;
     if (ok) break;
   }
-  a->pair_units = a->pairs / vp;
+  a->pair_units = cdiv(a->pairs, vp);
+  a->slots = a->pair_units * vp;
+  a->dslots = make_fastdiv(a->slots > 0 ? a->slots : 1);
   a->units = D / (2 * vp);
   a->lanes = 1;
   a->lanes_log = 0;
@@ -374,7 +389,7 @@ int rope_plan(RopeArgs* a, const cgRotation* rot, int T, int D, int esize, bool 
   // tokens a block: about 16 K elements, so that the angles and the launch of a block are spread over
   // enough data, but not so many that fewer than 1024 blocks are left for 256 CUs
   int tb = 16384 / (heads * D);
-  const int room = a->pairs > 0 ? ROPE_LDS_FLOATS / 2 / a->pairs : tb;
+  const int room = a->slots > 0 ? ROPE_LDS_FLOATS / 2 / a->slots : tb;
   if (tb > room) tb = room;
   if (tb > cdiv(T, 1024)) tb = cdiv(T, 1024);
   a->tb = tb < 1 ? 1 : tb;
@@ -386,8 +401,13 @@ int rope_plan(RopeArgs* a, const cgRotation* rot, int T, int D, int esize, bool 
 
 template <typename T, bool NORM, bool BWD>
 void rope_launch(const RopeArgs& a, int vp, int grid, hipStream_t st) {
+  if constexpr (sizeof(T) == 2 && !BWD) {
+    if (vp == 8) {
+      rope_kernel<T, 8, 1, NORM, BWD><<<grid, 256, 0, st>>>(a);
+      return;
+    }
+  }
   switch (vp) {
-    case 8: rope_kernel<T, 8, 1, NORM, BWD><<<grid, 256, 0, st>>>(a); break;
     case 4: rope_kernel<T, 4, 1, NORM, BWD><<<grid, 256, 0, st>>>(a); break;
     case 2: rope_kernel<T, 2, 1, NORM, BWD><<<grid, 256, 0, st>>>(a); break;
     default: rope_kernel<T, 1, 2, NORM, BWD><<<grid, 256, 0, st>>>(a); break;
@@ -481,7 +501,7 @@ extern "C" int cg_qk_norm_rotary_bwd(const cgHeadRows* q, const cgHeadRows* k, c
     CG_CHECK_LAUNCH(name);
   }
   if (dq_gain || dk_gain) {   // (T == 0: no partials, zeros)
-    rope_gain_kernel<<<cdiv(2 * D, 64), 1024, 0, (hipStream_t)stream>>>((const float*)ws, grid, D, dq_gain,
+    rope_gain_kernel<<<cdiv(2 * D, 16), 1024, 0, (hipStream_t)stream>>>((const float*)ws, grid, D, dq_gain,
                                                                        dk_gain);
     CG_CHECK_LAUNCH(name);
   }
