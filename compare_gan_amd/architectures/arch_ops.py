@@ -874,3 +874,69 @@ def non_local_block(x, name, use_sn):
     # gradient sigma * dy, and the dot product for d sigma)
     return conv1x1(attn_g, c, name="conv2d_attn_g", use_sn=use_sn, use_bias=False, logical_in=cg,
                    kernel_scale=sigma, residual=x.contiguous())
+
+
+# what multi_head_block keeps for a call shape: positions, frequencies and the plan live as long as the process (a
+# captured step reads them on every replay)
+_ATTENTION_CONSTANTS = {}
+
+
+def _attention_constants(n, h, w, heads, kv_heads, width, base, device):
+  key = (n, h, w, heads, kv_heads, width, base, str(device))
+  if key not in _ATTENTION_CONSTANTS:
+    cell = torch.arange(n * h * w, device=device) % (h * w)
+    positions = torch.stack((cell // w, cell % w), 1).to(torch.int32)
+    _ATTENTION_CONSTANTS[key] = (
+        positions, K.RotaryTable(width, base=base, axes=2, device=device),
+        K.AttentionPlan([h * w] * n, heads=heads, kv_heads=kv_heads, device=device))
+  return _ATTENTION_CONSTANTS[key]
+
+
+def multi_head_block(x, name, use_sn, num_heads=None, num_kv_heads=None, head_width=64, rotary_base=100.0):
+  """Self-attention with several heads on a map: x + sigma * W_o attention(q, k, v) with q, k, v 1x1
+  convolutions at full resolution, q and k RMS-normalised per head (trainable gains) and rotated by row (first
+  half of a head's pairs) and column (second half), every query seeing every position of its image.
+
+  num_heads: query heads of head_width entries (default: as many as fill the channels, at least one);
+  num_kv_heads: key / value heads they share (default: one each)."""
+  n, h, w, c = x.shape
+  heads = max(1, c // head_width) if num_heads is None else int(num_heads)
+  kv_heads = heads if num_kv_heads is None else int(num_kv_heads)
+  if heads < 1 or kv_heads < 1 or heads % kv_heads:
+    raise ValueError("num_heads (%d) must be a positive multiple of num_kv_heads (%d)" % (heads, kv_heads))
+  if head_width < 8 or head_width > 128 or head_width % 8:
+    raise ValueError("head_width must be a multiple of 8 up to 128, got %d" % head_width)
+  with variable_scope(name):
+    x_q, x_k, x_v, x = Fn.fork_n(x, 4) if _FORK_ATTENTION else (x, x, x, x)
+    q = conv1x1(x_q, heads * head_width, name="conv2d_q", use_sn=use_sn, use_bias=False)
+    k = conv1x1(x_k, kv_heads * head_width, name="conv2d_k", use_sn=use_sn, use_bias=False)
+    v = conv1x1(x_v, kv_heads * head_width, name="conv2d_v", use_sn=use_sn, use_bias=False)
+    q_gain = get_variable("q_gain", [head_width], constant(1.0))
+    k_gain = get_variable("k_gain", [head_width], constant(1.0))
+    if x.is_meta:
+      out = torch.empty((n, h, w, heads * head_width), dtype=BF16, device="meta")
+    else:
+      positions, table, plan = _attention_constants(n, h, w, heads, kv_heads, head_width, rotary_base, x.device)
+      rows = n * h * w
+      q, k = Fn.qk_norm_rotary(q.reshape(rows, heads, head_width), k.reshape(rows, kv_heads, head_width), q_gain,
+                               k_gain, positions, table)
+      out = Fn.packed_attention(q, k, v.reshape(rows, kv_heads, head_width), plan)
+      out = out.reshape(n, h, w, heads * head_width)
+    sigma = get_variable("sigma", [], constant(0.0))
+    if x.is_meta or not _FOLD_SIGMA:
+      out = conv1x1(out, c, name="conv2d_o", use_sn=use_sn, use_bias=False)
+      return x if x.is_meta else Fn.ScaledResidualFn.apply(x, out, sigma.reshape(1))
+    return conv1x1(out, c, name="conv2d_o", use_sn=use_sn, use_bias=False, kernel_scale=sigma,
+                   residual=x.contiguous())
+
+
+@gin.configurable(whitelist=["kind", "num_heads", "num_kv_heads", "head_width", "rotary_base"])
+def attention_block(x, name, use_sn, kind="non_local", num_heads=None, num_kv_heads=None, head_width=64,
+                    rotary_base=100.0):
+  """The self-attention of the BigGAN networks: `kind` "non_local" is the reference's single-head block
+  (non_local_block, arch_ops.py:709-758; the default), "multi_head" multi_head_block with the options behind it."""
+  if kind == "non_local":
+    return non_local_block(x, name, use_sn)
+  if kind == "multi_head":
+    return multi_head_block(x, name, use_sn, num_heads, num_kv_heads, head_width, rotary_base)
+  raise ValueError("attention_block.kind must be 'non_local' or 'multi_head', got %r" % (kind,))

@@ -103,7 +103,7 @@ class Generator(abstract_arch.AbstractGenerator):
       net = block(net, z=z_per_block[block_idx], y=y_per_block[block_idx],
                   is_training=is_training)
       if name in self._blocks_with_attention:
-        net = ops.non_local_block(net, "non_local_block", use_sn=self._spectral_norm)
+        net = ops.attention_block(net, "non_local_block", use_sn=self._spectral_norm)
     # final processing: UNconditional batch norm (resnet_biggan.py:293-295)
     net = ops.batch_norm(net, is_training=is_training, name="final_norm", relu=True)
     net = ops.conv2d(net, output_dim=self._image_shape[2], k_h=3, k_w=3, d_h=1, d_w=1,
@@ -152,7 +152,7 @@ class Discriminator(abstract_arch.AbstractDiscriminator):
                                  scale="none" if is_last_block else "down")
       net = block(net, z=None, y=y, is_training=is_training)
       if name in self._blocks_with_attention:
-        net = ops.non_local_block(net, "non_local_block", use_sn=self._spectral_norm)
+        net = ops.attention_block(net, "non_local_block", use_sn=self._spectral_norm)
     # relu + reduce_sum over [1, 2] + linear(C -> 1); h also feeds the projection term below
     out_logit, h = ops.pooled_linear_head(ops.relu(net), mean=False, scope="final_fc",
                                           use_sn=self._spectral_norm)

@@ -154,7 +154,7 @@ class Generator(abstract_arch.AbstractGenerator):
                                  out_channels=out_channels[block_idx], scale=scale)
       net = block(net, z=z, y=y, is_training=is_training)
       if scale == "up" and net.shape[1] == 64:       # self-attention at 64x64
-        net = ops.non_local_block(net, "non_local_block", use_sn=self._spectral_norm)
+        net = ops.attention_block(net, "non_local_block", use_sn=self._spectral_norm)
     net = ops.batch_norm(net, is_training=is_training, name="final_norm", relu=True)
     net = ops.conv2d(net, output_dim=self._image_shape[2], k_h=3, k_w=3, d_h=1, d_w=1,
                      name="final_conv", use_sn=self._spectral_norm, out_f32=True)
@@ -199,7 +199,7 @@ class Discriminator(abstract_arch.AbstractDiscriminator):
                                  out_channels=out_channels[block_idx], scale=scale)
       net = block(net, z=None, y=y, is_training=is_training)
       if scale == "none" and net.shape[1] == 64:     # self-attention at 64x64
-        net = ops.non_local_block(net, "non_local_block", use_sn=self._spectral_norm)
+        net = ops.attention_block(net, "non_local_block", use_sn=self._spectral_norm)
     # relu + reduce_sum over [1, 2] + linear(C -> 1); h also feeds the projection term below
     out_logit, h = ops.pooled_linear_head(ops.relu(net), mean=False, scope="final_fc",
                                           use_sn=self._spectral_norm)

@@ -1,0 +1,108 @@
+"""The multi-head attention block inside the networks that call it: forward and gradients against the chain in 64 bits,
+a BigGAN training step with it, captured and eager."""
+import math
+
+import pytest
+import torch
+
+from tests import gan_util as U
+
+pytestmark = pytest.mark.gpu
+
+HB = 2.0 ** -8
+
+
+@pytest.fixture(autouse=True)
+def clean_config():
+  from compare_gan_amd import gin
+  gin.clear_config()
+  yield
+  gin.clear_config()
+
+
+@pytest.mark.parametrize("n,h,w,c,heads,kv_heads,width", [(2, 8, 8, 64, None, None, 64), (3, 4, 6, 96, 4, 2, 32),
+                                                        (1, 5, 5, 32, 2, 1, 16)])
+def test_block_against_the_chain(dev, n, h, w, c, heads, kv_heads, width):
+  """Relative error of whole tensors: the input of each of the five stages (projection, norm + rotation, attention,
+  back projection, residual) and of their gradients is rounded to bf16, half a step of 2^-8 each, and the projections'
+  operand images are bf16 too: seven roundings, uncorrelated over the sums."""
+  from compare_gan_amd.architectures import arch_ops as ops
+  gen = torch.Generator().manual_seed(n + c)
+  store = ops.VariableStore(dev, seed=1)
+  x = torch.randn((n, h, w, c), generator=gen).bfloat16().to(dev).requires_grad_(True)
+  with ops.use_store(store):
+    ops.attention_block(x.detach(), "att", False, kind="multi_head", num_heads=heads, num_kv_heads=kv_heads,
+                        head_width=width)
+    with torch.no_grad():
+      for name, v in store.vars.items():      # weights of size 1 / sqrt(fan in), a sigma that shows
+        if name.endswith("kernel"):
+          v.copy_(torch.randn(v.shape, generator=gen).to(dev) / math.sqrt(v.shape[2]))
+        elif name.endswith("gain"):
+          v.copy_((1 + 0.2 * torch.randn(v.shape, generator=gen)).to(dev))
+        else:
+          v.fill_(0.7)
+    out = ops.attention_block(x, "att", False, kind="multi_head", num_heads=heads, num_kv_heads=kv_heads,
+                              head_width=width)
+  dout = torch.randn((n, h, w, c), generator=gen).bfloat16().to(dev)
+  names = sorted(store.vars)
+  grads = torch.autograd.grad(out, [x] + [store.vars[k] for k in names], dout)
+  heads = heads or max(1, c // width)
+  kv_heads = kv_heads or heads
+  v64 = {k.split("att/")[1]: store.vars[k].detach().double().cpu().requires_grad_(True) for k in names}
+  x64 = x.detach().double().cpu().requires_grad_(True)
+  rows = x64.reshape(n, h * w, c)
+  half = width // 4
+  f = 100.0 ** (-torch.arange(half, dtype=torch.float64) / half)
+  cell = torch.arange(h * w)
+  angle = torch.cat(((cell // w)[:, None] * f, (cell % w)[:, None] * f), 1)[None, :, None]
+
+  def norm_turn(t, gain):
+    t = t / torch.sqrt(t.square().mean(-1, keepdim=True) + 1e-6) * gain
+    a, b = t[..., :width // 2], t[..., width // 2:]
+    return torch.cat((a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()), -1)
+  q = norm_turn((rows @ v64["conv2d_q/kernel"][0, 0]).reshape(n, h * w, heads, width), v64["q_gain"])
+  k = norm_turn((rows @ v64["conv2d_k/kernel"][0, 0]).reshape(n, h * w, kv_heads, width), v64["k_gain"])
+  v = (rows @ v64["conv2d_v/kernel"][0, 0]).reshape(n, h * w, kv_heads, width)
+  k, v = (t.repeat_interleave(heads // kv_heads, 2) for t in (k, v))
+  p = torch.softmax(torch.einsum("nqhd,nkhd->nhqk", q, k) / math.sqrt(width), -1)
+  o = torch.einsum("nhqk,nkhd->nqhd", p, v).reshape(n, h * w, heads * width)
+  want = x64 + (v64["sigma"] * (o @ v64["conv2d_o/kernel"][0, 0])).reshape(n, h, w, c)
+  wgrads = torch.autograd.grad(want, [x64] + [v64[k.split("att/")[1]] for k in names], dout.double().cpu())
+  for name, a, b in zip(["out", "dx"] + names, (out,) + grads, (want,) + wgrads):
+    a, b = a.detach().double().cpu(), b.detach()
+    assert float((a - b).norm() / b.norm()) <= 7 * HB, name
+
+
+@pytest.mark.parametrize("arch", ["resnet_biggan", "resnet_biggan_deep"])
+def test_biggan_step_with_several_heads(dev, arch):
+  """biggan_imagenet128.gin with the multi-head block: a captured step is the eager one to the bit, losses are finite
+  and the block's variables get gradients (Adam moves them)."""
+  bsz = 2
+  bindings = ("options.batch_size = %d" % bsz, 'attention_block.kind = "multi_head"', "attention_block.num_heads = 4",
+              "attention_block.num_kv_heads = 2", "attention_block.head_width = 32")
+  if arch == "resnet_biggan":
+    bindings += ("resnet_biggan.Generator.ch = 32", "resnet_biggan.Discriminator.ch = 32")
+  else:
+    bindings += ('options.architecture = "resnet_biggan_deep_arch"', "resnet_biggan_deep.Generator.ch = 32",
+                 "resnet_biggan_deep.Discriminator.ch = 32", "G.batch_norm_fn = @conditional_batch_norm")
+  eager, options, dataset = U.build_product("biggan_imagenet128.gin", bsz, dev, seed=5, bindings=bindings)
+  graph, _, _ = U.build_product("biggan_imagenet128.gin", bsz, dev, seed=5, bindings=bindings)
+  it = dataset.train_batches(bsz * (options["disc_iters"] + 1), seed=21)
+  batches = [next(it) for _ in range(2)]
+  with torch.no_grad():       # sigma = 0 in front of a fresh block: its projections would see no gradient
+    for gan in (eager, graph):
+      for name, v in gan.store.vars.items():
+        if name.endswith("non_local_block/sigma"):
+          v.fill_(0.5)
+  before = {k: v.detach().clone() for k, v in eager.store.vars.items() if "non_local_block" in k}
+  assert any(k.endswith("q_gain") for k in before)
+  run = graph.capture_train_step()
+  for images, labels in batches:
+    x, y = torch.from_numpy(images).to(dev), torch.from_numpy(labels).to(dev)
+    oe, og = eager.train_step(x, y), run(x, y)
+    assert torch.isfinite(oe["g_loss"]).all() and torch.equal(oe["g_loss"], og["g_loss"])
+  torch.cuda.synchronize()
+  se, sg = eager.state_dict(), graph.state_dict()
+  assert not [k for k in se if not torch.equal(se[k], sg[k])]
+  still = [k for k, v in before.items() if k in eager.store.trainable and torch.equal(v, eager.store.vars[k])]
+  assert not still, still
