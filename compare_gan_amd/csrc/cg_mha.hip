@@ -196,8 +196,7 @@ __device__ __forceinline__ MhaReads<DP> mha_reads(int lane) {
 // S^T tile of 32 keys (rows `sub` of the LDS tile) and one wave's 32 rows
 template <int DP>
 __device__ __forceinline__ f32x16_t mha_product(mha_lds_ptr tile, const MhaReads<DP>& m,
-                                                const bf16x8_t (&f)[DP / 16], int sub) {
-  f32x16_t s = mha_zero();
+                                                const bf16x8_t (&f)[DP / 16], int sub, f32x16_t s = mha_zero()) {
 #pragma unroll
   for (int kd = 0; kd < DP / 16; ++kd) {
     const bf16x8_t x = *(mha_frag_ptr)(tile + m.row[kd] + sub * 64 * DP);
@@ -543,7 +542,7 @@ __device__ __forceinline__ float mha_lse2(float lse) { return lse == -INFINITY ?
 
 // dQ: 128 rows x all keys; S^T and dP^T = V dO^T side by side, dQ^T += K^T dS^T
 template <int DP>
-__global__ __launch_bounds__(256, 2) void mha_bwd_q_kernel(MhaArgs a) {
+__global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArgs a) {
   constexpr int TILE = KT * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -592,17 +591,17 @@ __global__ __launch_bounds__(256, 2) void mha_bwd_q_kernel(MhaArgs a) {
     if (k0 + KT < it.k1) stage(k0 + KT, buf ^ 1);
     if (k0 > most) continue;
     mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
-#pragma unroll 1
+#pragma unroll
     for (int n = 0; n < 2; ++n) {
+      __builtin_amdgcn_sched_barrier(0);      // one step's scores live at a time
       f32x16_t s = mha_product<DP>(ks, rd, qf, n);
       const f32x16_t dp = mha_product<DP>(vs, rd, df, n);
-      const bool masked = k0 + n * 32 + 31 > least;
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c, -lse2));
-        p *= dp[v] - delta;
-        if (masked) p = k0 + n * 32 + mha_key(v, half) <= last ? p : 0.f;
-        s[v] = p;
+      for (int v = 0; v < 16; ++v)
+        s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c, -lse2)) * (dp[v] - delta);
+      if (k0 + n * 32 + 31 > least) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] = k0 + n * 32 + mha_key(v, half) <= last ? s[v] : 0.f;
       }
       mha_accumulate<DP>(dq, ks, rd, s, n);
     }
@@ -631,7 +630,7 @@ template <int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaArgs a) {
   constexpr int TILE = KT * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][KT];   // [buffer][lse, delta][row]
+  __shared__ __attribute__((aligned(16))) float stat[2][2][KT];   // [buffer][lse, -delta][row]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
   const MhaItem it = mha_item(a, blockIdx.x);
@@ -684,7 +683,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
     if (r >= re) return wave == 0 ? INFINITY : 0.f;
     const int t = (int)fdiv((uint32_t)r, a.dG), g = r - t * a.G;
     const int64_t row = (int64_t)(it.q_start + t) * a.heads + it.hk * a.G + g;
-    return wave == 0 ? mha_lse2(a.lse_in[row]) : a.delta[row];
+    return wave == 0 ? mha_lse2(a.lse_in[row]) : -a.delta[row];
   };
   float next = 0.f;
   if (rb < re) {
@@ -702,30 +701,37 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
     }
     if (!some) continue;
     mha_lds_ptr qs = sm + buf * 2 * TILE, ds = qs + TILE;
-#pragma unroll 1
+#pragma unroll
     for (int n = 0; n < 2; ++n) {
+      __builtin_amdgcn_sched_barrier(0);      // one step's scores live at a time
       const int rs = r0 + n * 32;
       if (rs + 31 < wave_first || rs >= re) continue;
-      f32x16_t s = mha_product<DP>(qs, rd, kf, n);
-      f32x16_t dp = mha_product<DP>(ds, rd, vf, n);
-      const bool masked = rs < wave_all;
+      // dP starts from -delta: the rows of an accumulator are 4 v / 4 + .. , four statistics a read
+      f32x16_t dp;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const float4 ls = *reinterpret_cast<const float4*>(&stat[buf][0][n * 32 + 8 * g + 4 * half]);
-        const float4 de = *reinterpret_cast<const float4*>(&stat[buf][1][n * 32 + 8 * g + 4 * half]);
-        const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dev[4] = {de.x, de.y, de.z, de.w};
+        const f32x4_t de = *reinterpret_cast<const f32x4_t*>(&stat[buf][1][n * 32 + 8 * g + 4 * half]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dp[4 * g + j] = de[j];
+      }
+      f32x16_t s = mha_product<DP>(qs, rd, kf, n);
+      dp = mha_product<DP>(ds, rd, vf, n, dp);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_t ls = *reinterpret_cast<const f32x4_t*>(&stat[buf][0][n * 32 + 8 * g + 4 * half]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int v = 4 * g + j;
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c, -lsv[j]));
-          float x = p * (dp[v] - dev[j]);
-          if (masked) {
-            const bool see = rs + mha_key(v, half) >= mine;
-            p = see ? p : 0.f;
-            x = see ? x : 0.f;
-          }
-          s[v] = p;
-          dp[v] = x;
+          s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c, -ls[j]));
+          dp[v] *= s[v];
+        }
+      }
+      if (rs < wave_all) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const bool see = rs + mha_key(v, half) >= mine;
+          s[v] = see ? s[v] : 0.f;
+          dp[v] = see ? dp[v] : 0.f;
         }
       }
       mha_accumulate<DP>(dv, ds, rd, s, n);
