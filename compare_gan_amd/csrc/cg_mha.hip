@@ -169,6 +169,14 @@ __device__ __forceinline__ void mha_row_frags(bf16x8_t (&f)[KD], const bf16_t* p
   }
 }
 
+// Waits here for fragments loaded from memory.  Without it the first use is inside the tile loop, and the compiler,
+// which does not see the asm copies, puts a vmcnt wait there that holds every pass for the copies of the NEXT tile
+template <int KD>
+__device__ __forceinline__ void mha_settle(bf16x8_t (&f)[KD]) {
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd) asm volatile("" : "+v"(f[kd]));
+}
+
 // LDS offsets of a lane's reads in a tile of 2 DP byte rows
 template <int DP>
 struct MhaReads {
@@ -350,6 +358,7 @@ __global__ __launch_bounds__(256, 2) void mha_fwd_kernel(MhaArgs a) {
   for (int i = 0; i < DP / 32; ++i) o[i] = mha_zero();
   float m = -INFINITY, l = 0.f;
   if (it.k0 < it.k1) stage(it.k0, 0);
+  mha_settle(qf);
   int buf = 0;
   for (int k0 = it.k0; k0 < it.k1; k0 += KT, buf ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -421,6 +430,7 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
   const int first = it.k0 + wave * 32;
   constexpr int INFLIGHT = 2 * Stage::N;         // copies of one step
   if (first < it.k1) stage(first, 0);
+  mha_settle(qf);
   int buf = 0;
   for (int k0 = first; k0 < it.k1; k0 += NW * 32, buf ^= 1) {
     // the other buffer was read in the last step: those reads have returned (their values were used)
@@ -584,6 +594,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dq[i] = mha_zero();
   if (it.k0 < it.k1) stage(it.k0, 0);
+  mha_settle(qf);
+  mha_settle(df);
   int buf = 0;
   for (int k0 = it.k0; k0 < it.k1; k0 += KT, buf ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -676,24 +688,26 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
     dv[i] = mha_zero();
   }
 
-  // wave 0 / 1 carry the statistics of the next tile: one row a lane
+  // wave 0 / 1 carry the statistics of the next tile, one row a lane: loaded here, touched a tile later (a use next to
+  // the load would hold the two waves, and at the barrier all, for the load's whole latency in every tile)
   auto stat_load = [&](int r0) {
     const int r = r0 + lane;
-    if (wave > 1) return 0.f;
-    if (r >= re) return wave == 0 ? INFINITY : 0.f;
+    if (wave > 1 || r >= re) return wave == 0 ? -INFINITY : 0.f;
     const int t = (int)fdiv((uint32_t)r, a.dG), g = r - t * a.G;
     const int64_t row = (int64_t)(it.q_start + t) * a.heads + it.hk * a.G + g;
-    return wave == 0 ? mha_lse2(a.lse_in[row]) : -a.delta[row];
+    return wave == 0 ? a.lse_in[row] : a.delta[row];
   };
   float next = 0.f;
   if (rb < re) {
     next = stat_load(rb);
     stage(rb, 0);
   }
+  mha_settle(kf);
+  mha_settle(vf);
   int buf = 0;
   for (int r0 = rb; r0 < re; r0 += KT, buf ^= 1) {
-    if (wave < 2) stat[buf][wave][lane] = next;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (wave < 2) stat[buf][wave][lane] = wave == 0 ? mha_lse2(next) : -next;
     __syncthreads();
     if (r0 + KT < re) {
       next = stat_load(r0 + KT);
