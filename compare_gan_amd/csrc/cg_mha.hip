@@ -495,7 +495,7 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
   mha_store<DP>(a, it, col, m, l, o, half);
 }
 
-// ---- joins the partial results of a split item; one wave a row --------------------------------------
+// ---- joins the partial results of a split item; one wave a row, its parts' loads in flight together ------
 // item {seq, hk, row0, rows here, parts, first unit, units a part}
 __global__ __launch_bounds__(256) void mha_join_kernel(MhaArgs a) {
   const MhaItem it = mha_item(a, blockIdx.x);
@@ -504,16 +504,29 @@ __global__ __launch_bounds__(256) void mha_join_kernel(MhaArgs a) {
   const int64_t step = (int64_t)it.units * THIN_ROWS;
   for (int i = blockIdx.y * 4 + wave; i < it.k0; i += gridDim.y * 4) {
     const int64_t at = (int64_t)it.part * THIN_ROWS + i;
+    // one part a lane: the common exponent first
     float top = -INFINITY;
-    for (int p = 0; p < parts; ++p) top = fmaxf(top, a.ws_ml[(at + p * step) * 2]);
-    float total = 0.f, acc[2] = {0.f, 0.f};
-    for (int p = 0; p < parts; ++p) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + (at + p * step) * 2);
-      const float w = mha_weight(ml.x, top);
-      total += ml.y * w;
+    for (int p = lane; p < parts; p += 64) top = fmaxf(top, a.ws_ml[(at + p * step) * 2]);
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        if (lane + 64 * j < a.Dv) acc[j] += a.ws_o[(at + p * step) * a.Dv + lane + 64 * j] * w;
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    float total = 0.f, acc[2] = {0.f, 0.f};
+    for (int p0 = 0; p0 < parts; p0 += 64) {
+      float w = 0.f, l = 0.f;
+      if (p0 + lane < parts) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + (at + (p0 + lane) * step) * 2);
+        w = mha_weight(ml.x, top);
+        l = ml.y * w;
+      }
+      total += wave_sum(l);
+      const int n = min(64, parts - p0);
+      const float* src = a.ws_o + (at + p0 * step) * a.Dv;
+#pragma unroll 4
+      for (int p = 0; p < n; ++p) {
+        const float wp = __shfl(w, p, 64);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (lane + 64 * j < a.Dv) acc[j] += src[p * step * a.Dv + lane + 64 * j] * wp;
+      }
     }
     int t, h;
     mha_token(a, it, it.row0 + i, &t, &h);
@@ -638,26 +651,30 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
 
 // dK, dV: 128 keys x the rows that see them.  S[row][key] = Q K^T and dP = dO V^T with the keys in the lanes'
 // columns; dV^T += dO^T P, dK^T += Q^T dS.  Item {seq, hk, key0, first row, end row}.
+// At 128 wide heads the accumulators, K and V of a wave would be 192 registers and the rest spills (each reload also
+// waits for the copies in flight): V is read from LDS there, and the tiles are 32 rows so that two workgroups fit a CU.
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaArgs a) {
-  constexpr int TILE = KT * DP * 2;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
-  __shared__ __attribute__((aligned(16))) float stat[2][2][KT];   // [buffer][lse, -delta][row]
+  constexpr bool V_LDS = DP > 96;
+  constexpr int RT = V_LDS ? 32 : 64;             // rows of a tile
+  constexpr int TILE = RT * DP * 2, V_BYTES = V_LDS ? KEY_TILE * DP * 2 : 0;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE + V_BYTES];
+  __shared__ __attribute__((aligned(16))) float stat[2][2][RT];   // [buffer][lse, -delta][row]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
   const MhaItem it = mha_item(a, blockIdx.x);
   const int key = it.row0 + wave * 32 + col;
   const bool ok = key < it.Lk;
-  bf16x8_t kf[DP / 16], vf[DP / 16];
+  bf16x8_t kf[DP / 16], vf[V_LDS ? 1 : DP / 16];
   mha_row_frags(kf, a.k + (int64_t)(it.k_start + key) * a.kt + (int64_t)it.hk * a.kh, ok, a.D, half);
-  mha_row_frags(vf, a.v + (int64_t)(it.k_start + key) * a.vt + (int64_t)it.hk * a.vh, ok, a.Dv, half);
+  if constexpr (!V_LDS) mha_row_frags(vf, a.v + (int64_t)(it.k_start + key) * a.vt + (int64_t)it.hk * a.vh, ok, a.Dv, half);
   // first row that sees this key; rows of the wave's first and last key for skipping and masking
   auto first_row = [&](int k) { return a.causal ? max(0, k - it.shift) * a.G : 0; };
   const int mine = first_row(key);
   const int wave_first = first_row(it.row0 + wave * 32), wave_all = first_row(it.row0 + wave * 32 + 31);
   const bool some = it.row0 + wave * 32 < it.Lk;
   const int rb = it.k0, re = it.k1;
-  using Stage = MhaStage<DP, KT, 4>;
+  using Stage = MhaStage<DP, RT, 4>;
   const MhaReads<DP> rd = mha_reads<DP>(lane);
   const bf16_t* qb = a.q + (int64_t)it.hk * a.G * a.qh;
   const bf16_t* db = a.dout + (int64_t)it.hk * a.G * a.Dv;
@@ -665,7 +682,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
   mha_lds_ptr sm = (mha_lds_ptr)smem;
   const int64_t dt = (int64_t)a.heads * a.Dv;
   auto stage = [&](int r0, int buf) {
-    // rows r0 .. r0 + 63 gathered by (token, head) relative to the first one's token
+    // rows r0 .. gathered by (token, head) relative to the first one's token
     const int t0 = __builtin_amdgcn_readfirstlane((int)fdiv((uint32_t)r0, a.dG));
     const cg_i32x4_t qr = cg_make_rsrc(qb + (int64_t)(it.q_start + t0) * a.qt, 0x7fffffffu);
     const cg_i32x4_t dr = cg_make_rsrc(db + (int64_t)(it.q_start + t0) * dt, 0x7fffffffu);
@@ -692,31 +709,37 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
   // the load would hold the two waves, and at the barrier all, for the load's whole latency in every tile)
   auto stat_load = [&](int r0) {
     const int r = r0 + lane;
-    if (wave > 1 || r >= re) return wave == 0 ? -INFINITY : 0.f;
+    if (wave > 1 || lane >= RT || r >= re) return wave == 0 ? -INFINITY : 0.f;
     const int t = (int)fdiv((uint32_t)r, a.dG), g = r - t * a.G;
     const int64_t row = (int64_t)(it.q_start + t) * a.heads + it.hk * a.G + g;
     return wave == 0 ? a.lse_in[row] : a.delta[row];
   };
   float next = 0.f;
   if (rb < re) {
+    if constexpr (V_LDS) {                          // the item's 128 rows of V, once
+      uint32_t voff[MhaStage<DP, KEY_TILE, 4>::N];
+      mha_offsets<DP, KEY_TILE, 4>(voff, wave, lane, a.vt, a.Dv);
+      mha_copy<DP, KEY_TILE, 4>(voff, mha_rows<KEY_TILE>(a.v + (int64_t)it.hk * a.vh, it.k_start + it.row0, it.Lk - it.row0,
+                                                         a.vt, a.Dv), lds + 4 * TILE, wave);
+    }
     next = stat_load(rb);
     stage(rb, 0);
   }
   mha_settle(kf);
-  mha_settle(vf);
+  if constexpr (!V_LDS) mha_settle(vf);
   int buf = 0;
-  for (int r0 = rb; r0 < re; r0 += KT, buf ^= 1) {
+  for (int r0 = rb; r0 < re; r0 += RT, buf ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (wave < 2) stat[buf][wave][lane] = wave == 0 ? mha_lse2(next) : -next;
+    if (wave < 2 && lane < RT) stat[buf][wave][lane] = wave == 0 ? mha_lse2(next) : -next;
     __syncthreads();
-    if (r0 + KT < re) {
-      next = stat_load(r0 + KT);
-      stage(r0 + KT, buf ^ 1);
+    if (r0 + RT < re) {
+      next = stat_load(r0 + RT);
+      stage(r0 + RT, buf ^ 1);
     }
     if (!some) continue;
     mha_lds_ptr qs = sm + buf * 2 * TILE, ds = qs + TILE;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < RT / 32; ++n) {
       __builtin_amdgcn_sched_barrier(0);      // one step's scores live at a time
       const int rs = r0 + n * 32;
       if (rs + 31 < wave_first || rs >= re) continue;
@@ -729,7 +752,18 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
         for (int j = 0; j < 4; ++j) dp[4 * g + j] = de[j];
       }
       f32x16_t s = mha_product<DP>(qs, rd, kf, n);
-      dp = mha_product<DP>(ds, rd, vf, n, dp);
+      if (DP > 64) __builtin_amdgcn_sched_barrier(0);
+      if constexpr (V_LDS) {
+        mha_lds_ptr vs = sm + 4 * TILE + wave * 64 * DP;
+#pragma unroll
+        for (int kd = 0; kd < DP / 16; ++kd) {
+          const bf16x8_t x = *(mha_frag_ptr)(ds + rd.row[kd] + n * 64 * DP), y = *(mha_frag_ptr)(vs + rd.row[kd]);
+          dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, dp, 0, 0, 0);
+        }
+      } else {
+        dp = mha_product<DP>(ds, rd, vf, n, dp);
+      }
+      if (DP > 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4_t ls = *reinterpret_cast<const f32x4_t*>(&stat[buf][0][n * 32 + 8 * g + 4 * half]);
@@ -748,7 +782,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
           dp[v] = see ? dp[v] : 0.f;
         }
       }
+      if (DP > 64) __builtin_amdgcn_sched_barrier(0);
       mha_accumulate<DP>(dv, ds, rd, s, n);
+      if (DP > 64) __builtin_amdgcn_sched_barrier(0);
       mha_accumulate<DP>(dk, qs, rd, dp, n);
     }
   }
@@ -1114,8 +1150,8 @@ int mha_check(const char* name, const cgAttentionInput* in, const cgAttentionPla
     if (!ptr[i] && (i == 0 ? p->max_q_row : p->max_k_row) > 0) CG_FAIL(CG_ERR_BAD_ARG, "%s: null tensor", name);
     if ((uintptr_t)ptr[i] % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: tensors have to be 16-byte aligned", name);
   }
-  // a tile's byte offsets are 32-bit (its base is 64-bit): 64 rows, and the shared heads of one
-  if ((int64_t)KT * 2 * std::max(std::max(st[0], st[2]), st[4]) + 2 * G * st[1] >= 0x7fffff00ll ||
+  // a tile's byte offsets are 32-bit (its base is 64-bit): up to 128 rows, and the shared heads of one
+  if ((int64_t)KEY_TILE * 2 * std::max(std::max(st[0], st[2]), st[4]) + 2 * G * st[1] >= 0x7fffff00ll ||
       (int64_t)KT * 2 * p->heads * 128 >= 0x3fffff00ll)
     CG_FAIL(CG_ERR_UNSUPPORTED, "%s: strides too large", name);
   a->q = (const bf16_t*)in->q;
@@ -1227,7 +1263,7 @@ extern "C" int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAtten
   }
   if (plan->joins) {
     a.items = mha_list(plan, data, 3);
-    mha_join_kernel<<<dim3(plan->joins, 8), 256, 0, st>>>(a);
+    mha_join_kernel<<<dim3(plan->joins, plan->tiles ? 32 : 1), 256, 0, st>>>(a);
     CG_CHECK_LAUNCH(name);
   }
   return CG_OK;
