@@ -1013,8 +1013,8 @@ void mha_deal(std::vector<Work>* items, int units) {
 // A launch's items are split along the axis that they sum over (keys; rows for dK and dV) where one item is longer
 // than its share of the launch: the total over so many blocks (2 resident a CU, 256 CUs, a few rounds), but no part
 // below a length at which its fp32 result, written once and read once, is small against its own work.
-constexpr int64_t TILE_BLOCKS = 1024, THIN_BLOCKS = 1024;
-constexpr int TILE_SPLIT_MIN = 512, THIN_SPLIT_MIN = 512, GRAD_SPLIT_MIN = 1024;
+constexpr int64_t TILE_BLOCKS = 512, THIN_BLOCKS = 1024, GRAD_BLOCKS = 1024;
+constexpr int TILE_SPLIT_MIN = 512, THIN_SPLIT_MIN = 512, GRAD_SPLIT_MIN = 512;
 constexpr int THIN1_KEYS = 128;     // up to so many keys one wave does a thin item alone
 
 void mha_split(std::vector<Work>* items, int64_t blocks, int step, int least, int tile, int units_a_part,
@@ -1087,8 +1087,8 @@ int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_star
   int64_t parts = 0, dq_parts = 0, dkv_parts = 0;
   mha_split(&tiles, TILE_BLOCKS, KT, TILE_SPLIT_MIN, ROW_TILE, ROW_TILE / 32, all_rows, &joins, &parts);
   mha_split(&thin4, THIN_BLOCKS, 32, THIN_SPLIT_MIN, THIN_ROWS, 1, all_rows, &joins, &parts);
-  mha_split(&dq, TILE_BLOCKS, KT, GRAD_SPLIT_MIN, ROW_TILE, 1, all_rows, &dq_joins, &dq_parts);
-  mha_split(&dkv, TILE_BLOCKS, KT, GRAD_SPLIT_MIN, KEY_TILE, 1, all_keys, &dkv_joins, &dkv_parts);
+  mha_split(&dq, GRAD_BLOCKS, KT, GRAD_SPLIT_MIN, ROW_TILE, 1, all_rows, &dq_joins, &dq_parts);
+  mha_split(&dkv, GRAD_BLOCKS, KT, GRAD_SPLIT_MIN, KEY_TILE, 1, all_keys, &dkv_joins, &dkv_parts);
   if (parts > 0x7fffffff || dq_parts > 0x7fffffff || dkv_parts > 0x7fffffff) CG_FAIL(CG_ERR_UNSUPPORTED, "cg_host_attention_plan: too many partial results");
   const int units = B * kv_heads;
   std::vector<Work>* lists[9] = {&tiles, &thin4, &thin1, &joins, &dq, &dq_joins, &dkv, &dkv_joins, &small};
@@ -1275,7 +1275,7 @@ static int64_t mha_delta_bytes(const cgAttentionPlan* p, int q_rows) {
 }
 
 extern "C" size_t cg_packed_attention_bwd_workspace_bytes(const cgAttentionPlan* plan, int q_rows, int D, int Dv) {
-  if (!plan || q_rows < 1 || D < 1 || Dv < 1) return 0;
+  if (!plan || q_rows < 1 || D < 1 || Dv < 1 || plan->dq_tiles + plan->dkv_tiles == 0) return 0;
   const int64_t a = plan->dq_parts * D, b = plan->dkv_parts * (D + Dv);
   return (size_t)(mha_delta_bytes(plan, q_rows) + (a > b ? a : b) * ROW_TILE * (int64_t)sizeof(float));
 }
@@ -1289,7 +1289,8 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   if (rc) return rc;
   if (plan->max_q_row > 0) {
     if (!out || !lse || !dout || !dq) CG_FAIL(CG_ERR_BAD_ARG, "%s: null tensor", name);
-    if (!ws || ws_bytes < cg_packed_attention_bwd_workspace_bytes(plan, in->q_rows, in->D, in->Dv))
+    const size_t need = cg_packed_attention_bwd_workspace_bytes(plan, in->q_rows, in->D, in->Dv);
+    if (need > 0 && (!ws || ws_bytes < need))
       CG_FAIL(CG_ERR_WORKSPACE, "%s: workspace of %zu bytes", name, ws_bytes);
   }
   if (plan->max_k_row > 0 && (!dk || !dv)) CG_FAIL(CG_ERR_BAD_ARG, "%s: null gradient", name);
@@ -1303,7 +1304,7 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   a.dk = (bf16_t*)dk;
   a.dv = (bf16_t*)dv;
   a.delta = (const float*)ws;
-  if (plan->max_q_row > 0) a.ws_o = (float*)((char*)ws + mha_delta_bytes(plan, in->q_rows));
+  if (ws) a.ws_o = (float*)((char*)ws + mha_delta_bytes(plan, in->q_rows));
   const hipStream_t st = (hipStream_t)stream;
   const int dp = mha_width(in->D, in->Dv);
   if (plan->dq_tiles) {

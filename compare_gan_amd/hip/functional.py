@@ -1059,8 +1059,11 @@ class PackedAttentionFn(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, q, k, v, plan, scale):
+    # checked and laid out once: the backward pass runs on what the forward pass ran on
+    scale = K._attention_input(q, k, v, plan, scale)   # pylint: disable=protected-access
+    q, k, v = (K._attention_operand(t) for t in (q, k, v))   # pylint: disable=protected-access
     wanted = any(ctx.needs_input_grad[:3])
-    out, lse = K.packed_attention_fwd(q, k, v, plan, scale, want_lse=wanted)
+    out, lse = K._attention_rows(q, k, v, plan, scale, wanted)   # pylint: disable=protected-access
     if wanted:
       ctx.save_for_backward(q, k, v, out, lse)
       ctx.plan, ctx.scale = plan, scale
@@ -1070,7 +1073,8 @@ class PackedAttentionFn(torch.autograd.Function):
   @torch.autograd.function.once_differentiable
   def backward(ctx, dout):
     q, k, v, out, lse = ctx.saved_tensors
-    dq, dk, dv = K.packed_attention_bwd(q, k, v, ctx.plan, out, lse, _bf16(dout), ctx.scale)
+    dout = K._attention_operand(_bf16(dout))   # pylint: disable=protected-access
+    dq, dk, dv = K._attention_grads(q, k, v, ctx.plan, out, lse, dout, ctx.scale)   # pylint: disable=protected-access
     return dq, dk, dv, None, None
 
 

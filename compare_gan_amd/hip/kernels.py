@@ -1429,7 +1429,12 @@ def packed_attention_fwd(q, k, v, plan, scale=None, want_lse=True, out=None):
     scale: 1 / sqrt(D) by default.  Rows of q outside every sequence give zeros -- or keep what `out`, if
     given (dense), holds there."""
     scale = _attention_input(q, k, v, plan, scale)
-    q, k, v = _attention_operand(q), _attention_operand(k), _attention_operand(v)
+    return _attention_rows(_attention_operand(q), _attention_operand(k), _attention_operand(v), plan, scale, want_lse,
+                           out)
+
+
+def _attention_rows(q, k, v, plan, scale, want_lse, out=None):
+    """packed_attention_fwd on operands that are known to fit."""
     shape = (q.shape[0], q.shape[1], v.shape[2])
     if out is None:
         out = _rows_out(shape, plan.q_dense, plan.q_rows, q.device)
@@ -1458,15 +1463,22 @@ def packed_attention_bwd(q, k, v, plan, out, lse, dout, scale=None):
         _req(t, dt, nm)
         if tuple(t.shape) != shp or t.device != q.device:
             raise ValueError("%s must be %s on %s" % (nm, list(shp), q.device))
-    out, dout = _attention_operand(out), _attention_operand(dout)
+    return _attention_grads(q, k, v, plan, _attention_operand(out), lse, _attention_operand(dout), scale)
+
+
+def _attention_grads(q, k, v, plan, out, lse, dout, scale):
+    """packed_attention_bwd on operands that are known to fit (Fn.packed_attention's backward)."""
     dq = _rows_out(q.shape, plan.q_dense, plan.q_rows, q.device)
     dk = _rows_out(k.shape, plan.k_dense, plan.k_rows, q.device)
     dv = _rows_out(v.shape, plan.k_dense, plan.k_rows, q.device)
-    ws = _ws(lib().cg_packed_attention_bwd_workspace_bytes(plan.ref, q.shape[0], q.shape[2], v.shape[2]), q)
+    ws, nbytes = None, 0
+    if plan.info.dq_tiles or plan.info.dkv_tiles:
+        nbytes = lib().cg_packed_attention_bwd_workspace_bytes(plan.ref, q.shape[0], q.shape[2], v.shape[2])
+        ws = _ws(nbytes, q)
     with _On(q) as stream:
         check(lib().cg_packed_attention_bwd(
             _attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(), out.data_ptr(), lse.data_ptr(),
-            dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel(), stream),
+            dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(ws), nbytes, stream),
             "cg_packed_attention_bwd")
     return dq, dk, dv
 

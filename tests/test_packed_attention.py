@@ -216,7 +216,9 @@ def test_entry_points_refuse_without_a_launch():
     assert call(entry, v=fake + 8) == -2 and call(entry, q=None) == -1
     assert call(entry, k_stride_t=2 ** 26) == -2
   assert call("fwd") == -1          # no output
-  assert call("bwd") == -4          # no workspace
+  plan = K.AttentionPlan([100], heads=2, kv_heads=1, device="cpu")     # (4 rows need none)
+  info = ctypes.byref(plan.info)
+  assert call("bwd", q_rows=100, k_rows=100) == -4                     # no workspace
   rows = _lib.HeadRows(fake, 64, 64, 1, None)
   r = ctypes.byref(rows)
   rot = _lib.Rotation(fake, fake, 1.0, 1, 64, 0)
