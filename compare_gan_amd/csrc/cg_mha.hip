@@ -48,10 +48,10 @@ struct MhaArgs {
   const int4* seqs;         // {q_start, q_len, k_start, k_len}
   const int4* items;        // two int4 an item
   bf16_t* out;
+  bf16_t* out_low;          // what the rounding of out left over (training): delta is formed from both
   float* lse;
   float* ws_o;              // partial results, in units of 32 rows: [unit][32][Dv]
   float* ws_ml;             //                                        [unit][32][2]
-  const bf16_t* o_in;
   const bf16_t* dout;
   const float* lse_in;
   const float* delta;
@@ -227,6 +227,18 @@ __device__ __forceinline__ void mha_accumulate(f32x16_t (&acc)[DP / 32], mha_lds
     }
   }
 }
+// what the rounding of the weights left over, for rows that see few keys (FEW): their O is the mean of a few values, the
+// error of their weights does not average out, and delta = dO . O carries it into every dS of the row
+template <int DP>
+__device__ __forceinline__ void mha_accumulate_low(f32x16_t (&acc)[DP / 32], mha_lds_ptr tile, const MhaReads<DP>& m,
+                                                   const f32x16_t& p, int sub) {
+  f32x16_t low;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) low[v] = p[v] - bf2f(f2bf(p[v]));
+  mha_accumulate<DP>(acc, tile, m, low, sub);
+}
+constexpr int FEW = 64;
+
 __device__ __forceinline__ int mha_key(int v, int half) { return (v & 3) + 8 * (v >> 2) + 4 * half; }
 
 // Running softmax over the 64 (NS = 2) or 32 (NS = 1) keys of s: in s the scores, out the weights
@@ -288,7 +300,7 @@ __device__ __forceinline__ void mha_store_part(float* dst, const f32x16_t (&o)[D
 }
 
 // what a wave leaves behind: O^T in registers -> out, or a partial result
-template <int DP>
+template <int DP, bool GRAD>
 __device__ __forceinline__ void mha_store(const MhaArgs& a, const MhaItem& it, int r, float m, float l,
                                           f32x16_t (&o)[DP / 32], int half) {
   if (r >= it.rows) return;
@@ -309,16 +321,24 @@ __device__ __forceinline__ void mha_store(const MhaArgs& a, const MhaItem& it, i
     for (int g = 0; g < 4; ++g) {
       const int d = t * 32 + g * 8 + 4 * half;
       if (d < a.Dv) {
-        const float w[4] = {o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv};
-        *reinterpret_cast<uint2*>(dst + d) = pack4_bf16(w);
+        float w[4] = {o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv};
+        const uint2 hi = pack4_bf16(w);
+        *reinterpret_cast<uint2*>(dst + d) = hi;
+        if (GRAD) {
+          w[0] -= __uint_as_float(hi.x << 16);
+          w[1] -= __uint_as_float(hi.x & 0xffff0000u);
+          w[2] -= __uint_as_float(hi.y << 16);
+          w[3] -= __uint_as_float(hi.y & 0xffff0000u);
+          *reinterpret_cast<uint2*>(a.out_low + row * a.Dv + d) = pack4_bf16(w);
+        }
       }
     }
   if (a.lse && half == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * (1.f / LOG2E);
 }
 
 // ---- forward, 128 rows x all keys of the item ---------------------------------------------------
-template <int DP>
-__global__ __launch_bounds__(256, 2) void mha_fwd_kernel(MhaArgs a) {
+template <int DP, bool GRAD>
+__global__ __launch_bounds__(256, DP <= 64 ? 4 : DP <= 96 ? 3 : 2) void mha_fwd_kernel(MhaArgs a) {
   constexpr int TILE = KT * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -379,15 +399,19 @@ __global__ __launch_bounds__(256, 2) void mha_fwd_kernel(MhaArgs a) {
     mha_softmax<2, DP / 32>(s, a.c, m, l, o);
     mha_accumulate<DP>(o, vs, rd, s[0], 0);
     mha_accumulate<DP>(o, vs, rd, s[1], 1);
+    if (GRAD && most < FEW) {
+      mha_accumulate_low<DP>(o, vs, rd, s[0], 0);
+      mha_accumulate_low<DP>(o, vs, rd, s[1], 1);
+    }
   }
   l += __shfl_xor(l, 32, 64);
-  mha_store<DP>(a, it, r, m, l, o, half);
+  mha_store<DP, GRAD>(a, it, r, m, l, o, half);
 }
 
 // ---- forward, at most 32 rows: the keys split over the waves --------------------------------------
 // One wave holds all rows; each of the NW waves takes every NW-th step of 32 keys through an LDS ring of its
 // own (no barrier in the loop), and the waves' results are joined at the end.  Bound by reading K and V.
-template <int DP, int NW>
+template <int DP, int NW, bool GRAD>
 __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
   constexpr int TILE = 32 * DP * 2;              // one matrix, 32 keys
   constexpr int RING = 2 * 2 * TILE;             // K and V, two buffers, a wave
@@ -450,6 +474,7 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
     }
     mha_softmax<1, DP / 32>(s, a.c, m, l, o);
     mha_accumulate<DP>(o, vs, rd, s[0], 0);
+    if (GRAD && it.k1 <= FEW) mha_accumulate_low<DP>(o, vs, rd, s[0], 0);
   }
   l += __shfl_xor(l, 32, 64);
   if constexpr (NW > 1) {
@@ -492,7 +517,7 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
     m = top;
     l = total;
   }
-  mha_store<DP>(a, it, col, m, l, o, half);
+  mha_store<DP, GRAD>(a, it, col, m, l, o, half);
 }
 
 // ---- joins the partial results of a split item; one wave a row, its parts' loads in flight together ------
@@ -534,26 +559,33 @@ __global__ __launch_bounds__(256) void mha_join_kernel(MhaArgs a) {
     const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-      if (lane + 64 * j < a.Dv) a.out[row * a.Dv + lane + 64 * j] = f2bf(acc[j] * inv);
+      if (lane + 64 * j < a.Dv) {
+        const float x = acc[j] * inv;
+        const bf16_t hi = f2bf(x);
+        a.out[row * a.Dv + lane + 64 * j] = hi;
+        if (a.out_low) a.out_low[row * a.Dv + lane + 64 * j] = f2bf(x - bf2f(hi));
+      }
     if (a.lse && lane == 0)
       a.lse[row] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * (1.f / LOG2E);
   }
 }
 
 // ---- backward -----------------------------------------------------------------------------------
-// delta[row] = sum_d dout out; 16 lanes a row, 8 elements each
-__global__ __launch_bounds__(256) void mha_delta_kernel(const bf16_t* __restrict__ out,
+// delta[row] = sum_d dout (out + out_low); 16 lanes a row, 8 elements each.  dS = P (dP - delta) is a difference: with
+// the rounded out alone its error would come on top of the rounding of dS (dQ 1.5 instead of 1.4 roundings off).
+__global__ __launch_bounds__(256) void mha_delta_kernel(const bf16_t* __restrict__ out, const bf16_t* __restrict__ low,
                                                         const bf16_t* __restrict__ dout, int64_t rows, int Dv,
                                                         float* __restrict__ delta) {
   const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   const int d = (threadIdx.x & 15) * 8;
   float s = 0.f;
   if (row < rows && d < Dv) {
-    float x[8], y[8];
+    float x[8], y[8], z[8];
     unpack8_bf16(*reinterpret_cast<const uint4*>(out + row * Dv + d), x);
+    unpack8_bf16(*reinterpret_cast<const uint4*>(low + row * Dv + d), z);
     unpack8_bf16(*reinterpret_cast<const uint4*>(dout + row * Dv + d), y);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += x[j] * y[j];
+    for (int j = 0; j < 8; ++j) s += (x[j] + z[j]) * y[j];
   }
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -1011,17 +1043,23 @@ void mha_deal(std::vector<Work>* items, int units) {
 }
 
 // A launch's items are split along the axis that they sum over (keys; rows for dK and dV) where one item is longer
-// than its share of the launch: the total over so many blocks (2 resident a CU, 256 CUs, a few rounds), but no part
-// below a length at which its fp32 result, written once and read once, is small against its own work.
-constexpr int64_t TILE_BLOCKS = 512, THIN_BLOCKS = 1024, GRAD_BLOCKS = 1024;
-constexpr int TILE_SPLIT_MIN = 512, THIN_SPLIT_MIN = 512, GRAD_SPLIT_MIN = 512;
+// than its share of the launch.  A tile item's share is the total over 1024 (half of what one of the chip's 512 places,
+// 2 workgroups a CU, has to do: the longest items no longer delay the end; ragged batch of 25 k rows: dK / dV 330 us,
+// with the total over 512 402 us), but not below 1024 keys or rows where the total over 512 is more (a part's fp32
+// result, written once and read once, has to be small against its work; one sequence of 8192, 2 heads of 128, causal:
+// backward 206 us, in parts of 512 rows 231 us), and not below 512 at all.  Thin items are half as long: no tile of 128.
 constexpr int THIN1_KEYS = 128;     // up to so many keys one wave does a thin item alone
 
-void mha_split(std::vector<Work>* items, int64_t blocks, int step, int least, int tile, int units_a_part,
-               const std::vector<int64_t>& length, std::vector<Work>* joins, int64_t* parts) {
+int64_t mha_share(int64_t all, bool thin) {
+  const int64_t most = (all + 511) / 512, half = (all + 1023) / 1024;
+  return std::max<int64_t>(512, thin ? half : std::min(most, std::max<int64_t>(1024, half)));
+}
+
+void mha_split(std::vector<Work>* items, int step, int tile, int units_a_part, const std::vector<int64_t>& length,
+               std::vector<Work>* joins, int64_t* parts) {
   int64_t all = 0;
   for (const Work& w : *items) all += w.v[4] - w.v[3];
-  const int64_t chunk = std::max<int64_t>(least, (all + blocks - 1) / blocks);
+  const int64_t chunk = mha_share(all, tile == THIN_ROWS);
   std::vector<Work> out;
   for (const Work& w : *items) {
     const int64_t len = w.v[4] - w.v[3], steps = (len + step - 1) / step;
@@ -1085,10 +1123,10 @@ int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_star
     }
   }
   int64_t parts = 0, dq_parts = 0, dkv_parts = 0;
-  mha_split(&tiles, TILE_BLOCKS, KT, TILE_SPLIT_MIN, ROW_TILE, ROW_TILE / 32, all_rows, &joins, &parts);
-  mha_split(&thin4, THIN_BLOCKS, 32, THIN_SPLIT_MIN, THIN_ROWS, 1, all_rows, &joins, &parts);
-  mha_split(&dq, GRAD_BLOCKS, KT, GRAD_SPLIT_MIN, ROW_TILE, 1, all_rows, &dq_joins, &dq_parts);
-  mha_split(&dkv, GRAD_BLOCKS, KT, GRAD_SPLIT_MIN, KEY_TILE, 1, all_keys, &dkv_joins, &dkv_parts);
+  mha_split(&tiles, KT, ROW_TILE, ROW_TILE / 32, all_rows, &joins, &parts);
+  mha_split(&thin4, 32, THIN_ROWS, 1, all_rows, &joins, &parts);
+  mha_split(&dq, KT, ROW_TILE, 1, all_rows, &dq_joins, &dq_parts);
+  mha_split(&dkv, KT, KEY_TILE, 1, all_keys, &dkv_joins, &dkv_parts);
   if (parts > 0x7fffffff || dq_parts > 0x7fffffff || dkv_parts > 0x7fffffff) CG_FAIL(CG_ERR_UNSUPPORTED, "cg_host_attention_plan: too many partial results");
   const int units = B * kv_heads;
   std::vector<Work>* lists[9] = {&tiles, &thin4, &thin1, &joins, &dq, &dq_joins, &dkv, &dkv_joins, &small};
@@ -1192,9 +1230,12 @@ int mha_width(int D, int Dv) { return ((D > Dv ? D : Dv) + 31) / 32 * 32; }
     case 96: kernel(96)<<<grid, block, 0, st>>>(args); break;                  \
     default: kernel(128)<<<grid, block, 0, st>>>(args); break;                 \
   }
-#define MHA_FWD(dp) mha_fwd_kernel<dp>
-#define MHA_THIN4(dp) mha_thin_kernel<dp, 4>
-#define MHA_THIN1(dp) mha_thin_kernel<dp, 1>
+#define MHA_FWD(dp) mha_fwd_kernel<dp, false>
+#define MHA_THIN4(dp) mha_thin_kernel<dp, 4, false>
+#define MHA_THIN1(dp) mha_thin_kernel<dp, 1, false>
+#define MHA_FWD_GRAD(dp) mha_fwd_kernel<dp, true>
+#define MHA_THIN4_GRAD(dp) mha_thin_kernel<dp, 4, true>
+#define MHA_THIN1_GRAD(dp) mha_thin_kernel<dp, 1, true>
 #define MHA_BWD_Q(dp) mha_bwd_q_kernel<dp>
 #define MHA_BWD_KV(dp) mha_bwd_kv_kernel<dp>
 #define MHA_BWD_SMALL(dp) mha_bwd_small_kernel<dp>
@@ -1230,17 +1271,19 @@ extern "C" size_t cg_packed_attention_fwd_workspace_bytes(const cgAttentionPlan*
 }
 
 extern "C" int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAttentionPlan* plan, const int32_t* data,
-                                       void* out, float* lse, void* ws, size_t ws_bytes, cgStream stream) {
+                                       void* out, void* out_low, float* lse, void* ws, size_t ws_bytes,
+                                       cgStream stream) {
   const char* name = "cg_packed_attention_fwd";
   MhaArgs a = {};
   const int rc = mha_check(name, in, plan, data, &a);
   if (rc) return rc;
   if (plan->max_q_row == 0) return CG_OK;
   if (!out) CG_FAIL(CG_ERR_BAD_ARG, "%s: null output", name);
-  if ((uintptr_t)out % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: tensors have to be 16-byte aligned", name);
+  if ((uintptr_t)out % 16 || (uintptr_t)out_low % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: tensors have to be 16-byte aligned", name);
   if (plan->parts > 0 && (!ws || ws_bytes < cg_packed_attention_fwd_workspace_bytes(plan, in->Dv)))
     CG_FAIL(CG_ERR_WORKSPACE, "%s: workspace of %zu bytes", name, ws_bytes);
   a.out = (bf16_t*)out;
+  a.out_low = (bf16_t*)out_low;
   a.lse = lse;
   a.ws_o = (float*)ws;
   a.ws_ml = a.ws_o + plan->parts * THIN_ROWS * (int64_t)in->Dv;
@@ -1248,17 +1291,29 @@ extern "C" int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAtten
   const int dp = mha_width(in->D, in->Dv);
   if (plan->tiles) {
     a.items = mha_list(plan, data, 0);
-    MHA_LAUNCH(dp, MHA_FWD, plan->tiles, 256, st, a);
+    if (out_low) {
+      MHA_LAUNCH(dp, MHA_FWD_GRAD, plan->tiles, 256, st, a);
+    } else {
+      MHA_LAUNCH(dp, MHA_FWD, plan->tiles, 256, st, a);
+    }
     CG_CHECK_LAUNCH(name);
   }
   if (plan->thin4) {
     a.items = mha_list(plan, data, 1);
-    MHA_LAUNCH(dp, MHA_THIN4, plan->thin4, 256, st, a);
+    if (out_low) {
+      MHA_LAUNCH(dp, MHA_THIN4_GRAD, plan->thin4, 256, st, a);
+    } else {
+      MHA_LAUNCH(dp, MHA_THIN4, plan->thin4, 256, st, a);
+    }
     CG_CHECK_LAUNCH(name);
   }
   if (plan->thin1) {
     a.items = mha_list(plan, data, 2);
-    MHA_LAUNCH(dp, MHA_THIN1, plan->thin1, 64, st, a);
+    if (out_low) {
+      MHA_LAUNCH(dp, MHA_THIN1_GRAD, plan->thin1, 64, st, a);
+    } else {
+      MHA_LAUNCH(dp, MHA_THIN1, plan->thin1, 64, st, a);
+    }
     CG_CHECK_LAUNCH(name);
   }
   if (plan->joins) {
@@ -1281,23 +1336,22 @@ extern "C" size_t cg_packed_attention_bwd_workspace_bytes(const cgAttentionPlan*
 }
 
 extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAttentionPlan* plan, const int32_t* data,
-                                       const void* out, const float* lse, const void* dout, void* dq, void* dk,
-                                       void* dv, void* ws, size_t ws_bytes, cgStream stream) {
+                                       const void* out, const void* out_low, const float* lse, const void* dout,
+                                       void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, cgStream stream) {
   const char* name = "cg_packed_attention_bwd";
   MhaArgs a = {};
   const int rc = mha_check(name, in, plan, data, &a);
   if (rc) return rc;
   if (plan->max_q_row > 0) {
-    if (!out || !lse || !dout || !dq) CG_FAIL(CG_ERR_BAD_ARG, "%s: null tensor", name);
+    if (!out || !lse || !dout || !dq || (plan->dq_tiles && !out_low)) CG_FAIL(CG_ERR_BAD_ARG, "%s: null tensor", name);
     const size_t need = cg_packed_attention_bwd_workspace_bytes(plan, in->q_rows, in->D, in->Dv);
     if (need > 0 && (!ws || ws_bytes < need))
       CG_FAIL(CG_ERR_WORKSPACE, "%s: workspace of %zu bytes", name, ws_bytes);
   }
   if (plan->max_k_row > 0 && (!dk || !dv)) CG_FAIL(CG_ERR_BAD_ARG, "%s: null gradient", name);
-  const void* ptr[6] = {out, dout, dq, dk, dv, ws};
+  const void* ptr[7] = {out, out_low, dout, dq, dk, dv, ws};
   for (const void* p : ptr)
     if ((uintptr_t)p % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: tensors have to be 16-byte aligned", name);
-  a.o_in = (const bf16_t*)out;
   a.lse_in = lse;
   a.dout = (const bf16_t*)dout;
   a.dq = (bf16_t*)dq;
@@ -1310,7 +1364,8 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   if (plan->dq_tiles) {
     const int64_t rows = (int64_t)in->q_rows * plan->heads;
     if (rows > (int64_t)0x7fffffff * 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: too many rows", name);
-    mha_delta_kernel<<<(uint32_t)((rows + 15) / 16), 256, 0, st>>>(a.o_in, a.dout, rows, a.Dv, (float*)ws);
+    mha_delta_kernel<<<(uint32_t)((rows + 15) / 16), 256, 0, st>>>((const bf16_t*)out, (const bf16_t*)out_low, a.dout, rows, a.Dv,
+                                                                    (float*)ws);
     CG_CHECK_LAUNCH(name);
     a.items = mha_list(plan, data, 4);
     MHA_LAUNCH(dp, MHA_BWD_Q, plan->dq_tiles, 256, st, a);

@@ -203,9 +203,9 @@ SIGNATURES = {
                                       c_sz, vp]),
     "cg_host_attention_plan": (c_int, [vp, vp, vp, vp, c_int, c_int, c_int, c_int, vp, c_i64, vp]),
     "cg_packed_attention_fwd_workspace_bytes": (c_sz, [vp, c_int]),
-    "cg_packed_attention_fwd": (c_int, [vp, vp, vp, vp, vp, vp, c_sz, vp]),
+    "cg_packed_attention_fwd": (c_int, [vp, vp, vp, vp, vp, vp, vp, c_sz, vp]),
     "cg_packed_attention_bwd_workspace_bytes": (c_sz, [vp, c_int, c_int, c_int]),
-    "cg_packed_attention_bwd": (c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, c_sz, vp]),
+    "cg_packed_attention_bwd": (c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, c_sz, vp]),
     "cg_gan_loss": (c_int, [c_int, vp, c_int, vp, vp, vp, vp]),
     "cg_softmax_xent_eps": (c_int, [vp, vp, c_int, c_int, c_f32, vp, vp, vp]),
     "cg_s3gan_labels": (c_int, [vp, vp, c_int, c_int, c_int, vp, vp, vp]),

@@ -1063,19 +1063,19 @@ class PackedAttentionFn(torch.autograd.Function):
     scale = K._attention_input(q, k, v, plan, scale)   # pylint: disable=protected-access
     q, k, v = (K._attention_operand(t) for t in (q, k, v))   # pylint: disable=protected-access
     wanted = any(ctx.needs_input_grad[:3])
-    out, lse = K._attention_rows(q, k, v, plan, scale, wanted)   # pylint: disable=protected-access
+    out, saved = K._attention_rows(q, k, v, plan, scale, wanted)   # pylint: disable=protected-access
     if wanted:
-      ctx.save_for_backward(q, k, v, out, lse)
+      ctx.save_for_backward(q, k, v, out, *saved)
       ctx.plan, ctx.scale = plan, scale
     return out
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, dout):
-    q, k, v, out, lse = ctx.saved_tensors
+    q, k, v, out, lse, low = ctx.saved_tensors
     dout = K._attention_operand(_bf16(dout))   # pylint: disable=protected-access
-    dq, dk, dv = K._attention_grads(q, k, v, ctx.plan, out, lse, dout, ctx.scale)   # pylint: disable=protected-access
-    return dq, dk, dv, None, None
+    grads = K._attention_grads(q, k, v, ctx.plan, out, lse, low, dout, ctx.scale)   # pylint: disable=protected-access
+    return grads + (None, None)
 
 
 def packed_attention(q, k, v, plan, scale=None):

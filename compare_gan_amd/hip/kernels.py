@@ -1423,17 +1423,18 @@ def _rows_out(shape, dense, used, device, dtype=BF16):
     return torch.zeros(shape, dtype=dtype, device=device)
 
 
-def packed_attention_fwd(q, k, v, plan, scale=None, want_lse=True, out=None):
+def packed_attention_fwd(q, k, v, plan, scale=None, want_grad=True, out=None):
     """softmax(scale q k^T) v over the plan's sequences: q [rows, heads, D], k [rows, kv_heads, D],
-    v [rows, kv_heads, Dv] bf16 -> out [rows, heads, Dv] bf16, lse [rows, heads] fp32 (or None).
-    scale: 1 / sqrt(D) by default.  Rows of q outside every sequence give zeros -- or keep what `out`, if
-    given (dense), holds there."""
+    v [rows, kv_heads, Dv] bf16 -> (out [rows, heads, Dv] bf16, saved).  saved: what packed_attention_bwd needs
+    (lse [rows, heads] fp32, and what the rounding of out left over, or None where the plan has no use for it);
+    None without want_grad.  scale: 1 / sqrt(D) by default.  Rows of q outside every sequence give zeros -- or keep
+    what `out`, if given (dense), holds there."""
     scale = _attention_input(q, k, v, plan, scale)
-    return _attention_rows(_attention_operand(q), _attention_operand(k), _attention_operand(v), plan, scale, want_lse,
+    return _attention_rows(_attention_operand(q), _attention_operand(k), _attention_operand(v), plan, scale, want_grad,
                            out)
 
 
-def _attention_rows(q, k, v, plan, scale, want_lse, out=None):
+def _attention_rows(q, k, v, plan, scale, want_grad, out=None):
     """packed_attention_fwd on operands that are known to fit."""
     shape = (q.shape[0], q.shape[1], v.shape[2])
     if out is None:
@@ -1442,31 +1443,42 @@ def _attention_rows(q, k, v, plan, scale, want_lse, out=None):
         _req(out, BF16, "out")
         if tuple(out.shape) != shape or out.device != q.device or out.data_ptr() % 16:
             raise ValueError("out must be %s on %s, 16-byte aligned" % (list(shape), q.device))
-    lse = torch.empty(shape[:2], dtype=F32, device=q.device) if want_lse else None
+    lse = low = None
+    if want_grad:
+        lse = torch.empty(shape[:2], dtype=F32, device=q.device)
+        if plan.info.dq_tiles:
+            low = torch.empty(shape, dtype=BF16, device=q.device)
     nbytes, ws = 0, None
     if plan.info.parts:
         nbytes = lib().cg_packed_attention_fwd_workspace_bytes(plan.ref, shape[2])
         ws = _ws(nbytes, q)
     with _On(q) as stream:
         check(lib().cg_packed_attention_fwd(_attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(),
-                                            out.data_ptr(), _p(lse), _p(ws), nbytes, stream),
+                                            out.data_ptr(), _p(low), _p(lse), _p(ws), nbytes, stream),
               "cg_packed_attention_fwd")
-    return out, lse
+    return out, (lse, low) if want_grad else None
 
 
-def packed_attention_bwd(q, k, v, plan, out, lse, dout, scale=None):
-    """Gradients of packed_attention_fwd: dq, dk, dv, dense bf16 with zeros outside every sequence."""
+def packed_attention_bwd(q, k, v, plan, out, saved, dout, scale=None):
+    """Gradients of packed_attention_fwd (`saved`: its second result): dq, dk, dv, dense bf16 with zeros outside
+    every sequence."""
     scale = _attention_input(q, k, v, plan, scale)
     q, k, v = _attention_operand(q), _attention_operand(k), _attention_operand(v)
     shape = (q.shape[0], q.shape[1], v.shape[2])
-    for t, nm, dt, shp in ((out, "out", BF16, shape), (dout, "dout", BF16, shape), (lse, "lse", F32, shape[:2])):
+    if saved is None:
+        raise ValueError("saved must be the second result of packed_attention_fwd(want_grad=True)")
+    lse, low = saved
+    for t, nm, dt, shp in ((out, "out", BF16, shape), (dout, "dout", BF16, shape), (lse, "lse", F32, shape[:2]),
+                           (low, "the rest of out", BF16, shape)):
+        if t is None and nm == "the rest of out" and not plan.info.dq_tiles:
+            continue
         _req(t, dt, nm)
         if tuple(t.shape) != shp or t.device != q.device:
             raise ValueError("%s must be %s on %s" % (nm, list(shp), q.device))
-    return _attention_grads(q, k, v, plan, _attention_operand(out), lse, _attention_operand(dout), scale)
+    return _attention_grads(q, k, v, plan, _attention_operand(out), lse, low, _attention_operand(dout), scale)
 
 
-def _attention_grads(q, k, v, plan, out, lse, dout, scale):
+def _attention_grads(q, k, v, plan, out, lse, low, dout, scale):
     """packed_attention_bwd on operands that are known to fit (Fn.packed_attention's backward)."""
     dq = _rows_out(q.shape, plan.q_dense, plan.q_rows, q.device)
     dk = _rows_out(k.shape, plan.k_dense, plan.k_rows, q.device)
@@ -1477,7 +1489,7 @@ def _attention_grads(q, k, v, plan, out, lse, dout, scale):
         ws = _ws(nbytes, q)
     with _On(q) as stream:
         check(lib().cg_packed_attention_bwd(
-            _attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            _attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(), out.data_ptr(), _p(low), lse.data_ptr(),
             dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(ws), nbytes, stream),
             "cg_packed_attention_bwd")
     return dq, dk, dv

@@ -610,7 +610,8 @@ int cg_host_attention_plan(const int32_t* q_start, const int32_t* q_len, const i
                            int32_t* data_host, int64_t capacity, cgAttentionPlan* info);
 /* q [q_rows, heads, D], k [k_rows, kv_heads, D], v [k_rows, kv_heads, Dv] bf16, strides in elements, heads
  * contiguous inside; D and Dv multiples of 8, at most 128; scale > 0.  out [q_rows, heads, Dv] contiguous,
- * lse [q_rows, heads] fp32 (NULL: not wanted).  Rows that see no key: out 0, lse -inf.  Rows that belong to
+ * lse [q_rows, heads] fp32 and out_low like out (what its rounding left over): for the backward pass, NULL where
+ * none follows (out_low also where plan->dq_tiles is 0).  Rows that see no key: out 0, lse -inf.  Rows that belong to
  * no sequence are left as they were. */
 typedef struct {
   const void *q, *k, *v;
@@ -620,14 +621,14 @@ typedef struct {
 } cgAttentionInput;
 size_t cg_packed_attention_fwd_workspace_bytes(const cgAttentionPlan* plan, int Dv);
 int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAttentionPlan* plan, const int32_t* data,
-                            void* out, float* lse, void* ws, size_t ws_bytes, cgStream stream);
-/* Gradients: out, lse of the forward pass, dout [q_rows, heads, Dv] contiguous; dq [q_rows, heads, D],
+                            void* out, void* out_low, float* lse, void* ws, size_t ws_bytes, cgStream stream);
+/* Gradients: out, out_low, lse of the forward pass, dout [q_rows, heads, Dv] contiguous; dq [q_rows, heads, D],
  * dk [k_rows, kv_heads, D], dv [k_rows, kv_heads, Dv] contiguous bf16, every row of a sequence written
  * (the shared heads of a key head summed inside, no atomics). */
 size_t cg_packed_attention_bwd_workspace_bytes(const cgAttentionPlan* plan, int q_rows, int D, int Dv);
 int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAttentionPlan* plan, const int32_t* data,
-                            const void* out, const float* lse, const void* dout, void* dq, void* dk,
-                            void* dv, void* ws, size_t ws_bytes, cgStream stream);
+                            const void* out, const void* out_low, const float* lse, const void* dout,
+                            void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, cgStream stream);
 
 /* ------------------------------------------------------------------------------------------
  * Losses (gans/loss_lib.py:53-148) and WGAN-GP (gans/penalty_lib.py:59-82).

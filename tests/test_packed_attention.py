@@ -205,8 +205,8 @@ def test_entry_points_refuse_without_a_launch():
     f.update(kw)
     arg = ctypes.byref(_lib.AttentionInput(*[f[n] for n, _ in _lib.AttentionInput._fields_]))
     if entry == "fwd":
-      return lib.cg_packed_attention_fwd(arg, info, fake, None, None, None, 0, None)
-    return lib.cg_packed_attention_bwd(arg, info, fake, fake, fake, fake, fake, fake, fake, None, 0, None)
+      return lib.cg_packed_attention_fwd(arg, info, fake, None, None, None, None, 0, None)
+    return lib.cg_packed_attention_bwd(arg, info, fake, fake, fake, fake, fake, fake, fake, fake, None, 0, None)
   for entry in ("fwd", "bwd"):
     assert call(entry, D=60) == -2 and call(entry, Dv=136) == -2 and call(entry, D=0) == -2
     assert call(entry, scale=0.0) == -1 and call(entry, scale=float("nan")) == -1

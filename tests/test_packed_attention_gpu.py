@@ -5,7 +5,7 @@ Tolerances count roundings.  A value rounded to bf16 is off by at most half a st
 2^-24.  Attention: the weights P enter the matrix instruction in bf16, so |out - exact| <= HB sum_j P_j |v_j| (weights)
 + HB |out| (the result), plus the weights' own relative error rp: a score is a fp32 sum of D products, off by at most
 D HF sum |q k| scale, and the exponential and the sum of the weights add some 2^-20.  Backward likewise, with the error
-of delta = sum dout out (out was rounded) and of dS on its way into the matrix instruction.
+of delta = sum dout out (out and what its rounding left: 2^-16 of it) and of dS on its way into the matrix instruction.
 """
 import math
 import random
@@ -261,8 +261,9 @@ def exact_attention(q, k, v, dout, seqs, heads, kv_heads, causal, scale):
       dp = e @ c.t()
       delta = (e * o).sum(-1, keepdim=True)
       ds = p * (dp - delta)
-      # dP is a fp32 sum of Dv products; delta meets the rounded out; dS is rounded once
-      tds = (HB + rp) * ds.abs() + p * ((e.abs() * to).sum(-1, keepdim=True) +
+      # dP is a fp32 sum of Dv products; delta meets out's own error (its weights' roundings) and the rest of its
+      # rounding; dS is rounded once
+      tds = (HB + rp) * ds.abs() + p * ((e.abs() * (to - (HB - HB * HB) * o.abs())).sum(-1, keepdim=True) +
                                         (v.shape[2] * HF + rp) * (e.abs() @ c.abs().t()))
       res["dv"][0][k0:k0 + lk, h // g] += p.t() @ e
       res["dv"][1][k0:k0 + lk, h // g] += (HB + rp) * (p.t() @ e.abs())
@@ -454,13 +455,13 @@ def test_statistics_of_rows(K):
   gen = torch.Generator().manual_seed(6)
   q, k = normal(gen, (40, 1, 32)), normal(gen, (20, 1, 32))
   plan = K.AttentionPlan([40], [20], causal=True)
-  out, lse = K.packed_attention_fwd(q.cuda(), k.cuda(), k.cuda(), plan)
+  out, (lse, _) = K.packed_attention_fwd(q.cuda(), k.cuda(), k.cuda(), plan)
   s = q[:, 0].double() @ k[:, 0].double().t() / math.sqrt(32)
   s = s.masked_fill(torch.arange(20)[None] > torch.arange(40)[:, None] - 20, -math.inf)
   want = torch.logsumexp(s, -1)
   assert (lse[:20, 0] == -math.inf).all() and (out[:20] == 0).all()
   assert ((lse[20:, 0].cpu() - want[20:]).abs() < 1e-5).all()
-  assert K.packed_attention_fwd(q.cuda(), k.cuda(), k.cuda(), plan, want_lse=False)[1] is None
+  assert K.packed_attention_fwd(q.cuda(), k.cuda(), k.cuda(), plan, want_grad=False)[1] is None
 
 
 def test_infinite_and_missing_values_stay_in_their_rows(K, Fn):
@@ -537,9 +538,9 @@ def test_attention_refusals(K, Fn):
       Fn.packed_attention(**dict(good, **bad))
   with pytest.raises(ValueError):
     K.packed_attention_fwd(out=z(4, 2, 16), **good)
-  out, lse = K.packed_attention_fwd(**good)
+  out, saved = K.packed_attention_fwd(**good)
   with pytest.raises(ValueError):
-    K.packed_attention_bwd(good["q"], good["k"], good["v"], plan, out, lse, z(4, 2, 16))
+    K.packed_attention_bwd(good["q"], good["k"], good["v"], plan, out, saved, z(4, 2, 16))
   with pytest.raises(ValueError):
     K.packed_attention_bwd(good["q"], good["k"], good["v"], plan, out, None, out)
   q = z(4, 2, 16).requires_grad_(True)                # no second derivative: refused, not wrong
@@ -626,8 +627,8 @@ def test_captured_and_replayed(K, Fn):
 
   def step():
     a, b = K.qk_norm_rotary(q, k, gain, gain, pos, table)
-    out, lse = K.packed_attention_fwd(a, cache_k, cache_v, plan)
-    grads = K.packed_attention_bwd(a, cache_k, cache_v, plan, out, lse, dout)
+    out, saved = K.packed_attention_fwd(a, cache_k, cache_v, plan)
+    grads = K.packed_attention_bwd(a, cache_k, cache_v, plan, out, saved, dout)
     back = K.qk_norm_rotary_bwd(q, k, gain, gain, pos, table, grads[0], b)
     return (out, K.rotary(b, pos, table)) + grads + back
   side = torch.cuda.Stream()
