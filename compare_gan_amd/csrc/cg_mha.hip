@@ -227,6 +227,34 @@ __device__ __forceinline__ void mha_accumulate(f32x16_t (&acc)[DP / 32], mha_lds
     }
   }
 }
+// Entries that are not finite, where a causal mask cuts through a tile: a masked weight is 0, but 0 times an infinity or
+// NaN is NaN.  The tile's threads look its 16-byte chunks over, put zeros for such entries and keep the first (LAST: the
+// last) row that held one; the caller makes NaN of every result that sees that row.  So a value that is not finite reaches
+// whole rows here (elsewhere the entries that the product brings it to), and only those that see it.  Costs one read of
+// the tile by its workgroup, in tiles on the diagonal only.
+template <int DP, int ROWS, int NT, bool LAST>
+__device__ __forceinline__ void mha_clean(unsigned char* tile, int thread, int* bad) {
+  constexpr int CH = DP / 8, TOTAL = ROWS * CH;
+  static_assert(TOTAL % NT == 0, "chunks per thread");
+#pragma unroll 1
+  for (int i = thread; i < TOTAL; i += NT) {
+    uint4* at = reinterpret_cast<uint4*>(tile + i * 16);
+    uint4 q = *at;
+    const uint32_t odd = ((q.x & 0x7f807f80u) + 0x00800080u) | ((q.y & 0x7f807f80u) + 0x00800080u) |
+                         ((q.z & 0x7f807f80u) + 0x00800080u) | ((q.w & 0x7f807f80u) + 0x00800080u);
+    if (odd & 0x80008000u) {
+      s16x8_t v = __builtin_bit_cast(s16x8_t, q);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if ((v[e] & 0x7f80) == 0x7f80) v[e] = 0;
+      *at = __builtin_bit_cast(uint4, v);
+      if (LAST) atomicMax(bad, i / CH);
+      else atomicMin(bad, i / CH);
+    }
+  }
+}
+constexpr int NONE_BAD = 0x40000000;    // no row (LAST: its negative)
+
 // what the rounding of the weights left over, for rows that see few keys (FEW): their O is the mean of a few values, the
 // error of their weights does not average out, and delta = dO . O carries it into every dS of the row
 template <int DP>
@@ -288,14 +316,16 @@ __device__ __forceinline__ void mha_token(const MhaArgs& a, const MhaItem& it, i
 
 // a lane's row of an accumulator, fp32, to a partial result
 template <int DP>
-__device__ __forceinline__ void mha_store_part(float* dst, const f32x16_t (&o)[DP / 32], int width, int half) {
+__device__ __forceinline__ void mha_store_part(float* dst, const f32x16_t (&o)[DP / 32], int width, int half,
+                                               float f = 1.f) {
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = t * 32 + g * 8 + 4 * half;
       if (d < width)
-        *reinterpret_cast<float4*>(dst + d) = make_float4(o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]);
+        *reinterpret_cast<float4*>(dst + d) =
+            make_float4(o[t][4 * g] * f, o[t][4 * g + 1] * f, o[t][4 * g + 2] * f, o[t][4 * g + 3] * f);
     }
 }
 
@@ -341,9 +371,11 @@ template <int DP, bool GRAD>
 __global__ __launch_bounds__(256, DP <= 64 ? 4 : DP <= 96 ? 3 : 2) void mha_fwd_kernel(MhaArgs a) {
   constexpr int TILE = KT * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
+  __shared__ int sm_bad[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
   const MhaItem it = mha_item(a, blockIdx.x);
+  const int cut = a.causal ? (int)fdiv((uint32_t)it.row0, a.dG) + it.shift : NONE_BAD;   // last key of the first row
   const int r = it.row0 + wave * 32 + col;
   int t, h;
   mha_token(a, it, r, &t, &h);
@@ -381,9 +413,15 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : DP <= 96 ? 3 : 2) void mha_fwd_
   mha_settle(qf);
   int buf = 0;
   for (int k0 = it.k0; k0 < it.k1; k0 += KT, buf ^= 1) {
+    if (threadIdx.x == 0) sm_bad[buf] = NONE_BAD;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (k0 + KT < it.k1) stage(k0 + KT, buf ^ 1);
+    if (k0 + KT - 1 > cut) {                       // the diagonal
+      mha_clean<DP, KT, 256, false>(smem + buf * 2 * TILE + TILE, threadIdx.x, &sm_bad[buf]);
+      __syncthreads();
+      if (k0 + sm_bad[buf] <= last) l = __builtin_nanf("");
+    }
     if (k0 > most) continue;
     mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
     f32x16_t s[2];
@@ -417,6 +455,7 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
   constexpr int RING = 2 * 2 * TILE;             // K and V, two buffers, a wave
   __shared__ __attribute__((aligned(1024))) unsigned char smem[NW * RING];
   __shared__ float sm_m[NW][32], sm_l[NW][32];
+  __shared__ int sm_bad[NW];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
   const MhaItem it = mha_item(a, blockIdx.x);
@@ -466,6 +505,12 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
+    if (a.causal && k0 + 31 > least) {             // the diagonal: this wave's own tile and flag
+      if (lane == 0) sm_bad[wave] = NONE_BAD;
+      mha_clean<DP, 32, 64, false>(smem + wave * RING + buf * 2 * TILE + TILE, lane, &sm_bad[wave]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (k0 + *(volatile int*)&sm_bad[wave] <= last) l = __builtin_nanf("");
+    }
     f32x16_t s[1];
     s[0] = mha_product<DP>(ks, rd, qf, 0);
     if (k0 + 31 > least) {
@@ -600,9 +645,11 @@ template <int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArgs a) {
   constexpr int TILE = KT * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
+  __shared__ int sm_bad[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
   const MhaItem it = mha_item(a, blockIdx.x);
+  const int cut = a.causal ? (int)fdiv((uint32_t)it.row0, a.dG) + it.shift : NONE_BAD;   // last key of the first row
   const int r = it.row0 + wave * 32 + col;
   int t, h;
   mha_token(a, it, r, &t, &h);
@@ -639,13 +686,20 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dq[i] = mha_zero();
   if (it.k0 < it.k1) stage(it.k0, 0);
+  float scale = a.scale;         // NaN: the row saw a key that is not finite
   mha_settle(qf);
   mha_settle(df);
   int buf = 0;
   for (int k0 = it.k0; k0 < it.k1; k0 += KT, buf ^= 1) {
+    if (threadIdx.x == 0) sm_bad[buf] = NONE_BAD;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (k0 + KT < it.k1) stage(k0 + KT, buf ^ 1);
+    if (k0 + KT - 1 > cut) {                       // the diagonal
+      mha_clean<DP, KT, 256, false>(smem + buf * 2 * TILE, threadIdx.x, &sm_bad[buf]);
+      __syncthreads();
+      if (k0 + sm_bad[buf] <= last) scale = __builtin_nanf("");
+    }
     if (k0 > most) continue;
     mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
 #pragma unroll
@@ -665,7 +719,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
   }
   if (!ok) return;
   if (it.part >= 0) {
-    mha_store_part<DP>(a.ws_o + ((int64_t)it.part * ROW_TILE + r - it.row0) * a.D, dq, a.D, half);
+    mha_store_part<DP>(a.ws_o + ((int64_t)it.part * ROW_TILE + r - it.row0) * a.D, dq, a.D, half, scale == scale ? 1.f : scale);
     return;
   }
   bf16_t* dst = a.dq + row * a.D;
@@ -675,7 +729,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
     for (int g = 0; g < 4; ++g) {
       const int d = i * 32 + g * 8 + 4 * half;
       if (d < a.D) {
-        const float w[4] = {dq[i][4 * g] * a.scale, dq[i][4 * g + 1] * a.scale, dq[i][4 * g + 2] * a.scale, dq[i][4 * g + 3] * a.scale};
+        const float w[4] = {dq[i][4 * g] * scale, dq[i][4 * g + 1] * scale, dq[i][4 * g + 2] * scale, dq[i][4 * g + 3] * scale};
         *reinterpret_cast<uint2*>(dst + d) = pack4_bf16(w);
       }
     }
@@ -692,6 +746,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
   constexpr int TILE = RT * DP * 2, V_BYTES = V_LDS ? KEY_TILE * DP * 2 : 0;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE + V_BYTES];
   __shared__ __attribute__((aligned(16))) float stat[2][2][RT];   // [buffer][lse, -delta][row]
+  __shared__ int sm_bad[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
   const MhaItem it = mha_item(a, blockIdx.x);
@@ -704,6 +759,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
   auto first_row = [&](int k) { return a.causal ? max(0, k - it.shift) * a.G : 0; };
   const int mine = first_row(key);
   const int wave_first = first_row(it.row0 + wave * 32), wave_all = first_row(it.row0 + wave * 32 + 31);
+  const int all_first = first_row(min(it.row0 + KEY_TILE, it.Lk) - 1);   // first row that sees all keys of the item
   const bool some = it.row0 + wave * 32 < it.Lk;
   const int rb = it.k0, re = it.k1;
   using Stage = MhaStage<DP, RT, 4>;
@@ -757,16 +813,24 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
     next = stat_load(rb);
     stage(rb, 0);
   }
+  float scale = a.scale;         // NaN: the key was seen by a row that is not finite
   mha_settle(kf);
   if constexpr (!V_LDS) mha_settle(vf);
   int buf = 0;
   for (int r0 = rb; r0 < re; r0 += RT, buf ^= 1) {
+    if (threadIdx.x == 0) sm_bad[buf] = -NONE_BAD;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (wave < 2 && lane < RT) stat[buf][wave][lane] = wave == 0 ? mha_lse2(next) : -next;
     __syncthreads();
     if (r0 + RT < re) {
       next = stat_load(r0 + RT);
       stage(r0 + RT, buf ^ 1);
+    }
+    if (r0 < all_first) {                          // the diagonal
+      mha_clean<DP, RT, 256, true>(smem + buf * 2 * TILE, threadIdx.x, &sm_bad[buf]);
+      mha_clean<DP, RT, 256, true>(smem + buf * 2 * TILE + TILE, threadIdx.x, &sm_bad[buf]);
+      __syncthreads();
+      if (r0 + sm_bad[buf] >= mine) scale = __builtin_nanf("");
     }
     if (!some) continue;
     mha_lds_ptr qs = sm + buf * 2 * TILE, ds = qs + TILE;
@@ -821,10 +885,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
     }
   }
   if (!ok) return;
+  const float one = scale == scale ? 1.f : scale;
   if (it.part >= 0) {
     float* dst = a.ws_o + ((int64_t)it.part * KEY_TILE + key - it.row0) * (a.D + a.Dv);
-    mha_store_part<DP>(dst, dk, a.D, half);
-    mha_store_part<DP>(dst + a.D, dv, a.Dv, half);
+    mha_store_part<DP>(dst, dk, a.D, half, one);
+    mha_store_part<DP>(dst + a.D, dv, a.Dv, half, one);
     return;
   }
   bf16_t* dkp = a.dk + ((int64_t)(it.k_start + key) * a.kv_heads + it.hk) * a.D;
@@ -834,8 +899,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = i * 32 + g * 8 + 4 * half;
-      const float w[4] = {dk[i][4 * g] * a.scale, dk[i][4 * g + 1] * a.scale, dk[i][4 * g + 2] * a.scale, dk[i][4 * g + 3] * a.scale};
-      const float u[4] = {dv[i][4 * g], dv[i][4 * g + 1], dv[i][4 * g + 2], dv[i][4 * g + 3]};
+      const float w[4] = {dk[i][4 * g] * scale, dk[i][4 * g + 1] * scale, dk[i][4 * g + 2] * scale, dk[i][4 * g + 3] * scale};
+      const float u[4] = {dv[i][4 * g] * one, dv[i][4 * g + 1] * one, dv[i][4 * g + 2] * one, dv[i][4 * g + 3] * one};
       if (d < a.D) *reinterpret_cast<uint2*>(dkp + d) = pack4_bf16(w);
       if (d < a.Dv) *reinterpret_cast<uint2*>(dvp + d) = pack4_bf16(u);
     }
@@ -879,6 +944,7 @@ template <int DP>
 __global__ __launch_bounds__(64) void mha_bwd_small_kernel(MhaArgs a) {
   constexpr int TILE = 32 * DP * 2;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[3 * TILE];   // K, Q, dO
+  __shared__ int sm_bad[2];
   const int lane = threadIdx.x, half = lane >> 5, col = lane & 31;
   const MhaItem it = mha_item(a, blockIdx.x);
   using Stage = MhaStage<DP, 32, 1>;
@@ -908,13 +974,24 @@ __global__ __launch_bounds__(64) void mha_bwd_small_kernel(MhaArgs a) {
   const bool row_ok = col < it.rows, key_ok = col < it.Lk;
   bf16x8_t vf[DP / 16];
   mha_row_frags(vf, a.v + (int64_t)(it.k_start + col) * a.vt + (int64_t)it.hk * a.vh, key_ok, a.Dv, half);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if (lane < 2) sm_bad[lane] = lane ? -NONE_BAD : NONE_BAD;
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   bf16x8_t kf[DP / 16], qf[DP / 16], df[DP / 16];
 #pragma unroll
   for (int kd = 0; kd < DP / 16; ++kd) {
     kf[kd] = *(mha_frag_ptr)(ks + rd.row[kd]);
     qf[kd] = *(mha_frag_ptr)(qs + rd.row[kd]);
     df[kd] = *(mha_frag_ptr)(ds + rd.row[kd]);
+  }
+  int bad_key = NONE_BAD, bad_row = -NONE_BAD;
+  if (a.causal) {       // (the scores above keep what is not finite: they are masked one by one)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    mha_clean<DP, 32, 64, false>(smem, lane, &sm_bad[0]);
+    mha_clean<DP, 32, 64, true>(smem + TILE, lane, &sm_bad[1]);
+    mha_clean<DP, 32, 64, true>(smem + 2 * TILE, lane, &sm_bad[1]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    bad_key = *(volatile int*)&sm_bad[0];
+    bad_row = *(volatile int*)&sm_bad[1];
   }
   auto product = [&](const bf16x8_t (&x)[DP / 16], const bf16x8_t (&y)[DP / 16]) {
     f32x16_t s = mha_zero();
@@ -966,7 +1043,8 @@ __global__ __launch_bounds__(64) void mha_bwd_small_kernel(MhaArgs a) {
   };
   clear();
   mha_accumulate<DP>(acc, ks, rd, s, 0);
-  if (row_ok) store(a.dq + ((int64_t)(it.q_start + t) * a.heads + h) * a.D, a.scale, a.D);
+  if (row_ok)
+    store(a.dq + ((int64_t)(it.q_start + t) * a.heads + h) * a.D, bad_key <= last ? __builtin_nanf("") : a.scale, a.D);
   // keys in the lanes' columns: dK, dV
   f32x16_t sk = product(qf, kf);
   f32x16_t dk = product(df, vf);
@@ -982,10 +1060,11 @@ __global__ __launch_bounds__(64) void mha_bwd_small_kernel(MhaArgs a) {
   const int64_t key = (int64_t)(it.k_start + col) * a.kv_heads + it.hk;
   clear();
   mha_accumulate<DP>(acc, ds, rd, sk, 0);
-  if (key_ok) store(a.dv + key * a.Dv, 1.f, a.Dv);
+  const float one = bad_row >= mine ? __builtin_nanf("") : 1.f;
+  if (key_ok) store(a.dv + key * a.Dv, one, a.Dv);
   clear();
   mha_accumulate<DP>(acc, qs, rd, dk, 0);
-  if (key_ok) store(a.dk + key * a.D, a.scale, a.D);
+  if (key_ok) store(a.dk + key * a.D, a.scale * one, a.D);
 }
 
 // ---- the plan ------------------------------------------------------------------------------------

@@ -481,6 +481,70 @@ def test_infinite_and_missing_values_stay_in_their_rows(K, Fn):
   assert Fn.packed_attention(q, k, v, plan).isnan().all()
 
 
+MASKED_PLACES = [
+    # lengths, heads, kv_heads, D, the poisoned token of the first sequence
+    ([40], 2, 2, 64, 25), ([20], 1, 1, 128, 7), ([9, 9], 3, 1, 32, 8), ([300], 2, 1, 64, 130), ([700], 1, 1, 128, 699),
+    ([129], 4, 1, 96, 0), ([2100], 1, 1, 64, 2049), ([64, 64], 2, 2, 32, 63),
+]
+
+
+@pytest.mark.parametrize("poison", [float("nan"), float("inf")])
+@pytest.mark.parametrize("case", MASKED_PLACES, ids=[str(i) for i in range(len(MASKED_PLACES))])
+def test_values_that_are_not_finite_in_masked_places(K, Fn, case, poison):
+  """A token whose key and value (query and incoming gradient) are not finite, causal: every result that does not see it
+  is the clean one to the bit, every one that does is not finite."""
+  lens, heads, kv_heads, d, at = case
+  gen = torch.Generator().manual_seed(at)
+  n = sum(lens)
+  plan = K.AttentionPlan(lens, heads=heads, kv_heads=kv_heads, causal=True)
+  q, k, v = (normal(gen, (n, h, d)).cuda() for h in (heads, kv_heads, kv_heads))
+  dout = normal(gen, (n, heads, d)).cuda()
+
+  def run(q, k, v, dout):
+    out, saved = K.packed_attention_fwd(q, k, v, plan)
+    return (out,) + K.packed_attention_bwd(q, k, v, plan, out, saved, dout)
+  clean = run(q, k, v, dout)
+  see = torch.zeros(n, dtype=torch.bool)             # rows that see the token's key
+  see[at:lens[0]] = True
+  seen = torch.zeros(n, dtype=torch.bool)            # keys that the token's row sees
+  seen[:at + 1] = True
+  for which in ("k", "v"):
+    kk, vv = k.clone(), v.clone()
+    (kk if which == "k" else vv)[at, :, 3] = poison
+    got = run(q, kk, vv, dout)
+    for x, y in zip(got[:2], clean[:2]):             # out, dq
+      assert torch.equal(x[~see], y[~see])
+      if which == "v" or poison != poison:           # (an infinite key may give a weight of 0)
+        assert (~torch.isfinite(x[see].float())).any(-1).all()
+    for x, y in zip(got[2:], clean[2:]):             # dk, dv of keys behind: no row that sees the token sees more
+      behind = torch.zeros(n, dtype=torch.bool)
+      behind[lens[0]:] = True
+      assert torch.equal(x[behind], y[behind])
+  for which in ("q", "dout"):
+    qq, dd = q.clone(), dout.clone()
+    (qq if which == "q" else dd)[at, :, 3] = poison
+    got = run(qq, k, v, dd)
+    own = torch.zeros(n, dtype=torch.bool)
+    own[at] = True
+    assert torch.equal(got[1][~own], clean[1][~own])
+    for x, y in zip(got[2:], clean[2:]):             # dk, dv of the keys that the row does not see
+      assert torch.equal(x[~seen], y[~seen])
+      if poison != poison:
+        assert (~torch.isfinite(x[seen].float())).any(-1).all()
+
+
+def test_new_token_with_values_that_are_not_finite_behind_it(K, Fn):
+  """Chunk of 6 new tokens against a cache, the last ones not finite: the first ones see nothing of them."""
+  gen = torch.Generator().manual_seed(2)
+  q, k, v = normal(gen, (6, 4, 64)).cuda(), normal(gen, (1000, 1, 64)).cuda(), normal(gen, (1000, 1, 64)).cuda()
+  plan = K.AttentionPlan([6], [1000], heads=4, kv_heads=1, causal=True)
+  clean = Fn.packed_attention(q, k, v, plan)
+  k[998:] = float("nan")
+  v[997:] = float("inf")
+  got = Fn.packed_attention(q, k, v, plan)
+  assert torch.equal(got[:3], clean[:3]) and not torch.isfinite(got[3:].float()).any(-1).any()
+
+
 def test_same_result_every_time(K, Fn):
   """No atomics: two runs agree to the bit, alone and with another stream's call in between."""
   gen = torch.Generator().manual_seed(8)
