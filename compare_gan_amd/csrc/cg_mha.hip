@@ -1452,7 +1452,7 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   }
   if (plan->dq_joins) {
     a.items = mha_list(plan, data, 5);
-    mha_join_grad_kernel<false><<<dim3(plan->dq_joins, 4), 256, 0, st>>>(a);
+    mha_join_grad_kernel<false><<<dim3(plan->dq_joins, 16), 256, 0, st>>>(a);
     CG_CHECK_LAUNCH(name);
   }
   if (plan->dkv_tiles) {
@@ -1462,7 +1462,7 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   }
   if (plan->dkv_joins) {
     a.items = mha_list(plan, data, 7);
-    mha_join_grad_kernel<true><<<dim3(plan->dkv_joins, 4), 256, 0, st>>>(a);
+    mha_join_grad_kernel<true><<<dim3(plan->dkv_joins, 16), 256, 0, st>>>(a);
     CG_CHECK_LAUNCH(name);
   }
   if (plan->small) {

@@ -1011,15 +1011,18 @@ class RotaryFn(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, x, positions, table):
+    out = K.rotary(x, positions, table)
     ctx.save_for_backward(positions)
     ctx.table = table
-    return K.rotary(x, positions, table)
+    return out
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, dy):
     (positions,) = ctx.saved_tensors
-    return K.rotary(dy, positions, ctx.table, inverse=True), None, None
+    # (checked in the forward pass; what arrives here has x's shape, type and device)
+    dx = K._rotate(K._head_inner(dy), positions.contiguous(), ctx.table, True)   # pylint: disable=protected-access
+    return dx, None, None
 
 
 def rotary(x, positions, table):
@@ -1033,18 +1036,19 @@ class QkNormRotaryFn(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, q, k, q_gain, k_gain, positions, table, eps):
-    q_out, k_out = K.qk_norm_rotary(q, k, q_gain, k_gain, positions, table, eps)
+    positions = K._qk_args(q, k, q_gain, k_gain, positions, table, eps)   # pylint: disable=protected-access
+    q, k = K._head_inner(q), K._head_inner(k)   # pylint: disable=protected-access
     ctx.save_for_backward(q, k, q_gain, k_gain, positions)
     ctx.table, ctx.eps = table, eps
-    return q_out, k_out
+    return K._qk_rows(q, k, q_gain, k_gain, positions, table, eps)   # pylint: disable=protected-access
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, dq_out, dk_out):
     q, k, q_gain, k_gain, positions = ctx.saved_tensors
-    dq, dk, dqg, dkg = K.qk_norm_rotary_bwd(q, k, q_gain, k_gain, positions, ctx.table, dq_out.contiguous(),
-                                            dk_out.contiguous(), ctx.eps)
-    return dq, dk, dqg, dkg, None, None, None
+    grads = K._qk_grads(q, k, q_gain, k_gain, positions, ctx.table, dq_out.contiguous(),   # pylint: disable=protected-access
+                        dk_out.contiguous(), ctx.eps)
+    return grads + (None, None, None)
 
 
 def qk_norm_rotary(q, k, q_gain, k_gain, positions=None, table=None, eps=1e-6):

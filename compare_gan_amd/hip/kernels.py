@@ -1167,6 +1167,7 @@ class RotaryTable(object):
             self.amplitude = 0.1 * math.log(factor) + 1.0
         self.rotary_dim, self.axes, self.layout = rotary_dim, axes, layout
         self.freq = torch.tensor(turns * axes, dtype=F64, device=device)
+        self.index = self.freq.get_device()
         self._tail = (self.freq.data_ptr(), self.amplitude, axes, rotary_dim, 1 if layout == "interleaved" else 0)
         _ready_on_every_stream(self.freq)
 
@@ -1188,7 +1189,7 @@ def _req_heads(t, name, like=None):
     if t.dim() != 3:
         raise ValueError("%s must be [rows, heads, width], got %d dimensions" % (name, t.dim()))
     if like is not None:
-        if t.device != like.device:
+        if t.get_device() != like.get_device():
             raise ValueError("%s is on %s, the other tensors on %s" % (name, t.device, like.device))
         if t.dtype != like.dtype:
             raise ValueError("%s must be %s, got %s" % (name, like.dtype, t.dtype))
@@ -1223,21 +1224,24 @@ def _rotary_args(x, positions, table):
         raise ValueError("table must be a RotaryTable")
     if not torch.is_tensor(positions) or not positions.is_cuda or positions.dtype != torch.int32:
         raise ValueError("positions must be an int32 tensor on the GPU")
-    want = (x.shape[0],) if table.axes == 1 else (x.shape[0], table.axes)
-    if positions.shape != want and positions.shape != (x.shape[0], table.axes):
+    rows, _, width = x.shape
+    shape = positions.shape
+    if shape != (rows, table.axes) and (table.axes > 1 or shape != (rows,)):
         raise ValueError("positions must be %s for %d axes, got %s" % (
-            list(want), table.axes, list(positions.shape)))
-    if positions.device != x.device or table.freq.device != x.device:
+            [rows] if table.axes == 1 else [rows, table.axes], table.axes, list(shape)))
+    index = x.get_device()
+    if positions.get_device() != index or table.index != index:
         raise ValueError("positions, table and tensors must be on one device")
-    if table.rotary_dim > x.shape[2]:
-        raise ValueError("rotary_dim %d exceeds the head width %d" % (table.rotary_dim, x.shape[2]))
+    if table.rotary_dim > width:
+        raise ValueError("rotary_dim %d exceeds the head width %d" % (table.rotary_dim, width))
     return positions.contiguous()
 
 
 def _req_width(x, name):
     if x.dtype not in HEAD_TYPES:
         raise ValueError("%s must be bfloat16 or float32, got %s" % (name, x.dtype))
-    if x.shape[1] < 1 or x.shape[2] < 2 or x.shape[2] % 2 or x.shape[2] > 256:
+    _, heads, width = x.shape
+    if heads < 1 or width < 2 or width % 2 or width > 256:
         raise ValueError("%s: heads of even width up to 256 expected, got %s" % (name, list(x.shape)))
 
 
@@ -1247,7 +1251,11 @@ def rotary(x, positions, table, inverse=False):
     _req_heads(x, "x")
     _req_width(x, "x")
     positions = _rotary_args(x, positions, table)
-    x = _head_inner(x)
+    return _rotate(_head_inner(x), positions, table, inverse)
+
+
+def _rotate(x, positions, table, inverse):
+    """rotary on arguments that are known to fit (Fn.rotary's backward)."""
     rows, _, width = x.shape
     y = _dense_like(x)
     with _On(x) as stream:
@@ -1261,13 +1269,14 @@ def _qk_args(q, k, q_gain, k_gain, positions, table, eps):
     _req_width(q, "q")
     _req_heads(k, "k", q)
     _req_width(k, "k")
-    if k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+    rows, _, width = q.shape
+    if k.shape[0] != rows or k.shape[2] != width:
         raise ValueError("q %s and k %s must agree in rows and width" % (list(q.shape), list(k.shape)))
     for g, nm in ((q_gain, "q_gain"), (k_gain, "k_gain")):
         if g is not None:
             _req(g, F32, nm)
-            if tuple(g.shape) != (q.shape[2],) or g.device != q.device:
-                raise ValueError("%s must be [%d] on %s" % (nm, q.shape[2], q.device))
+            if g.shape != (width,) or g.get_device() != q.get_device():
+                raise ValueError("%s must be [%d] on %s" % (nm, width, q.device))
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError("eps must be finite and not negative, got %r" % (eps,))
     if (positions is None) != (table is None):
@@ -1279,7 +1288,11 @@ def qk_norm_rotary(q, k, q_gain, k_gain, positions, table, eps=1e-6):
     """RMS norm of every head of q [T, heads, D] and k [T, kv_heads, D] over its D entries, times the gains
     (fp32 [D] or None), then the rotation (positions = table = None: none), in one launch."""
     positions = _qk_args(q, k, q_gain, k_gain, positions, table, eps)
-    q, k = _head_inner(q), _head_inner(k)
+    return _qk_rows(_head_inner(q), _head_inner(k), q_gain, k_gain, positions, table, eps)
+
+
+def _qk_rows(q, k, q_gain, k_gain, positions, table, eps):
+    """qk_norm_rotary on arguments that are known to fit."""
     rows, _, width = q.shape
     q_out, k_out = _dense_like(q), _dense_like(k)
     rot = None if table is None else table.packed(positions)
@@ -1298,7 +1311,11 @@ def qk_norm_rotary_bwd(q, k, q_gain, k_gain, positions, table, dq_out, dk_out, e
     _req(dk_out, q.dtype, "dk_out")
     if dq_out.shape != q.shape or dk_out.shape != k.shape or dq_out.device != q.device or dk_out.device != q.device:
         raise ValueError("dq_out and dk_out must have the shapes and the device of q and k")
-    q, k = _head_inner(q), _head_inner(k)
+    return _qk_grads(_head_inner(q), _head_inner(k), q_gain, k_gain, positions, table, dq_out, dk_out, eps)
+
+
+def _qk_grads(q, k, q_gain, k_gain, positions, table, dq_out, dk_out, eps):
+    """qk_norm_rotary_bwd on arguments that are known to fit (Fn.qk_norm_rotary's backward)."""
     rows, _, width = q.shape
     dq, dk = _dense_like(q), _dense_like(k)
     dqg = None if q_gain is None else torch.empty_like(q_gain)
@@ -1351,6 +1368,7 @@ class AttentionPlan(object):
         self.k_dense = int(k_lengths.sum(dtype=np.int64)) == self.k_rows
         self.device = torch.device(device)
         self.data = torch.from_numpy(self.host).to(self.device)
+        self.index = self.data.get_device()
         _ready_on_every_stream(self.data)
 
 
@@ -1391,20 +1409,20 @@ def _attention_input(q, k, v, plan, scale):
         raise ValueError("q must be %s, got %s" % (BF16, q.dtype))
     _req_heads(k, "k", q)
     _req_heads(v, "v", q)
-    if plan.data.device != q.device:
+    if plan.index != q.get_device():
         raise ValueError("the plan is on %s, the tensors on %s" % (plan.data.device, q.device))
-    if q.shape[1] != plan.heads or k.shape[1] != plan.kv_heads or v.shape[1] != plan.kv_heads:
+    (q_rows, heads, d), (k_rows, kv_heads, dk), (v_rows, v_heads, dv) = q.shape, k.shape, v.shape
+    if heads != plan.heads or kv_heads != plan.kv_heads or v_heads != plan.kv_heads:
         raise ValueError("the plan is for %d heads over %d, got q %s, k %s, v %s" % (
             plan.heads, plan.kv_heads, list(q.shape), list(k.shape), list(v.shape)))
-    if k.shape[2] != q.shape[2] or v.shape[0] != k.shape[0]:
+    if dk != d or v_rows != k_rows:
         raise ValueError("q %s, k %s and v %s do not fit together" % (list(q.shape), list(k.shape), list(v.shape)))
-    for w in (q.shape[2], v.shape[2]):
-        if w < 8 or w > 128 or w % 8:
-            raise ValueError("head widths must be multiples of 8 up to 128, got %d" % w)
-    if q.shape[0] < plan.q_rows or k.shape[0] < plan.k_rows:
+    if not (8 <= d <= 128 and 8 <= dv <= 128) or d % 8 or dv % 8:
+        raise ValueError("head widths must be multiples of 8 up to 128, got %d and %d" % (d, dv))
+    if q_rows < plan.q_rows or k_rows < plan.k_rows:
         raise ValueError("the plan's sequences end at query row %d and key row %d, got q %s and k %s" % (
             plan.q_rows, plan.k_rows, list(q.shape), list(k.shape)))
-    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError("scale must be positive and finite, got %r" % (scale,))
     return scale

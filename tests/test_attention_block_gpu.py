@@ -68,9 +68,12 @@ def test_block_against_the_chain(dev, n, h, w, c, heads, kv_heads, width):
   o = torch.einsum("nhqk,nkhd->nqhd", p, v).reshape(n, h * w, heads * width)
   want = x64 + (v64["sigma"] * (o @ v64["conv2d_o/kernel"][0, 0])).reshape(n, h, w, c)
   wgrads = torch.autograd.grad(want, [x64] + [v64[k.split("att/")[1]] for k in names], dout.double().cpu())
+  # sigma's gradient is one sum of n h w c terms of either sign, each off by its own relative roundings: its error is to
+  # be held against the norm of the terms, not against what their signs leave of the sum
+  terms = float((dout.double().cpu() * (o @ v64["conv2d_o/kernel"][0, 0]).reshape(n, h, w, c)).norm().detach())
   for name, a, b in zip(["out", "dx"] + names, (out,) + grads, (want,) + wgrads):
     a, b = a.detach().double().cpu(), b.detach()
-    assert float((a - b).norm() / b.norm()) <= 7 * HB, name
+    assert float((a - b).norm()) <= 7 * HB * (terms if name == "att/sigma" else float(b.norm())), name
 
 
 @pytest.mark.parametrize("arch", ["resnet_biggan", "resnet_biggan_deep"])
