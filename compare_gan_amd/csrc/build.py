@@ -16,9 +16,13 @@ SOURCES = ["cg_error.hip", "cg_gconv.hip", "cg_conv_fast.hip", "cg_conv_halo.hip
            "cg_rope.hip", "cg_mha.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
-         # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results
-         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-I" + os.path.join(ROOT, "include"), "-I" + HERE]
+
+# No packed fp32 arithmetic (v_pk_add / mul / fma_f32: some of its forms have given wrong results now and then) in the
+# sources below.  The others are built as they always were: without it their sums round differently in the last bit, and
+# the networks' results with them.
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+SOURCE_FLAGS = {"cg_rope.hip": NO_PACKED_FP32, "cg_mha.hip": NO_PACKED_FP32}
 
 
 def _newer(src, dst):
@@ -31,7 +35,7 @@ def _compile(src):
     deps = [srcp, os.path.join(HERE, "cg_common.h"), os.path.join(HERE, "cg_conv_fast.h"),
             os.path.join(ROOT, "include", "cgamd.h")]
     if any(_newer(d, obj) for d in deps):
-        cmd = [HIPCC] + FLAGS + ["-c", srcp, "-o", obj]
+        cmd = [HIPCC] + FLAGS + SOURCE_FLAGS.get(src, []) + ["-c", srcp, "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("hipcc failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))
@@ -61,7 +65,7 @@ def build_timing():
     objs = []
     for src in SOURCES:
         obj = os.path.join(odir, os.path.splitext(src)[0] + ".o")
-        cmd = [HIPCC] + FLAGS + ["-DCG_CONV_TIMING", "-c", os.path.join(HERE, src), "-o", obj]
+        cmd = [HIPCC] + FLAGS + SOURCE_FLAGS.get(src, []) + ["-DCG_CONV_TIMING", "-c", os.path.join(HERE, src), "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("hipcc failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))

@@ -1253,7 +1253,7 @@ int mha_check(const char* name, const cgAttentionInput* in, const cgAttentionPla
     CG_FAIL(CG_ERR_BAD_ARG, "%s: not a plan of cg_host_attention_plan", name);
   if (in->D < 8 || in->D > 128 || in->D % 8 || in->Dv < 8 || in->Dv > 128 || in->Dv % 8)
     CG_FAIL(CG_ERR_UNSUPPORTED, "%s: head widths %d and %d (multiples of 8, at most 128)", name, in->D, in->Dv);
-  if (!(in->scale > 0.f) || in->scale > 3.0e38f) CG_FAIL(CG_ERR_BAD_ARG, "%s: scale has to be positive and finite", name);
+  if (!(in->scale >= 0.99e-30f && in->scale <= 1.01e30f)) CG_FAIL(CG_ERR_BAD_ARG, "%s: scale has to be in [1e-30, 1e30]", name);
   if (in->q_rows < p->max_q_row || in->k_rows < p->max_k_row)
     CG_FAIL(CG_ERR_BAD_ARG, "%s: %d query and %d key rows, the plan's sequences need %d and %d", name, in->q_rows,
             in->k_rows, p->max_q_row, p->max_k_row);

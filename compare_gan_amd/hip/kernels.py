@@ -1374,12 +1374,14 @@ class AttentionPlan(object):
 
 def _sequences(starts, lengths, name):
     """(starts, lengths) as int32 arrays; refuses negative and overlapping sequences."""
-    lengths = np.asarray(lengths, dtype=np.int64).reshape(-1)
+    lengths = np.asarray(lengths).reshape(-1)
     if lengths.size < 1:
         raise ValueError("%s_lengths must name at least one sequence" % name)
-    if starts is None:
-        starts = np.concatenate(([0], np.cumsum(lengths)[:-1]))
-    starts = np.asarray(starts, dtype=np.int64).reshape(-1)
+    starts = None if starts is None else np.asarray(starts).reshape(-1)
+    if lengths.dtype.kind not in "iu" or (starts is not None and starts.dtype.kind not in "iu"):
+        raise ValueError("%s: starts and lengths must be whole numbers" % name)
+    lengths = lengths.astype(np.int64)
+    starts = np.cumsum(lengths) - lengths if starts is None else starts.astype(np.int64)
     if starts.size != lengths.size:
         raise ValueError("%s_starts names %d sequences, %s_lengths %d" % (name, starts.size, name, lengths.size))
     if (lengths < 0).any() or (starts < 0).any() or (starts + lengths >= 2 ** 30).any():
@@ -1423,8 +1425,8 @@ def _attention_input(q, k, v, plan, scale):
         raise ValueError("the plan's sequences end at query row %d and key row %d, got q %s and k %s" % (
             plan.q_rows, plan.k_rows, list(q.shape), list(k.shape)))
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError("scale must be positive and finite, got %r" % (scale,))
+    if not 1e-30 <= scale <= 1e30:      # (NaN: not in it either; in fp32 and times log2(e) it stays finite)
+        raise ValueError("scale must be in [1e-30, 1e30], got %r" % (scale,))
     return scale
 
 

@@ -609,7 +609,7 @@ int cg_host_attention_plan(const int32_t* q_start, const int32_t* q_len, const i
                            const int32_t* k_len, int sequences, int heads, int kv_heads, int causal,
                            int32_t* data_host, int64_t capacity, cgAttentionPlan* info);
 /* q [q_rows, heads, D], k [k_rows, kv_heads, D], v [k_rows, kv_heads, Dv] bf16, strides in elements, heads
- * contiguous inside; D and Dv multiples of 8, at most 128; scale > 0.  out [q_rows, heads, Dv] contiguous,
+ * contiguous inside; D and Dv multiples of 8, at most 128; scale in [1e-30, 1e30].  out [q_rows, heads, Dv] contiguous,
  * lse [q_rows, heads] fp32 and out_low like out (what its rounding left over): for the backward pass, NULL where
  * none follows (out_low also where plan->dq_tiles is 0).  Rows that see no key: out 0, lse -inf.  Rows that belong to
  * no sequence are left as they were. */

@@ -173,7 +173,7 @@ def test_plan_spreads_few_rows_over_the_chip():
     dict(q_lengths=[4], heads=3, kv_heads=2), dict(q_lengths=[4], heads=0),
     dict(q_lengths=[4, 4], q_starts=[0, 2]), dict(q_lengths=[4, 4], q_starts=[0]),
     dict(q_lengths=[4, 4], k_starts=[3, 0]), dict(q_lengths=[4], k_starts=[-1]),
-    dict(q_lengths=[2 ** 30]), dict(q_lengths=[2 ** 40]), dict(q_lengths=[4], heads=8192)])
+    dict(q_lengths=[2.5]), dict(q_lengths=[4], k_starts=[0.5]), dict(q_lengths=[2 ** 30]), dict(q_lengths=[2 ** 40]), dict(q_lengths=[4], heads=8192)])
 def test_plan_refusals(kw):
   with pytest.raises((ValueError, _lib.CgamdError)):
     K.AttentionPlan(device="cpu", **kw)

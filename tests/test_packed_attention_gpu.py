@@ -596,7 +596,7 @@ def test_attention_refusals(K, Fn):
   for bad in (dict(q=z(4, 2, 16, dtype=torch.float32)), dict(k=z(4, 1, 16, dtype=torch.half)), dict(q=z(4, 1, 16)),
               dict(k=z(4, 2, 16)), dict(k=z(4, 1, 24)), dict(v=z(5, 1, 24)), dict(q=z(3, 2, 16)),
               dict(k=z(3, 1, 16), v=z(3, 1, 16)), dict(q=z(4, 2, 12), k=z(4, 1, 12)), dict(v=z(4, 1, 136)),
-              dict(q=z(4, 32)), dict(plan=None), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+              dict(q=z(4, 32)), dict(plan=None), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=1e300), dict(scale=1e-60),
               dict(plan=K.AttentionPlan([4], heads=2, kv_heads=1, device="cpu")), dict(v=z(4, 1, 24).cpu())):
     with pytest.raises(ValueError):
       Fn.packed_attention(**dict(good, **bad))
