@@ -52,9 +52,10 @@ struct MhaArgs {
   float* lse;
   float* ws_o;              // partial results, in units of 32 rows: [unit][32][Dv]
   float* ws_ml;             //                                        [unit][32][2]
+  const bf16_t *o_in, *o_low;
   const bf16_t* dout;
   const float* lse_in;
-  const float* delta;
+  float* delta;
   bf16_t *dq, *dk, *dv;
   int heads, G, kv_heads, D, Dv, causal;
   float c, scale;           // scale * log2(e)
@@ -616,31 +617,13 @@ __global__ __launch_bounds__(256) void mha_join_kernel(MhaArgs a) {
 }
 
 // ---- backward -----------------------------------------------------------------------------------
-// delta[row] = sum_d dout (out + out_low); 16 lanes a row, 8 elements each.  dS = P (dP - delta) is a difference: with
-// the rounded out alone its error would come on top of the rounding of dS (dQ 1.5 instead of 1.4 roundings off).
-__global__ __launch_bounds__(256) void mha_delta_kernel(const bf16_t* __restrict__ out, const bf16_t* __restrict__ low,
-                                                        const bf16_t* __restrict__ dout, int64_t rows, int Dv,
-                                                        float* __restrict__ delta) {
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int d = (threadIdx.x & 15) * 8;
-  float s = 0.f;
-  if (row < rows && d < Dv) {
-    float x[8], y[8], z[8];
-    unpack8_bf16(*reinterpret_cast<const uint4*>(out + row * Dv + d), x);
-    unpack8_bf16(*reinterpret_cast<const uint4*>(low + row * Dv + d), z);
-    unpack8_bf16(*reinterpret_cast<const uint4*>(dout + row * Dv + d), y);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s += (x[j] + z[j]) * y[j];
-  }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if (row < rows && (threadIdx.x & 15) == 0) delta[row] = s;
-}
-
 // what the weights are rebuilt from, in exponents of two; a row that saw no key: +inf (weights 0)
 __device__ __forceinline__ float mha_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * LOG2E; }
 
-// dQ: 128 rows x all keys; S^T and dP^T = V dO^T side by side, dQ^T += K^T dS^T
+// dQ: 128 rows x all keys; S^T and dP^T = V dO^T side by side, dQ^T += K^T dS^T.  delta = dO . (out + out_low) of its
+// rows is formed on the way in (dO is in registers for dP) and left for the dK / dV kernel behind it.  dS = P (dP - delta)
+// is a difference: with the rounded out alone its error would come on top of the rounding of dS (dQ 1.5 instead of 1.4
+// roundings off).
 template <int DP>
 __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArgs a) {
   constexpr int TILE = KT * DP * 2;
@@ -659,7 +642,21 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
   mha_row_frags(qf, a.q + (int64_t)(it.q_start + t) * a.qt + (int64_t)h * a.qh, ok, a.D, half);
   mha_row_frags(df, a.dout + row * a.Dv, ok, a.Dv, half);
   const float lse2 = ok ? mha_lse2(a.lse_in[row]) : INFINITY;
-  const float delta = ok ? a.delta[row] : 0.f;
+  float delta = 0.f;
+#pragma unroll
+  for (int kd = 0; kd < DP / 16; ++kd) {
+    const int d = kd * 16 + half * 8;
+    if (ok && d < a.Dv) {
+      float x[8], y[8], z[8];
+      unpack8_bf16(*reinterpret_cast<const uint4*>(a.o_in + row * a.Dv + d), x);
+      unpack8_bf16(*reinterpret_cast<const uint4*>(a.o_low + row * a.Dv + d), y);
+      unpack8_bf16(__builtin_bit_cast(uint4, df[kd]), z);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta += (x[j] + y[j]) * z[j];
+    }
+  }
+  delta += __shfl_xor(delta, 32, 64);
+  if (ok && half == 0) a.delta[row] = delta;     // (parts of a split item write the same value)
   const int last = ok ? min(it.k1 - 1, t + it.shift) : -1;
   int least = last, most = last;
 #pragma unroll
@@ -1436,16 +1433,13 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   a.dq = (bf16_t*)dq;
   a.dk = (bf16_t*)dk;
   a.dv = (bf16_t*)dv;
-  a.delta = (const float*)ws;
+  a.o_in = (const bf16_t*)out;
+  a.o_low = (const bf16_t*)out_low;
+  a.delta = (float*)ws;
   if (ws) a.ws_o = (float*)((char*)ws + mha_delta_bytes(plan, in->q_rows));
   const hipStream_t st = (hipStream_t)stream;
   const int dp = mha_width(in->D, in->Dv);
   if (plan->dq_tiles) {
-    const int64_t rows = (int64_t)in->q_rows * plan->heads;
-    if (rows > (int64_t)0x7fffffff * 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: too many rows", name);
-    mha_delta_kernel<<<(uint32_t)((rows + 15) / 16), 256, 0, st>>>((const bf16_t*)out, (const bf16_t*)out_low, a.dout, rows, a.Dv,
-                                                                    (float*)ws);
-    CG_CHECK_LAUNCH(name);
     a.items = mha_list(plan, data, 4);
     MHA_LAUNCH(dp, MHA_BWD_Q, plan->dq_tiles, 256, st, a);
     CG_CHECK_LAUNCH(name);

@@ -386,9 +386,11 @@ int rope_plan(RopeArgs* a, const cgRotation* rot, int T, int D, int esize, bool 
   }
   int heads = 0;
   for (int s = 0; s < a->ntensors; ++s) heads += a->t[s].heads;
-  // tokens a block: about 16 K elements, so that the angles and the launch of a block are spread over
-  // enough data, but not so many that fewer than 1024 blocks are left for 256 CUs
-  int tb = 16384 / (heads * D);
+  // Tokens a block, so that its angles and its launch are spread over enough data, but not so many that fewer than 1024
+  // blocks are left for 256 CUs.  A rotation alone: about 6 K elements (262 144 tokens x 3 heads of 64: 32 us, with 16 K
+  // 34 us; 65 536 x 16 heads of 128: 94 us, 98 us); with the norm, whose gains are read once a block: 32 K (65 536 x 40
+  // heads of 128: 277 us, with 16 K 306 us).
+  int tb = (a->ntensors == 2 ? 32768 : 6144) / (heads * D);
   const int room = a->slots > 0 ? ROPE_LDS_FLOATS / 2 / a->slots : tb;
   if (tb > room) tb = room;
   if (tb > cdiv(T, 1024)) tb = cdiv(T, 1024);

@@ -1096,24 +1096,17 @@ _ROTATION = struct.Struct("@PPfiii0q")
 _ATTENTION_INPUT = struct.Struct("@PPPqqqqqqiiiif0q")
 
 
-class _On(object):
-    """Launches on `t`'s device and its current stream (`stream`), whichever device is current."""
-
-    __slots__ = ("stream", "_ctx")
-
-    def __init__(self, t):
-        index = t.get_device()
-        self._ctx = None if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
-        self.stream = torch._C._cuda_getCurrentRawStream(index)
-
-    def __enter__(self):
-        if self._ctx is not None:
-            self._ctx.__enter__()
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
+def _launch(entry, t, *args):
+    """Calls an entry point with `t`'s device current, whichever one is, and that device's current stream."""
+    index = t.get_device()
+    fn = getattr(lib(), entry)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, entry)
 
 
 class RotaryTable(object):
@@ -1258,9 +1251,8 @@ def _rotate(x, positions, table, inverse):
     """rotary on arguments that are known to fit (Fn.rotary's backward)."""
     rows, _, width = x.shape
     y = _dense_like(x)
-    with _On(x) as stream:
-        check(lib().cg_rotary(_head_rows(x), rows, width, HEAD_TYPES[x.dtype], table.packed(positions),
-                              1 if inverse else 0, y.data_ptr(), stream), "cg_rotary")
+    _launch("cg_rotary", x, _head_rows(x), rows, width, HEAD_TYPES[x.dtype], table.packed(positions),
+            1 if inverse else 0, y.data_ptr())
     return y
 
 
@@ -1296,10 +1288,8 @@ def _qk_rows(q, k, q_gain, k_gain, positions, table, eps):
     rows, _, width = q.shape
     q_out, k_out = _dense_like(q), _dense_like(k)
     rot = None if table is None else table.packed(positions)
-    with _On(q) as stream:
-        check(lib().cg_qk_norm_rotary_fwd(
-            _head_rows(q, q_gain), _head_rows(k, k_gain), rows, width, HEAD_TYPES[q.dtype], eps, rot,
-            q_out.data_ptr(), k_out.data_ptr(), stream), "cg_qk_norm_rotary_fwd")
+    _launch("cg_qk_norm_rotary_fwd", q, _head_rows(q, q_gain), _head_rows(k, k_gain), rows, width,
+            HEAD_TYPES[q.dtype], eps, rot, q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
@@ -1322,11 +1312,9 @@ def _qk_grads(q, k, q_gain, k_gain, positions, table, dq_out, dk_out, eps):
     dkg = None if k_gain is None else torch.empty_like(k_gain)
     ws = _ws(lib().cg_qk_norm_rotary_bwd_workspace_bytes(rows, width), q)
     rot = None if table is None else table.packed(positions)
-    with _On(q) as stream:
-        check(lib().cg_qk_norm_rotary_bwd(
-            _head_rows(q, q_gain), _head_rows(k, k_gain), dq_out.data_ptr(), dk_out.data_ptr(), rows, width,
-            HEAD_TYPES[q.dtype], eps, rot, dq.data_ptr(), dk.data_ptr(), _p(dqg), _p(dkg), ws.data_ptr(),
-            ws.numel(), stream), "cg_qk_norm_rotary_bwd")
+    _launch("cg_qk_norm_rotary_bwd", q, _head_rows(q, q_gain), _head_rows(k, k_gain), dq_out.data_ptr(),
+            dk_out.data_ptr(), rows, width, HEAD_TYPES[q.dtype], eps, rot, dq.data_ptr(), dk.data_ptr(), _p(dqg),
+            _p(dkg), ws.data_ptr(), ws.numel())
     return dq, dk, dqg, dkg
 
 
@@ -1436,11 +1424,9 @@ def _attention_packed(q, k, v, scale):
                                  *_row_strides(v), q.shape[0], k.shape[0], q.shape[2], v.shape[2], scale)
 
 
-def _rows_out(shape, dense, used, device, dtype=BF16):
-    """An output whose rows outside every sequence are zero."""
-    if dense and used == shape[0]:
-        return torch.empty(shape, dtype=dtype, device=device)
-    return torch.zeros(shape, dtype=dtype, device=device)
+def _rows_out(shape, dense, used, like):
+    """A dense bf16 output on `like`'s device whose rows outside every sequence are zero."""
+    return like.new_empty(shape) if dense and used == shape[0] else like.new_zeros(shape)
 
 
 def packed_attention_fwd(q, k, v, plan, scale=None, want_grad=True, out=None):
@@ -1458,7 +1444,7 @@ def _attention_rows(q, k, v, plan, scale, want_grad, out=None):
     """packed_attention_fwd on operands that are known to fit."""
     shape = (q.shape[0], q.shape[1], v.shape[2])
     if out is None:
-        out = _rows_out(shape, plan.q_dense, plan.q_rows, q.device)
+        out = _rows_out(shape, plan.q_dense, plan.q_rows, q)
     else:
         _req(out, BF16, "out")
         if tuple(out.shape) != shape or out.device != q.device or out.data_ptr() % 16:
@@ -1467,15 +1453,13 @@ def _attention_rows(q, k, v, plan, scale, want_grad, out=None):
     if want_grad:
         lse = torch.empty(shape[:2], dtype=F32, device=q.device)
         if plan.info.dq_tiles:
-            low = torch.empty(shape, dtype=BF16, device=q.device)
+            low = q.new_empty(shape)
     nbytes, ws = 0, None
     if plan.info.parts:
         nbytes = lib().cg_packed_attention_fwd_workspace_bytes(plan.ref, shape[2])
         ws = _ws(nbytes, q)
-    with _On(q) as stream:
-        check(lib().cg_packed_attention_fwd(_attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(),
-                                            out.data_ptr(), _p(low), _p(lse), _p(ws), nbytes, stream),
-              "cg_packed_attention_fwd")
+    _launch("cg_packed_attention_fwd", q, _attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(),
+            out.data_ptr(), _p(low), _p(lse), _p(ws), nbytes)
     return out, (lse, low) if want_grad else None
 
 
@@ -1500,18 +1484,16 @@ def packed_attention_bwd(q, k, v, plan, out, saved, dout, scale=None):
 
 def _attention_grads(q, k, v, plan, out, lse, low, dout, scale):
     """packed_attention_bwd on operands that are known to fit (Fn.packed_attention's backward)."""
-    dq = _rows_out(q.shape, plan.q_dense, plan.q_rows, q.device)
-    dk = _rows_out(k.shape, plan.k_dense, plan.k_rows, q.device)
-    dv = _rows_out(v.shape, plan.k_dense, plan.k_rows, q.device)
+    dq = _rows_out(q.shape, plan.q_dense, plan.q_rows, q)
+    dk = _rows_out(k.shape, plan.k_dense, plan.k_rows, q)
+    dv = _rows_out(v.shape, plan.k_dense, plan.k_rows, q)
     ws, nbytes = None, 0
     if plan.info.dq_tiles or plan.info.dkv_tiles:
         nbytes = lib().cg_packed_attention_bwd_workspace_bytes(plan.ref, q.shape[0], q.shape[2], v.shape[2])
         ws = _ws(nbytes, q)
-    with _On(q) as stream:
-        check(lib().cg_packed_attention_bwd(
-            _attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(), out.data_ptr(), _p(low), lse.data_ptr(),
-            dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(ws), nbytes, stream),
-            "cg_packed_attention_bwd")
+    _launch("cg_packed_attention_bwd", q, _attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(),
+            out.data_ptr(), _p(low), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            _p(ws), nbytes)
     return dq, dk, dv
 
 
