@@ -42,6 +42,8 @@ constexpr int ROW_TILE = 128;    // rows of a forward / dQ work item: 4 waves of
 constexpr int KEY_TILE = 128;    // keys of a dK / dV work item: 4 waves of 32
 constexpr int THIN_ROWS = 32;    // rows of a thin work item: one wave's
 
+constexpr int mha_wider(int DK, int DV) { return DK > DV ? DK : DV; }
+
 struct MhaArgs {
   const bf16_t *q, *k, *v;
   int64_t qt, qh, kt, kh, vt, vh;
@@ -331,13 +333,13 @@ __device__ __forceinline__ void mha_store_part(float* dst, const f32x16_t (&o)[D
 }
 
 // what a wave leaves behind: O^T in registers -> out, or a partial result
-template <int DP, bool GRAD>
+template <int DV, bool GRAD>
 __device__ __forceinline__ void mha_store(const MhaArgs& a, const MhaItem& it, int r, float m, float l,
-                                          f32x16_t (&o)[DP / 32], int half) {
+                                          f32x16_t (&o)[DV / 32], int half) {
   if (r >= it.rows) return;
   if (it.part >= 0) {
     const int64_t at = (int64_t)it.part * THIN_ROWS + (r - it.row0);
-    mha_store_part<DP>(a.ws_o + at * a.Dv, o, a.Dv, half);
+    mha_store_part<DV>(a.ws_o + at * a.Dv, o, a.Dv, half);
     if (half == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m, l);
     return;
   }
@@ -347,7 +349,7 @@ __device__ __forceinline__ void mha_store(const MhaArgs& a, const MhaItem& it, i
   const float inv = l == 0.f ? 0.f : 1.f / l;       // a row that sees no key: 0
   bf16_t* dst = a.out + row * a.Dv;
 #pragma unroll
-  for (int t = 0; t < DP / 32; ++t)
+  for (int t = 0; t < DV / 32; ++t)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = t * 32 + g * 8 + 4 * half;
@@ -368,10 +370,10 @@ __device__ __forceinline__ void mha_store(const MhaArgs& a, const MhaItem& it, i
 }
 
 // ---- forward, 128 rows x all keys of the item ---------------------------------------------------
-template <int DP, bool GRAD>
-__global__ __launch_bounds__(256, DP <= 64 ? 4 : DP <= 96 ? 3 : 2) void mha_fwd_kernel(MhaArgs a) {
-  constexpr int TILE = KT * DP * 2;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
+template <int DK, int DV, bool GRAD>
+__global__ __launch_bounds__(256, mha_wider(DK, DV) <= 64 ? 4 : mha_wider(DK, DV) <= 96 ? 3 : 2) void mha_fwd_kernel(MhaArgs a) {
+  constexpr int TK = KT * DK * 2, TILES = TK + KT * DV * 2;      // K, and K with V
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * TILES];
   __shared__ int sm_bad[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
@@ -381,7 +383,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : DP <= 96 ? 3 : 2) void mha_fwd_
   int t, h;
   mha_token(a, it, r, &t, &h);
   const bool ok = r < it.rows;
-  bf16x8_t qf[DP / 16];
+  bf16x8_t qf[DK / 16];
   mha_row_frags(qf, a.q + (int64_t)(it.q_start + t) * a.qt + (int64_t)h * a.qh, ok, a.D, half);
   // last key this row sees (exclusive end of the item's keys included)
   const int last = ok ? min(it.k1 - 1, t + it.shift) : -1;
@@ -393,22 +395,22 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : DP <= 96 ? 3 : 2) void mha_fwd_
   }
   least = __builtin_amdgcn_readfirstlane(least);
   most = __builtin_amdgcn_readfirstlane(most);
-  using Stage = MhaStage<DP, KT, 4>;
-  uint32_t koff[Stage::N], voff[Stage::N];
-  mha_offsets<DP, KT, 4>(koff, wave, lane, a.kt, a.D);
-  mha_offsets<DP, KT, 4>(voff, wave, lane, a.vt, a.Dv);
-  const MhaReads<DP> rd = mha_reads<DP>(lane);
+  uint32_t koff[MhaStage<DK, KT, 4>::N], voff[MhaStage<DV, KT, 4>::N];
+  mha_offsets<DK, KT, 4>(koff, wave, lane, a.kt, a.D);
+  mha_offsets<DV, KT, 4>(voff, wave, lane, a.vt, a.Dv);
+  const MhaReads<DK> rk = mha_reads<DK>(lane);
+  const MhaReads<DV> rv = mha_reads<DV>(lane);
   const bf16_t* kb = a.k + (int64_t)it.hk * a.kh;
   const bf16_t* vb = a.v + (int64_t)it.hk * a.vh;
   const uint32_t lds = cg_lds_addr(smem);
   mha_lds_ptr sm = (mha_lds_ptr)smem;
   auto stage = [&](int k0, int buf) {
-    mha_copy<DP, KT, 4>(koff, mha_rows<KT>(kb, it.k_start + k0, it.Lk - k0, a.kt, a.D), lds + buf * 2 * TILE, wave);
-    mha_copy<DP, KT, 4>(voff, mha_rows<KT>(vb, it.k_start + k0, it.Lk - k0, a.vt, a.Dv), lds + buf * 2 * TILE + TILE, wave);
+    mha_copy<DK, KT, 4>(koff, mha_rows<KT>(kb, it.k_start + k0, it.Lk - k0, a.kt, a.D), lds + buf * TILES, wave);
+    mha_copy<DV, KT, 4>(voff, mha_rows<KT>(vb, it.k_start + k0, it.Lk - k0, a.vt, a.Dv), lds + buf * TILES + TK, wave);
   };
-  f32x16_t o[DP / 32];
+  f32x16_t o[DV / 32];
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) o[i] = mha_zero();
+  for (int i = 0; i < DV / 32; ++i) o[i] = mha_zero();
   float m = -INFINITY, l = 0.f;
   if (it.k0 < it.k1) stage(it.k0, 0);
   mha_settle(qf);
@@ -419,15 +421,15 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : DP <= 96 ? 3 : 2) void mha_fwd_
     __syncthreads();
     if (k0 + KT < it.k1) stage(k0 + KT, buf ^ 1);
     if (k0 + KT - 1 > cut) {                       // the diagonal
-      mha_clean<DP, KT, 256, false>(smem + buf * 2 * TILE + TILE, threadIdx.x, &sm_bad[buf]);
+      mha_clean<DV, KT, 256, false>(smem + buf * TILES + TK, threadIdx.x, &sm_bad[buf]);
       __syncthreads();
       if (k0 + sm_bad[buf] <= last) l = __builtin_nanf("");
     }
     if (k0 > most) continue;
-    mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
+    mha_lds_ptr ks = sm + buf * TILES, vs = ks + TK;
     f32x16_t s[2];
-    s[0] = mha_product<DP>(ks, rd, qf, 0);
-    s[1] = mha_product<DP>(ks, rd, qf, 1);
+    s[0] = mha_product<DK>(ks, rk, qf, 0);
+    s[1] = mha_product<DK>(ks, rk, qf, 1);
     if (k0 + KT - 1 > least) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -435,25 +437,25 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : DP <= 96 ? 3 : 2) void mha_fwd_
         for (int v = 0; v < 16; ++v)
           s[n][v] = k0 + n * 32 + mha_key(v, half) <= last ? s[n][v] : -INFINITY;
     }
-    mha_softmax<2, DP / 32>(s, a.c, m, l, o);
-    mha_accumulate<DP>(o, vs, rd, s[0], 0);
-    mha_accumulate<DP>(o, vs, rd, s[1], 1);
+    mha_softmax<2, DV / 32>(s, a.c, m, l, o);
+    mha_accumulate<DV>(o, vs, rv, s[0], 0);
+    mha_accumulate<DV>(o, vs, rv, s[1], 1);
     if (GRAD && most < FEW) {
-      mha_accumulate_low<DP>(o, vs, rd, s[0], 0);
-      mha_accumulate_low<DP>(o, vs, rd, s[1], 1);
+      mha_accumulate_low<DV>(o, vs, rv, s[0], 0);
+      mha_accumulate_low<DV>(o, vs, rv, s[1], 1);
     }
   }
   l += __shfl_xor(l, 32, 64);
-  mha_store<DP, GRAD>(a, it, r, m, l, o, half);
+  mha_store<DV, GRAD>(a, it, r, m, l, o, half);
 }
 
 // ---- forward, at most 32 rows: the keys split over the waves --------------------------------------
 // One wave holds all rows; each of the NW waves takes every NW-th step of 32 keys through an LDS ring of its
 // own (no barrier in the loop), and the waves' results are joined at the end.  Bound by reading K and V.
-template <int DP, int NW, bool GRAD>
+template <int DK, int DV, int NW, bool GRAD>
 __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
-  constexpr int TILE = 32 * DP * 2;              // one matrix, 32 keys
-  constexpr int RING = 2 * 2 * TILE;             // K and V, two buffers, a wave
+  constexpr int TK = 32 * DK * 2, TILES = TK + 32 * DV * 2;      // 32 keys of K, and with V
+  constexpr int RING = 2 * TILES;                // two buffers, a wave
   __shared__ __attribute__((aligned(1024))) unsigned char smem[NW * RING];
   __shared__ float sm_m[NW][32], sm_l[NW][32];
   __shared__ int sm_bad[NW];
@@ -463,7 +465,7 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
   int t, h;
   mha_token(a, it, col, &t, &h);
   const bool ok = col < it.rows;
-  bf16x8_t qf[DP / 16];
+  bf16x8_t qf[DK / 16];
   mha_row_frags(qf, a.q + (int64_t)(it.q_start + t) * a.qt + (int64_t)h * a.qh, ok, a.D, half);
   const int last = ok ? min(it.k1 - 1, t + it.shift) : -1;
   int least = last;
@@ -474,25 +476,27 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
     for (int s = 0; s < it.rows; ++s) least = min(least, __shfl(last, s, 64));
   }
   least = __builtin_amdgcn_readfirstlane(least);
-  using Stage = MhaStage<DP, 32, 1>;
-  uint32_t koff[Stage::N], voff[Stage::N];
-  mha_offsets<DP, 32, 1>(koff, 0, lane, a.kt, a.D);
-  mha_offsets<DP, 32, 1>(voff, 0, lane, a.vt, a.Dv);
-  const MhaReads<DP> rd = mha_reads<DP>(lane);
+  using StageK = MhaStage<DK, 32, 1>;
+  using StageV = MhaStage<DV, 32, 1>;
+  uint32_t koff[StageK::N], voff[StageV::N];
+  mha_offsets<DK, 32, 1>(koff, 0, lane, a.kt, a.D);
+  mha_offsets<DV, 32, 1>(voff, 0, lane, a.vt, a.Dv);
+  const MhaReads<DK> rk = mha_reads<DK>(lane);
+  const MhaReads<DV> rv = mha_reads<DV>(lane);
   const bf16_t* kb = a.k + (int64_t)it.hk * a.kh;
   const bf16_t* vb = a.v + (int64_t)it.hk * a.vh;
   const uint32_t lds = cg_lds_addr(smem) + wave * RING;
   mha_lds_ptr sm = (mha_lds_ptr)smem + wave * RING;
   auto stage = [&](int k0, int buf) {
-    mha_copy<DP, 32, 1>(koff, mha_rows<32>(kb, it.k_start + k0, it.Lk - k0, a.kt, a.D), lds + buf * 2 * TILE, 0);
-    mha_copy<DP, 32, 1>(voff, mha_rows<32>(vb, it.k_start + k0, it.Lk - k0, a.vt, a.Dv), lds + buf * 2 * TILE + TILE, 0);
+    mha_copy<DK, 32, 1>(koff, mha_rows<32>(kb, it.k_start + k0, it.Lk - k0, a.kt, a.D), lds + buf * TILES, 0);
+    mha_copy<DV, 32, 1>(voff, mha_rows<32>(vb, it.k_start + k0, it.Lk - k0, a.vt, a.Dv), lds + buf * TILES + TK, 0);
   };
-  f32x16_t o[DP / 32];
+  f32x16_t o[DV / 32];
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) o[i] = mha_zero();
+  for (int i = 0; i < DV / 32; ++i) o[i] = mha_zero();
   float m = -INFINITY, l = 0.f;
   const int first = it.k0 + wave * 32;
-  constexpr int INFLIGHT = 2 * Stage::N;         // copies of one step
+  constexpr int INFLIGHT = StageK::N + StageV::N;         // copies of one step
   if (first < it.k1) stage(first, 0);
   mha_settle(qf);
   int buf = 0;
@@ -505,22 +509,22 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
+    mha_lds_ptr ks = sm + buf * TILES, vs = ks + TK;
     if (a.causal && k0 + 31 > least) {             // the diagonal: this wave's own tile and flag
       if (lane == 0) sm_bad[wave] = NONE_BAD;
-      mha_clean<DP, 32, 64, false>(smem + wave * RING + buf * 2 * TILE + TILE, lane, &sm_bad[wave]);
+      mha_clean<DV, 32, 64, false>(smem + wave * RING + buf * TILES + TK, lane, &sm_bad[wave]);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (k0 + *(volatile int*)&sm_bad[wave] <= last) l = __builtin_nanf("");
     }
     f32x16_t s[1];
-    s[0] = mha_product<DP>(ks, rd, qf, 0);
+    s[0] = mha_product<DK>(ks, rk, qf, 0);
     if (k0 + 31 > least) {
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[0][v] = k0 + mha_key(v, half) <= last ? s[0][v] : -INFINITY;
     }
-    mha_softmax<1, DP / 32>(s, a.c, m, l, o);
-    mha_accumulate<DP>(o, vs, rd, s[0], 0);
-    if (GRAD && it.k1 <= FEW) mha_accumulate_low<DP>(o, vs, rd, s[0], 0);
+    mha_softmax<1, DV / 32>(s, a.c, m, l, o);
+    mha_accumulate<DV>(o, vs, rv, s[0], 0);
+    if (GRAD && it.k1 <= FEW) mha_accumulate_low<DV>(o, vs, rv, s[0], 0);
   }
   l += __shfl_xor(l, 32, 64);
   if constexpr (NW > 1) {
@@ -539,23 +543,23 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
     // joined two waves at a time in a fixed order: wave w hands its scaled O to wave w - step
     float* box = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
+    for (int i = 0; i < DV / 32; ++i)
 #pragma unroll
       for (int v = 0; v < 16; ++v) o[i][v] *= mine;
 #pragma unroll
     for (int step = NW / 2; step > 0; step >>= 1) {
       if (wave >= step && wave < 2 * step) {
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
+        for (int i = 0; i < DV / 32; ++i)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) box[((wave - step) * (DP / 32) * 16 + i * 16 + v) * 64 + lane] = o[i][v];
+          for (int v = 0; v < 16; ++v) box[((wave - step) * (DV / 32) * 16 + i * 16 + v) * 64 + lane] = o[i][v];
       }
       __syncthreads();
       if (wave < step) {
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
+        for (int i = 0; i < DV / 32; ++i)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) o[i][v] += box[(wave * (DP / 32) * 16 + i * 16 + v) * 64 + lane];
+          for (int v = 0; v < 16; ++v) o[i][v] += box[(wave * (DV / 32) * 16 + i * 16 + v) * 64 + lane];
       }
       __syncthreads();
     }
@@ -563,7 +567,7 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
     m = top;
     l = total;
   }
-  mha_store<DP, GRAD>(a, it, col, m, l, o, half);
+  mha_store<DV, GRAD>(a, it, col, m, l, o, half);
 }
 
 // ---- joins the partial results of a split item; one wave a row, its parts' loads in flight together ------
@@ -624,10 +628,10 @@ __device__ __forceinline__ float mha_lse2(float lse) { return lse == -INFINITY ?
 // rows is formed on the way in (dO is in registers for dP) and left for the dK / dV kernel behind it.  dS = P (dP - delta)
 // is a difference: with the rounded out alone its error would come on top of the rounding of dS (dQ 1.5 instead of 1.4
 // roundings off).
-template <int DP>
-__global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArgs a) {
-  constexpr int TILE = KT * DP * 2;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];
+template <int DK, int DV>
+__global__ __launch_bounds__(256, mha_wider(DK, DV) <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArgs a) {
+  constexpr int TK = KT * DK * 2, TILES = TK + KT * DV * 2;      // K, and K with V
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * TILES];
   __shared__ int sm_bad[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, col = lane & 31;
@@ -638,13 +642,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
   mha_token(a, it, r, &t, &h);
   const bool ok = r < it.rows;
   const int64_t row = (int64_t)(it.q_start + t) * a.heads + h;
-  bf16x8_t qf[DP / 16], df[DP / 16];
+  bf16x8_t qf[DK / 16], df[DV / 16];
   mha_row_frags(qf, a.q + (int64_t)(it.q_start + t) * a.qt + (int64_t)h * a.qh, ok, a.D, half);
   mha_row_frags(df, a.dout + row * a.Dv, ok, a.Dv, half);
   const float lse2 = ok ? mha_lse2(a.lse_in[row]) : INFINITY;
   float delta = 0.f;
 #pragma unroll
-  for (int kd = 0; kd < DP / 16; ++kd) {
+  for (int kd = 0; kd < DV / 16; ++kd) {
     const int d = kd * 16 + half * 8;
     if (ok && d < a.Dv) {
       float x[8], y[8], z[8];
@@ -666,22 +670,22 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
   }
   least = __builtin_amdgcn_readfirstlane(least);
   most = __builtin_amdgcn_readfirstlane(most);
-  using Stage = MhaStage<DP, KT, 4>;
-  uint32_t koff[Stage::N], voff[Stage::N];
-  mha_offsets<DP, KT, 4>(koff, wave, lane, a.kt, a.D);
-  mha_offsets<DP, KT, 4>(voff, wave, lane, a.vt, a.Dv);
-  const MhaReads<DP> rd = mha_reads<DP>(lane);
+  uint32_t koff[MhaStage<DK, KT, 4>::N], voff[MhaStage<DV, KT, 4>::N];
+  mha_offsets<DK, KT, 4>(koff, wave, lane, a.kt, a.D);
+  mha_offsets<DV, KT, 4>(voff, wave, lane, a.vt, a.Dv);
+  const MhaReads<DK> rk = mha_reads<DK>(lane);
+  const MhaReads<DV> rv = mha_reads<DV>(lane);
   const bf16_t* kb = a.k + (int64_t)it.hk * a.kh;
   const bf16_t* vb = a.v + (int64_t)it.hk * a.vh;
   const uint32_t lds = cg_lds_addr(smem);
   mha_lds_ptr sm = (mha_lds_ptr)smem;
   auto stage = [&](int k0, int buf) {
-    mha_copy<DP, KT, 4>(koff, mha_rows<KT>(kb, it.k_start + k0, it.Lk - k0, a.kt, a.D), lds + buf * 2 * TILE, wave);
-    mha_copy<DP, KT, 4>(voff, mha_rows<KT>(vb, it.k_start + k0, it.Lk - k0, a.vt, a.Dv), lds + buf * 2 * TILE + TILE, wave);
+    mha_copy<DK, KT, 4>(koff, mha_rows<KT>(kb, it.k_start + k0, it.Lk - k0, a.kt, a.D), lds + buf * TILES, wave);
+    mha_copy<DV, KT, 4>(voff, mha_rows<KT>(vb, it.k_start + k0, it.Lk - k0, a.vt, a.Dv), lds + buf * TILES + TK, wave);
   };
-  f32x16_t dq[DP / 32];
+  f32x16_t dq[DK / 32];
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) dq[i] = mha_zero();
+  for (int i = 0; i < DK / 32; ++i) dq[i] = mha_zero();
   if (it.k0 < it.k1) stage(it.k0, 0);
   float scale = a.scale;         // NaN: the row saw a key that is not finite
   mha_settle(qf);
@@ -693,17 +697,17 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
     __syncthreads();
     if (k0 + KT < it.k1) stage(k0 + KT, buf ^ 1);
     if (k0 + KT - 1 > cut) {                       // the diagonal
-      mha_clean<DP, KT, 256, false>(smem + buf * 2 * TILE, threadIdx.x, &sm_bad[buf]);
+      mha_clean<DK, KT, 256, false>(smem + buf * TILES, threadIdx.x, &sm_bad[buf]);
       __syncthreads();
       if (k0 + sm_bad[buf] <= last) scale = __builtin_nanf("");
     }
     if (k0 > most) continue;
-    mha_lds_ptr ks = sm + buf * 2 * TILE, vs = ks + TILE;
+    mha_lds_ptr ks = sm + buf * TILES, vs = ks + TK;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       __builtin_amdgcn_sched_barrier(0);      // one step's scores live at a time
-      f32x16_t s = mha_product<DP>(ks, rd, qf, n);
-      const f32x16_t dp = mha_product<DP>(vs, rd, df, n);
+      f32x16_t s = mha_product<DK>(ks, rk, qf, n);
+      const f32x16_t dp = mha_product<DV>(vs, rv, df, n);
 #pragma unroll
       for (int v = 0; v < 16; ++v)
         s[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[v], a.c, -lse2)) * (dp[v] - delta);
@@ -711,17 +715,17 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
 #pragma unroll
         for (int v = 0; v < 16; ++v) s[v] = k0 + n * 32 + mha_key(v, half) <= last ? s[v] : 0.f;
       }
-      mha_accumulate<DP>(dq, ks, rd, s, n);
+      mha_accumulate<DK>(dq, ks, rk, s, n);
     }
   }
   if (!ok) return;
   if (it.part >= 0) {
-    mha_store_part<DP>(a.ws_o + ((int64_t)it.part * ROW_TILE + r - it.row0) * a.D, dq, a.D, half, scale == scale ? 1.f : scale);
+    mha_store_part<DK>(a.ws_o + ((int64_t)it.part * ROW_TILE + r - it.row0) * a.D, dq, a.D, half, scale == scale ? 1.f : scale);
     return;
   }
   bf16_t* dst = a.dq + row * a.D;
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
+  for (int i = 0; i < DK / 32; ++i)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = i * 32 + g * 8 + 4 * half;
@@ -736,12 +740,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 4 : 2) void mha_bwd_q_kernel(MhaArg
 // columns; dV^T += dO^T P, dK^T += Q^T dS.  Item {seq, hk, key0, first row, end row}.
 // At 128 wide heads the accumulators, K and V of a wave would be 192 registers and the rest spills (each reload also
 // waits for the copies in flight): V is read from LDS there, and the tiles are 32 rows so that two workgroups fit a CU.
-template <int DP>
-__global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaArgs a) {
-  constexpr bool V_LDS = DP > 96;
+template <int DK, int DV>
+__global__ __launch_bounds__(256, mha_wider(DK, DV) <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaArgs a) {
+  constexpr bool V_LDS = DK + DV > 224;
   constexpr int RT = V_LDS ? 32 : 64;             // rows of a tile
-  constexpr int TILE = RT * DP * 2, V_BYTES = V_LDS ? KEY_TILE * DP * 2 : 0;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE + V_BYTES];
+  constexpr int TQ = RT * DK * 2, TILES = TQ + RT * DV * 2;      // Q, and Q with dO
+  constexpr int V_BYTES = V_LDS ? KEY_TILE * DV * 2 : 0;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * TILES + V_BYTES];
   __shared__ __attribute__((aligned(16))) float stat[2][2][RT];   // [buffer][lse, -delta][row]
   __shared__ int sm_bad[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -749,7 +754,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
   const MhaItem it = mha_item(a, blockIdx.x);
   const int key = it.row0 + wave * 32 + col;
   const bool ok = key < it.Lk;
-  bf16x8_t kf[DP / 16], vf[V_LDS ? 1 : DP / 16];
+  bf16x8_t kf[DK / 16], vf[V_LDS ? 1 : DV / 16];
   mha_row_frags(kf, a.k + (int64_t)(it.k_start + key) * a.kt + (int64_t)it.hk * a.kh, ok, a.D, half);
   if constexpr (!V_LDS) mha_row_frags(vf, a.v + (int64_t)(it.k_start + key) * a.vt + (int64_t)it.hk * a.vh, ok, a.Dv, half);
   // first row that sees this key; rows of the wave's first and last key for skipping and masking
@@ -759,8 +764,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
   const int all_first = first_row(min(it.row0 + KEY_TILE, it.Lk) - 1);   // first row that sees all keys of the item
   const bool some = it.row0 + wave * 32 < it.Lk;
   const int rb = it.k0, re = it.k1;
-  using Stage = MhaStage<DP, RT, 4>;
-  const MhaReads<DP> rd = mha_reads<DP>(lane);
+  const MhaReads<DK> rk = mha_reads<DK>(lane);
+  const MhaReads<DV> rv = mha_reads<DV>(lane);
   const bf16_t* qb = a.q + (int64_t)it.hk * a.G * a.qh;
   const bf16_t* db = a.dout + (int64_t)it.hk * a.G * a.Dv;
   const uint32_t lds = cg_lds_addr(smem);
@@ -771,24 +776,27 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
     const int t0 = __builtin_amdgcn_readfirstlane((int)fdiv((uint32_t)r0, a.dG));
     const cg_i32x4_t qr = cg_make_rsrc(qb + (int64_t)(it.q_start + t0) * a.qt, 0x7fffffffu);
     const cg_i32x4_t dr = cg_make_rsrc(db + (int64_t)(it.q_start + t0) * dt, 0x7fffffffu);
+    auto gather = [&](auto stage_of, const cg_i32x4_t& rs, int width, uint32_t row_bytes, uint32_t head_bytes,
+                      uint32_t to) {
+      using Stage = decltype(stage_of);
 #pragma unroll
-    for (int n = 0; n < Stage::N; ++n) {
-      int i, c;
-      Stage::place(n, wave, lane, &i, &c);
-      const int r = r0 + i;
-      const int t = (int)fdiv((uint32_t)r, a.dG), g = r - t * a.G;
-      const bool in = r < re;
-      const uint32_t at = lds + buf * 2 * TILE + (uint32_t)(n * 4 + wave) * 1024u;
-      cg_dma16_asm(qr, in && c < a.D ? (uint32_t)(t - t0) * (uint32_t)(a.qt * 2) + (uint32_t)g * (uint32_t)(a.qh * 2) + c * 2 : OUTSIDE, 0u, at);
-      cg_dma16_asm(dr, in && c < a.Dv ? (uint32_t)(t - t0) * (uint32_t)(dt * 2) + (uint32_t)g * (uint32_t)(a.Dv * 2) + c * 2 : OUTSIDE, 0u, at + TILE);
-    }
+      for (int n = 0; n < Stage::N; ++n) {
+        int i, c;
+        Stage::place(n, wave, lane, &i, &c);
+        const int r = r0 + i;
+        const int t = (int)fdiv((uint32_t)r, a.dG), g = r - t * a.G;
+        cg_dma16_asm(rs, r < re && c < width ? (uint32_t)(t - t0) * row_bytes + (uint32_t)g * head_bytes + c * 2 : OUTSIDE,
+                     0u, to + (uint32_t)(n * 4 + wave) * 1024u);
+      }
+    };
+    gather(MhaStage<DK, RT, 4>(), qr, a.D, (uint32_t)(a.qt * 2), (uint32_t)(a.qh * 2), lds + buf * TILES);
+    gather(MhaStage<DV, RT, 4>(), dr, a.Dv, (uint32_t)(dt * 2), (uint32_t)(a.Dv * 2), lds + buf * TILES + TQ);
   };
-  f32x16_t dk[DP / 32], dv[DP / 32];
+  f32x16_t dk[DK / 32], dv[DV / 32];
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) {
-    dk[i] = mha_zero();
-    dv[i] = mha_zero();
-  }
+  for (int i = 0; i < DK / 32; ++i) dk[i] = mha_zero();
+#pragma unroll
+  for (int i = 0; i < DV / 32; ++i) dv[i] = mha_zero();
 
   // wave 0 / 1 carry the statistics of the next tile, one row a lane: loaded here, touched a tile later (a use next to
   // the load would hold the two waves, and at the barrier all, for the load's whole latency in every tile)
@@ -802,10 +810,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
   float next = 0.f;
   if (rb < re) {
     if constexpr (V_LDS) {                          // the item's 128 rows of V, once
-      uint32_t voff[MhaStage<DP, KEY_TILE, 4>::N];
-      mha_offsets<DP, KEY_TILE, 4>(voff, wave, lane, a.vt, a.Dv);
-      mha_copy<DP, KEY_TILE, 4>(voff, mha_rows<KEY_TILE>(a.v + (int64_t)it.hk * a.vh, it.k_start + it.row0, it.Lk - it.row0,
-                                                         a.vt, a.Dv), lds + 4 * TILE, wave);
+      uint32_t voff[MhaStage<DV, KEY_TILE, 4>::N];
+      mha_offsets<DV, KEY_TILE, 4>(voff, wave, lane, a.vt, a.Dv);
+      mha_copy<DV, KEY_TILE, 4>(voff, mha_rows<KEY_TILE>(a.v + (int64_t)it.hk * a.vh, it.k_start + it.row0, it.Lk - it.row0,
+                                                         a.vt, a.Dv), lds + 2 * TILES, wave);
     }
     next = stat_load(rb);
     stage(rb, 0);
@@ -824,13 +832,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
       stage(r0 + RT, buf ^ 1);
     }
     if (r0 < all_first) {                          // the diagonal
-      mha_clean<DP, RT, 256, true>(smem + buf * 2 * TILE, threadIdx.x, &sm_bad[buf]);
-      mha_clean<DP, RT, 256, true>(smem + buf * 2 * TILE + TILE, threadIdx.x, &sm_bad[buf]);
+      mha_clean<DK, RT, 256, true>(smem + buf * TILES, threadIdx.x, &sm_bad[buf]);
+      mha_clean<DV, RT, 256, true>(smem + buf * TILES + TQ, threadIdx.x, &sm_bad[buf]);
       __syncthreads();
       if (r0 + sm_bad[buf] >= mine) scale = __builtin_nanf("");
     }
     if (!some) continue;
-    mha_lds_ptr qs = sm + buf * 2 * TILE, ds = qs + TILE;
+    mha_lds_ptr qs = sm + buf * TILES, ds = qs + TQ;
 #pragma unroll
     for (int n = 0; n < RT / 32; ++n) {
       __builtin_amdgcn_sched_barrier(0);      // one step's scores live at a time
@@ -844,19 +852,19 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
 #pragma unroll
         for (int j = 0; j < 4; ++j) dp[4 * g + j] = de[j];
       }
-      f32x16_t s = mha_product<DP>(qs, rd, kf, n);
-      if (DP > 64) __builtin_amdgcn_sched_barrier(0);
+      f32x16_t s = mha_product<DK>(qs, rk, kf, n);
+      if (mha_wider(DK, DV) > 64) __builtin_amdgcn_sched_barrier(0);
       if constexpr (V_LDS) {
-        mha_lds_ptr vs = sm + 4 * TILE + wave * 64 * DP;
+        mha_lds_ptr vs = sm + 2 * TILES + wave * 64 * DV;
 #pragma unroll
-        for (int kd = 0; kd < DP / 16; ++kd) {
-          const bf16x8_t x = *(mha_frag_ptr)(ds + rd.row[kd] + n * 64 * DP), y = *(mha_frag_ptr)(vs + rd.row[kd]);
+        for (int kd = 0; kd < DV / 16; ++kd) {
+          const bf16x8_t x = *(mha_frag_ptr)(ds + rv.row[kd] + n * 64 * DV), y = *(mha_frag_ptr)(vs + rv.row[kd]);
           dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, dp, 0, 0, 0);
         }
       } else {
-        dp = mha_product<DP>(ds, rd, vf, n, dp);
+        dp = mha_product<DV>(ds, rv, vf, n, dp);
       }
-      if (DP > 64) __builtin_amdgcn_sched_barrier(0);
+      if (mha_wider(DK, DV) > 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4_t ls = *reinterpret_cast<const f32x4_t*>(&stat[buf][0][n * 32 + 8 * g + 4 * half]);
@@ -875,32 +883,34 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaAr
           dp[v] = see ? dp[v] : 0.f;
         }
       }
-      if (DP > 64) __builtin_amdgcn_sched_barrier(0);
-      mha_accumulate<DP>(dv, ds, rd, s, n);
-      if (DP > 64) __builtin_amdgcn_sched_barrier(0);
-      mha_accumulate<DP>(dk, qs, rd, dp, n);
+      if (mha_wider(DK, DV) > 64) __builtin_amdgcn_sched_barrier(0);
+      mha_accumulate<DV>(dv, ds, rv, s, n);
+      if (mha_wider(DK, DV) > 64) __builtin_amdgcn_sched_barrier(0);
+      mha_accumulate<DK>(dk, qs, rk, dp, n);
     }
   }
   if (!ok) return;
   const float one = scale == scale ? 1.f : scale;
   if (it.part >= 0) {
     float* dst = a.ws_o + ((int64_t)it.part * KEY_TILE + key - it.row0) * (a.D + a.Dv);
-    mha_store_part<DP>(dst, dk, a.D, half, one);
-    mha_store_part<DP>(dst + a.D, dv, a.Dv, half, one);
+    mha_store_part<DK>(dst, dk, a.D, half, one);
+    mha_store_part<DV>(dst + a.D, dv, a.Dv, half, one);
     return;
   }
   bf16_t* dkp = a.dk + ((int64_t)(it.k_start + key) * a.kv_heads + it.hk) * a.D;
   bf16_t* dvp = a.dv + ((int64_t)(it.k_start + key) * a.kv_heads + it.hk) * a.Dv;
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
+  auto store = [&](const f32x16_t& acc, int i, float f, bf16_t* dst, int width) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = i * 32 + g * 8 + 4 * half;
-      const float w[4] = {dk[i][4 * g] * scale, dk[i][4 * g + 1] * scale, dk[i][4 * g + 2] * scale, dk[i][4 * g + 3] * scale};
-      const float u[4] = {dv[i][4 * g] * one, dv[i][4 * g + 1] * one, dv[i][4 * g + 2] * one, dv[i][4 * g + 3] * one};
-      if (d < a.D) *reinterpret_cast<uint2*>(dkp + d) = pack4_bf16(w);
-      if (d < a.Dv) *reinterpret_cast<uint2*>(dvp + d) = pack4_bf16(u);
+      const float w[4] = {acc[4 * g] * f, acc[4 * g + 1] * f, acc[4 * g + 2] * f, acc[4 * g + 3] * f};
+      if (d < width) *reinterpret_cast<uint2*>(dst + d) = pack4_bf16(w);
     }
+  };
+#pragma unroll
+  for (int i = 0; i < DK / 32; ++i) store(dk[i], i, scale, dkp, a.D);
+#pragma unroll
+  for (int i = 0; i < DV / 32; ++i) store(dv[i], i, one, dvp, a.Dv);
 }
 
 // sums the partial gradients of a split item in their order: item {seq, hk, row0, rows here, parts, first part},
@@ -937,63 +947,70 @@ __global__ __launch_bounds__(256) void mha_join_grad_kernel(MhaArgs a) {
 // and dO read.  The scores are formed both ways round (S^T for dQ, S for dK and dV); the softmax statistics and
 // delta = sum_k P dP come from the scores themselves, exact in fp32, and reach the other orientation by lane
 // exchanges.  Bound by latency: a launch of one wave workgroups, many a CU.
-template <int DP>
+template <int DK, int DV>
 __global__ __launch_bounds__(64) void mha_bwd_small_kernel(MhaArgs a) {
-  constexpr int TILE = 32 * DP * 2;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[3 * TILE];   // K, Q, dO
+  constexpr int TK = 32 * DK * 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * TK + 32 * DV * 2];   // K, Q, dO
   __shared__ int sm_bad[2];
   const int lane = threadIdx.x, half = lane >> 5, col = lane & 31;
   const MhaItem it = mha_item(a, blockIdx.x);
-  using Stage = MhaStage<DP, 32, 1>;
-  const MhaReads<DP> rd = mha_reads<DP>(lane);
+  const MhaReads<DK> rk = mha_reads<DK>(lane);
+  const MhaReads<DV> rv = mha_reads<DV>(lane);
   const uint32_t lds = cg_lds_addr(smem);
-  mha_lds_ptr ks = (mha_lds_ptr)smem, qs = ks + TILE, ds = ks + 2 * TILE;
+  mha_lds_ptr ks = (mha_lds_ptr)smem, qs = ks + TK, ds = ks + 2 * TK;
   const int64_t dt = (int64_t)a.heads * a.Dv;
   {
-    uint32_t koff[Stage::N];
-    mha_offsets<DP, 32, 1>(koff, 0, lane, a.kt, a.D);
-    mha_copy<DP, 32, 1>(koff, mha_rows<32>(a.k + (int64_t)it.hk * a.kh, it.k_start, it.Lk, a.kt, a.D), lds, 0);
+    uint32_t koff[MhaStage<DK, 32, 1>::N];
+    mha_offsets<DK, 32, 1>(koff, 0, lane, a.kt, a.D);
+    mha_copy<DK, 32, 1>(koff, mha_rows<32>(a.k + (int64_t)it.hk * a.kh, it.k_start, it.Lk, a.kt, a.D), lds, 0);
     const cg_i32x4_t qr = cg_make_rsrc(a.q + (int64_t)it.hk * a.G * a.qh + (int64_t)it.q_start * a.qt, 0x7fffffffu);
     const cg_i32x4_t dr = cg_make_rsrc(a.dout + (int64_t)it.hk * a.G * a.Dv + (int64_t)it.q_start * dt, 0x7fffffffu);
+    auto gather = [&](auto stage_of, const cg_i32x4_t& rs, int width, uint32_t row_bytes, uint32_t head_bytes,
+                      uint32_t to) {
+      using Stage = decltype(stage_of);
 #pragma unroll
-    for (int n = 0; n < Stage::N; ++n) {
-      int r, c;
-      Stage::place(n, 0, lane, &r, &c);
-      const int t = (int)fdiv((uint32_t)r, a.dG), g = r - t * a.G;
-      // rows that see no key are left out: their dO may hold anything
-      const bool in = r < it.rows && t + it.shift >= 0;
-      cg_dma16_asm(qr, in && c < a.D ? (uint32_t)t * (uint32_t)(a.qt * 2) + (uint32_t)g * (uint32_t)(a.qh * 2) + c * 2 : OUTSIDE, 0u, lds + TILE + n * 1024u);
-      cg_dma16_asm(dr, in && c < a.Dv ? (uint32_t)t * (uint32_t)(dt * 2) + (uint32_t)g * (uint32_t)(a.Dv * 2) + c * 2 : OUTSIDE, 0u, lds + 2 * TILE + n * 1024u);
-    }
+      for (int n = 0; n < Stage::N; ++n) {
+        int r, c;
+        Stage::place(n, 0, lane, &r, &c);
+        const int t = (int)fdiv((uint32_t)r, a.dG), g = r - t * a.G;
+        // rows that see no key are left out: their dO may hold anything
+        const bool in = r < it.rows && t + it.shift >= 0 && c < width;
+        cg_dma16_asm(rs, in ? (uint32_t)t * row_bytes + (uint32_t)g * head_bytes + c * 2 : OUTSIDE, 0u, to + n * 1024u);
+      }
+    };
+    gather(MhaStage<DK, 32, 1>(), qr, a.D, (uint32_t)(a.qt * 2), (uint32_t)(a.qh * 2), lds + TK);
+    gather(MhaStage<DV, 32, 1>(), dr, a.Dv, (uint32_t)(dt * 2), (uint32_t)(a.Dv * 2), lds + 2 * TK);
   }
   int t, h;
   mha_token(a, it, col, &t, &h);
   const bool row_ok = col < it.rows, key_ok = col < it.Lk;
-  bf16x8_t vf[DP / 16];
+  bf16x8_t vf[DV / 16];
   mha_row_frags(vf, a.v + (int64_t)(it.k_start + col) * a.vt + (int64_t)it.hk * a.vh, key_ok, a.Dv, half);
   if (lane < 2) sm_bad[lane] = lane ? -NONE_BAD : NONE_BAD;
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  bf16x8_t kf[DP / 16], qf[DP / 16], df[DP / 16];
+  bf16x8_t kf[DK / 16], qf[DK / 16], df[DV / 16];
 #pragma unroll
-  for (int kd = 0; kd < DP / 16; ++kd) {
-    kf[kd] = *(mha_frag_ptr)(ks + rd.row[kd]);
-    qf[kd] = *(mha_frag_ptr)(qs + rd.row[kd]);
-    df[kd] = *(mha_frag_ptr)(ds + rd.row[kd]);
+  for (int kd = 0; kd < DK / 16; ++kd) {
+    kf[kd] = *(mha_frag_ptr)(ks + rk.row[kd]);
+    qf[kd] = *(mha_frag_ptr)(qs + rk.row[kd]);
   }
+#pragma unroll
+  for (int kd = 0; kd < DV / 16; ++kd) df[kd] = *(mha_frag_ptr)(ds + rv.row[kd]);
   int bad_key = NONE_BAD, bad_row = -NONE_BAD;
   if (a.causal) {       // (the scores above keep what is not finite: they are masked one by one)
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    mha_clean<DP, 32, 64, false>(smem, lane, &sm_bad[0]);
-    mha_clean<DP, 32, 64, true>(smem + TILE, lane, &sm_bad[1]);
-    mha_clean<DP, 32, 64, true>(smem + 2 * TILE, lane, &sm_bad[1]);
+    mha_clean<DK, 32, 64, false>(smem, lane, &sm_bad[0]);
+    mha_clean<DK, 32, 64, true>(smem + TK, lane, &sm_bad[1]);
+    mha_clean<DV, 32, 64, true>(smem + 2 * TK, lane, &sm_bad[1]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     bad_key = *(volatile int*)&sm_bad[0];
     bad_row = *(volatile int*)&sm_bad[1];
   }
-  auto product = [&](const bf16x8_t (&x)[DP / 16], const bf16x8_t (&y)[DP / 16]) {
+  auto product = [&](const auto& x, const auto& y) {
     f32x16_t s = mha_zero();
 #pragma unroll
-    for (int kd = 0; kd < DP / 16; ++kd) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[kd], y[kd], s, 0, 0, 0);
+    for (size_t kd = 0; kd < sizeof(x) / sizeof(x[0]); ++kd)
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[kd], y[kd], s, 0, 0, 0);
     return s;
   };
   // rows in the lanes' columns: statistics, delta, dQ
@@ -1023,25 +1040,25 @@ __global__ __launch_bounds__(64) void mha_bwd_small_kernel(MhaArgs a) {
   delta += __shfl_xor(delta, 32, 64);
 #pragma unroll
   for (int v = 0; v < 16; ++v) s[v] = mha_key(v, half) <= last ? s[v] * (dp[v] - delta) : 0.f;
-  f32x16_t acc[DP / 32];
-  auto clear = [&]() {
+  auto finish = [&](auto& acc, mha_lds_ptr tile, const auto& reads, const f32x16_t& w, bf16_t* dst, bool ok, float f,
+                    int width) {
+    constexpr int N = sizeof(acc) / sizeof(acc[0]);
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) acc[i] = mha_zero();
-  };
-  auto store = [&](bf16_t* dst, float f, int width) {
+    for (int i = 0; i < N; ++i) acc[i] = mha_zero();
+    mha_accumulate<N * 32>(acc, tile, reads, w, 0);
+    if (!ok) return;
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int d = i * 32 + g * 8 + 4 * half;
-        const float w[4] = {acc[i][4 * g] * f, acc[i][4 * g + 1] * f, acc[i][4 * g + 2] * f, acc[i][4 * g + 3] * f};
-        if (d < width) *reinterpret_cast<uint2*>(dst + d) = pack4_bf16(w);
+        const float x[4] = {acc[i][4 * g] * f, acc[i][4 * g + 1] * f, acc[i][4 * g + 2] * f, acc[i][4 * g + 3] * f};
+        if (d < width) *reinterpret_cast<uint2*>(dst + d) = pack4_bf16(x);
       }
   };
-  clear();
-  mha_accumulate<DP>(acc, ks, rd, s, 0);
-  if (row_ok)
-    store(a.dq + ((int64_t)(it.q_start + t) * a.heads + h) * a.D, bad_key <= last ? __builtin_nanf("") : a.scale, a.D);
+  f32x16_t acc_k[DK / 32], acc_v[DV / 32];
+  finish(acc_k, ks, rk, s, a.dq + ((int64_t)(it.q_start + t) * a.heads + h) * a.D, row_ok,
+         bad_key <= last ? __builtin_nanf("") : a.scale, a.D);
   // keys in the lanes' columns: dK, dV
   f32x16_t sk = product(qf, kf);
   f32x16_t dk = product(df, vf);
@@ -1055,13 +1072,9 @@ __global__ __launch_bounds__(64) void mha_bwd_small_kernel(MhaArgs a) {
     dk[v] = see ? sk[v] * (dk[v] - rdelta) : 0.f;
   }
   const int64_t key = (int64_t)(it.k_start + col) * a.kv_heads + it.hk;
-  clear();
-  mha_accumulate<DP>(acc, ds, rd, sk, 0);
   const float one = bad_row >= mine ? __builtin_nanf("") : 1.f;
-  if (key_ok) store(a.dv + key * a.Dv, one, a.Dv);
-  clear();
-  mha_accumulate<DP>(acc, qs, rd, dk, 0);
-  if (key_ok) store(a.dk + key * a.D, a.scale * one, a.D);
+  finish(acc_v, ds, rv, sk, a.dv + key * a.Dv, key_ok, one, a.Dv);
+  finish(acc_k, qs, rk, dk, a.dk + key * a.D, key_ok, a.scale * one, a.D);
 }
 
 // ---- the plan ------------------------------------------------------------------------------------
@@ -1294,27 +1307,36 @@ const int4* mha_list(const cgAttentionPlan* p, const int32_t* data, int which) {
   return (const int4*)(data + at);
 }
 
-// padded head width: both matrices of a tile have it
-int mha_width(int D, int Dv) { return ((D > Dv ? D : Dv) + 31) / 32 * 32; }
+// padded head width
+int mha_width(int D) { return (D + 31) / 32 * 32; }
 
 }  // namespace
 
-#define MHA_LAUNCH(dp, kernel, grid, block, st, args)                          \
-  switch (dp) {                                                                \
-    case 32: kernel(32)<<<grid, block, 0, st>>>(args); break;                  \
-    case 64: kernel(64)<<<grid, block, 0, st>>>(args); break;                  \
-    case 96: kernel(96)<<<grid, block, 0, st>>>(args); break;                  \
-    default: kernel(128)<<<grid, block, 0, st>>>(args); break;                 \
+// the kernel of the two padded head widths
+#define MHA_LAUNCH_DV(dk, dv, kernel, grid, block, st, args)                   \
+  switch (dv) {                                                                \
+    case 32: kernel(dk, 32)<<<grid, block, 0, st>>>(args); break;              \
+    case 64: kernel(dk, 64)<<<grid, block, 0, st>>>(args); break;              \
+    case 96: kernel(dk, 96)<<<grid, block, 0, st>>>(args); break;              \
+    default: kernel(dk, 128)<<<grid, block, 0, st>>>(args); break;             \
   }
-#define MHA_FWD(dp) mha_fwd_kernel<dp, false>
-#define MHA_THIN4(dp) mha_thin_kernel<dp, 4, false>
-#define MHA_THIN1(dp) mha_thin_kernel<dp, 1, false>
-#define MHA_FWD_GRAD(dp) mha_fwd_kernel<dp, true>
-#define MHA_THIN4_GRAD(dp) mha_thin_kernel<dp, 4, true>
-#define MHA_THIN1_GRAD(dp) mha_thin_kernel<dp, 1, true>
-#define MHA_BWD_Q(dp) mha_bwd_q_kernel<dp>
-#define MHA_BWD_KV(dp) mha_bwd_kv_kernel<dp>
-#define MHA_BWD_SMALL(dp) mha_bwd_small_kernel<dp>
+#define MHA_LAUNCH(dk, dv, kernel, grid, block, st, args)                      \
+  switch (dk) {                                                                \
+    case 32: MHA_LAUNCH_DV(32, dv, kernel, grid, block, st, args) break;       \
+    case 64: MHA_LAUNCH_DV(64, dv, kernel, grid, block, st, args) break;       \
+    case 96: MHA_LAUNCH_DV(96, dv, kernel, grid, block, st, args) break;       \
+    default: MHA_LAUNCH_DV(128, dv, kernel, grid, block, st, args) break;      \
+  }
+#define MHA_FWD(dk, dv) mha_fwd_kernel<dk, dv, false>
+#define MHA_THIN4(dk, dv) mha_thin_kernel<dk, dv, 4, false>
+#define MHA_THIN1(dk, dv) mha_thin_kernel<dk, dv, 1, false>
+#define MHA_FWD_GRAD(dk, dv) mha_fwd_kernel<dk, dv, true>
+#define MHA_THIN4_GRAD(dk, dv) mha_thin_kernel<dk, dv, 4, true>
+#define MHA_THIN1_GRAD(dk, dv) mha_thin_kernel<dk, dv, 1, true>
+#define MHA_BWD_Q(dk, dv) mha_bwd_q_kernel<dk, dv>
+// (96 with 128 would spill like 128 with 128 does without V in LDS: padded to it)
+#define MHA_BWD_KV(dk, dv) mha_bwd_kv_kernel<(dk + dv == 224 ? 128 : dk), (dk + dv == 224 ? 128 : dv)>
+#define MHA_BWD_SMALL(dk, dv) mha_bwd_small_kernel<dk, dv>
 
 extern "C" int cg_host_attention_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start,
                                       const int32_t* k_len, int sequences, int heads, int kv_heads, int causal,
@@ -1364,31 +1386,31 @@ extern "C" int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAtten
   a.ws_o = (float*)ws;
   a.ws_ml = a.ws_o + plan->parts * THIN_ROWS * (int64_t)in->Dv;
   const hipStream_t st = (hipStream_t)stream;
-  const int dp = mha_width(in->D, in->Dv);
+  const int dkp = mha_width(in->D), dvp = mha_width(in->Dv);
   if (plan->tiles) {
     a.items = mha_list(plan, data, 0);
     if (out_low) {
-      MHA_LAUNCH(dp, MHA_FWD_GRAD, plan->tiles, 256, st, a);
+      MHA_LAUNCH(dkp, dvp, MHA_FWD_GRAD, plan->tiles, 256, st, a);
     } else {
-      MHA_LAUNCH(dp, MHA_FWD, plan->tiles, 256, st, a);
+      MHA_LAUNCH(dkp, dvp, MHA_FWD, plan->tiles, 256, st, a);
     }
     CG_CHECK_LAUNCH(name);
   }
   if (plan->thin4) {
     a.items = mha_list(plan, data, 1);
     if (out_low) {
-      MHA_LAUNCH(dp, MHA_THIN4_GRAD, plan->thin4, 256, st, a);
+      MHA_LAUNCH(dkp, dvp, MHA_THIN4_GRAD, plan->thin4, 256, st, a);
     } else {
-      MHA_LAUNCH(dp, MHA_THIN4, plan->thin4, 256, st, a);
+      MHA_LAUNCH(dkp, dvp, MHA_THIN4, plan->thin4, 256, st, a);
     }
     CG_CHECK_LAUNCH(name);
   }
   if (plan->thin1) {
     a.items = mha_list(plan, data, 2);
     if (out_low) {
-      MHA_LAUNCH(dp, MHA_THIN1_GRAD, plan->thin1, 64, st, a);
+      MHA_LAUNCH(dkp, dvp, MHA_THIN1_GRAD, plan->thin1, 64, st, a);
     } else {
-      MHA_LAUNCH(dp, MHA_THIN1, plan->thin1, 64, st, a);
+      MHA_LAUNCH(dkp, dvp, MHA_THIN1, plan->thin1, 64, st, a);
     }
     CG_CHECK_LAUNCH(name);
   }
@@ -1438,10 +1460,10 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   a.delta = (float*)ws;
   if (ws) a.ws_o = (float*)((char*)ws + mha_delta_bytes(plan, in->q_rows));
   const hipStream_t st = (hipStream_t)stream;
-  const int dp = mha_width(in->D, in->Dv);
+  const int dkp = mha_width(in->D), dvp = mha_width(in->Dv);
   if (plan->dq_tiles) {
     a.items = mha_list(plan, data, 4);
-    MHA_LAUNCH(dp, MHA_BWD_Q, plan->dq_tiles, 256, st, a);
+    MHA_LAUNCH(dkp, dvp, MHA_BWD_Q, plan->dq_tiles, 256, st, a);
     CG_CHECK_LAUNCH(name);
   }
   if (plan->dq_joins) {
@@ -1451,7 +1473,7 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   }
   if (plan->dkv_tiles) {
     a.items = mha_list(plan, data, 6);
-    MHA_LAUNCH(dp, MHA_BWD_KV, plan->dkv_tiles, 256, st, a);
+    MHA_LAUNCH(dkp, dvp, MHA_BWD_KV, plan->dkv_tiles, 256, st, a);
     CG_CHECK_LAUNCH(name);
   }
   if (plan->dkv_joins) {
@@ -1461,7 +1483,7 @@ extern "C" int cg_packed_attention_bwd(const cgAttentionInput* in, const cgAtten
   }
   if (plan->small) {
     a.items = mha_list(plan, data, 8);
-    MHA_LAUNCH(dp, MHA_BWD_SMALL, plan->small, 64, st, a);
+    MHA_LAUNCH(dkp, dvp, MHA_BWD_SMALL, plan->small, 64, st, a);
     CG_CHECK_LAUNCH(name);
   }
   return CG_OK;

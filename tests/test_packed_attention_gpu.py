@@ -321,6 +321,18 @@ ATTENTION = [
     ([513], None, 2, 2, 104, 104, False),
     ([1000], [1100], 1, 1, 128, 128, True),
     ([7], [1900], 3, 1, 64, 64, True),
+    # key and value widths in every pair of the kernels' widths of 32, 64, 96 and 128
+    ([130, 17], None, 2, 1, 128, 32, True),
+    ([130, 17], None, 2, 1, 16, 128, True),
+    ([200], [150], 2, 2, 128, 96, False),
+    ([150], [200], 4, 1, 96, 128, True),
+    ([150, 3], None, 2, 1, 32, 64, True),
+    ([150, 3], None, 2, 1, 64, 32, False),
+    ([150, 65], None, 2, 1, 24, 80, True),
+    ([150, 65], None, 2, 1, 88, 24, True),
+    ([133, 20], None, 2, 1, 48, 96, True),
+    ([133, 20], None, 2, 1, 120, 48, False),
+    ([133, 20], None, 2, 1, 96, 88, True),
 ]
 
 
