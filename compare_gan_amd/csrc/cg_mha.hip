@@ -16,10 +16,10 @@
 //   element e of lane half h  <->  key 16 ks + 4 h + (e & 3) + 8 (e >> 2)
 // which the first operand matches by reading V transposed (ds_read_b64_tr_b16) at those keys.  P, dS and
 // all the sums never touch LDS.  Statistics and accumulators are fp32; P and dS are rounded to bf16 on their
-// way into the matrix instruction (half a step of 2^-9 relative each, independent errors over the sum).
+// way into the matrix instruction (at most half a step, 2^-8 relative, each; independent errors over the sum).
 //
 // LDS.  Tiles are copied by buffer_load ... lds (16 bytes a lane), two buffers: tile i + 1 is in flight while
-// tile i is multiplied, one barrier a tile.  Rows keep their pitch of 2 DP bytes; instead of padding, the
+// tile i is multiplied, one barrier a tile.  Rows keep their pitch of 2 DK or 2 DV bytes; instead of padding, the
 // 16-byte chunks of a row are exchanged by an XOR with bits of the row number (mha_swz) so that both the
 // b128 reads of K (32 rows, one chunk) and the transposed reads of V (8 rows, 4 chunks) spread over all banks.
 // Rows behind the end of a sequence and columns behind D are outside the buffer descriptor and arrive as zeros.
@@ -265,7 +265,7 @@ __device__ __forceinline__ void mha_accumulate_low(f32x16_t (&acc)[DP / 32], mha
                                                    const f32x16_t& p, int sub) {
   f32x16_t low;
 #pragma unroll
-  for (int v = 0; v < 16; ++v) low[v] = p[v] - bf2f(f2bf(p[v]));
+  for (int v = 0; v < 16; ++v) low[v] = p[v] - bf2f(f2bf(p[v]));    // (packed conversions: 34 spills, 938 -> 1092 us)
   mha_accumulate<DP>(acc, tile, m, low, sub);
 }
 constexpr int FEW = 64;
@@ -570,13 +570,52 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
   mha_store<DV, GRAD>(a, it, col, m, l, o, half);
 }
 
-// ---- joins the partial results of a split item; one wave a row, its parts' loads in flight together ------
-// item {seq, hk, row0, rows here, parts, first unit, units a part}
+// ---- joins the partial results of a split item ----------------------------------------------------
+// item {seq, hk, row0, rows here, parts, first unit, units a part}.  Of a tile (128 rows, few parts): a thread takes four
+// values of a row.  Of a thin item (at most 32 rows, up to hundreds of parts): a wave takes a row, its lanes the parts'
+// statistics, and the parts' loads are in flight together.  Bound by the bytes of the partial results.
 __global__ __launch_bounds__(256) void mha_join_kernel(MhaArgs a) {
   const MhaItem it = mha_item(a, blockIdx.x);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int parts = it.k1;
   const int64_t step = (int64_t)it.units * THIN_ROWS;
+  if (it.units > 1) {
+    const int quads = a.Dv / 4;
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < it.k0 * quads; i += gridDim.y * 256) {
+      const int n = i / quads, d = (i - n * quads) * 4;
+      const int64_t at = (int64_t)it.part * THIN_ROWS + n;
+      float top = -INFINITY;
+#pragma unroll 8
+      for (int p = 0; p < parts; ++p) top = fmaxf(top, a.ws_ml[(at + p * step) * 2]);
+      float total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int p = 0; p < parts; ++p) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + (at + p * step) * 2);
+        const float4 o = *reinterpret_cast<const float4*>(a.ws_o + (at + p * step) * a.Dv + d);
+        const float w = mha_weight(ml.x, top);
+        total += ml.y * w;
+        x[0] += o.x * w; x[1] += o.y * w; x[2] += o.z * w; x[3] += o.w * w;
+      }
+      int t, h;
+      mha_token(a, it, it.row0 + n, &t, &h);
+      const int64_t row = (int64_t)(it.q_start + t) * a.heads + h;
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] *= inv;
+      const uint2 packed = pack4_bf16(x);
+      *reinterpret_cast<uint2*>(a.out + row * a.Dv + d) = packed;
+      if (a.out_low) {
+        x[0] -= __uint_as_float(packed.x << 16);
+        x[1] -= __uint_as_float(packed.x & 0xffff0000u);
+        x[2] -= __uint_as_float(packed.y << 16);
+        x[3] -= __uint_as_float(packed.y & 0xffff0000u);
+        *reinterpret_cast<uint2*>(a.out_low + row * a.Dv + d) = pack4_bf16(x);
+      }
+      if (a.lse && d == 0)
+        a.lse[row] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * (1.f / LOG2E);
+    }
+    return;
+  }
   for (int i = blockIdx.y * 4 + wave; i < it.k0; i += gridDim.y * 4) {
     const int64_t at = (int64_t)it.part * THIN_ROWS + i;
     // one part a lane: the common exponent first
@@ -1132,16 +1171,18 @@ void mha_deal(std::vector<Work>* items, int units) {
 }
 
 // A launch's items are split along the axis that they sum over (keys; rows for dK and dV) where one item is longer
-// than its share of the launch.  A tile item's share is the total over 1024 (half of what one of the chip's 512 places,
-// 2 workgroups a CU, has to do: the longest items no longer delay the end; ragged batch of 25 k rows: dK / dV 330 us,
-// with the total over 512 402 us), but not below 1024 keys or rows where the total over 512 is more (a part's fp32
-// result, written once and read once, has to be small against its work; one sequence of 8192, 2 heads of 128, causal:
-// backward 206 us, in parts of 512 rows 231 us), and not below 512 at all.  Thin items are half as long: no tile of 128.
+// than its share of the launch.  A tile item's share is the total over 1536 (a third of what one of the chip's 512 places,
+// 2 workgroups a CU, has to do: the longest items no longer delay the end; ragged training batch of 25 k rows, all its
+// kernels: 790 us, over 1024 823 us, over 768 849 us, over 2048 794 us), but not below 1024 keys or rows where the total
+// over 512 is more (a part's fp32 result, written once and read once, has to be small against its work: 8 causal sequences
+// of 4096, 2 key heads of 128 with 4 query heads each, forward 294 us and over 2048 335 us; one sequence of 8192, 2 heads
+// of 128, causal: backward 206 us, in parts of 512 rows 231 us), and not below 512 at all.  Thin items have no tile of 128
+// rows and no part of 1024 keys to lose.
 constexpr int THIN1_KEYS = 128;     // up to so many keys one wave does a thin item alone
 
 int64_t mha_share(int64_t all, bool thin) {
-  const int64_t most = (all + 511) / 512, half = (all + 1023) / 1024;
-  return std::max<int64_t>(512, thin ? half : std::min(most, std::max<int64_t>(1024, half)));
+  const int64_t most = (all + 511) / 512, third = (all + 1535) / 1536;
+  return std::max<int64_t>(512, thin ? third : std::min(most, std::max<int64_t>(1024, third)));
 }
 
 void mha_split(std::vector<Work>* items, int step, int tile, int units_a_part, const std::vector<int64_t>& length,
@@ -1416,7 +1457,7 @@ extern "C" int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAtten
   }
   if (plan->joins) {
     a.items = mha_list(plan, data, 3);
-    mha_join_kernel<<<dim3(plan->joins, plan->tiles ? 32 : 1), 256, 0, st>>>(a);
+    mha_join_kernel<<<dim3(plan->joins, plan->tiles ? 8 : 1), 256, 0, st>>>(a);
     CG_CHECK_LAUNCH(name);
   }
   return CG_OK;

@@ -364,6 +364,7 @@ def test_split_over_keys_with_many_rows(K, Fn):
   """Few tiles of 128 rows against many keys: partial results joined; with gradients."""
   run_attention(K, Fn, [70], [5000], 2, 1, 64, 64, True, True)
   run_attention(K, Fn, [300, 3], [3000, 2000], 1, 1, 128, 96, False, True)
+  run_attention(K, Fn, [16], [40000], 4, 1, 72, 40, True, True)       # tens of parts a tile
 
 
 @pytest.mark.parametrize("spread", [0.0, 8.0])
