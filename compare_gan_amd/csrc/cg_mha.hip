@@ -571,90 +571,72 @@ __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
 }
 
 // ---- joins the partial results of a split item ----------------------------------------------------
-// item {seq, hk, row0, rows here, parts, first unit, units a part}.  Of a tile (128 rows, few parts): a thread takes four
-// values of a row.  Of a thin item (at most 32 rows, up to hundreds of parts): a wave takes a row, its lanes the parts'
-// statistics, and the parts' loads are in flight together.  Bound by the bytes of the partial results.
+// item {seq, hk, row0, rows here, parts, first unit, units a part}.  A block's rows, four values a thread; where they are
+// less than 256 threads the parts are dealt to groups of threads as well, and the groups' results joined through LDS in
+// their order: a few rows with hundreds of parts are a few loads behind one another.  Bound by the partial results' bytes.
 __global__ __launch_bounds__(256) void mha_join_kernel(MhaArgs a) {
+  __shared__ float box[6][256];
   const MhaItem it = mha_item(a, blockIdx.x);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int parts = it.k1;
+  const int parts = it.k1, quads = a.Dv / 4;
   const int64_t step = (int64_t)it.units * THIN_ROWS;
-  if (it.units > 1) {
-    const int quads = a.Dv / 4;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < it.k0 * quads; i += gridDim.y * 256) {
-      const int n = i / quads, d = (i - n * quads) * 4;
-      const int64_t at = (int64_t)it.part * THIN_ROWS + n;
-      float top = -INFINITY;
+  const int share = (it.k0 + gridDim.y - 1) / gridDim.y, first = blockIdx.y * share;
+  const int units = min(share, it.k0 - first) * quads;
+  if (units <= 0) return;
+  const int groups = units < 256 ? 256 / units : 1;
+  const int group = groups > 1 ? threadIdx.x / units : 0;
+  for (int u = threadIdx.x - group * units; u < units; u += 256) {
+    const int i = u / quads, d = (u - i * quads) * 4, n = first + i;
+    const int64_t at = (int64_t)it.part * THIN_ROWS + n;
+    float top = -INFINITY, total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (group < groups) {
 #pragma unroll 8
-      for (int p = 0; p < parts; ++p) top = fmaxf(top, a.ws_ml[(at + p * step) * 2]);
-      float total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int p = group; p < parts; p += groups) top = fmaxf(top, a.ws_ml[(at + p * step) * 2]);
 #pragma unroll 4
-      for (int p = 0; p < parts; ++p) {
+      for (int p = group; p < parts; p += groups) {
         const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + (at + p * step) * 2);
         const float4 o = *reinterpret_cast<const float4*>(a.ws_o + (at + p * step) * a.Dv + d);
         const float w = mha_weight(ml.x, top);
         total += ml.y * w;
         x[0] += o.x * w; x[1] += o.y * w; x[2] += o.z * w; x[3] += o.w * w;
       }
-      int t, h;
-      mha_token(a, it, it.row0 + n, &t, &h);
-      const int64_t row = (int64_t)(it.q_start + t) * a.heads + h;
-      const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] *= inv;
-      const uint2 packed = pack4_bf16(x);
-      *reinterpret_cast<uint2*>(a.out + row * a.Dv + d) = packed;
-      if (a.out_low) {
-        x[0] -= __uint_as_float(packed.x << 16);
-        x[1] -= __uint_as_float(packed.x & 0xffff0000u);
-        x[2] -= __uint_as_float(packed.y << 16);
-        x[3] -= __uint_as_float(packed.y & 0xffff0000u);
-        *reinterpret_cast<uint2*>(a.out_low + row * a.Dv + d) = pack4_bf16(x);
-      }
-      if (a.lse && d == 0)
-        a.lse[row] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * (1.f / LOG2E);
     }
-    return;
-  }
-  for (int i = blockIdx.y * 4 + wave; i < it.k0; i += gridDim.y * 4) {
-    const int64_t at = (int64_t)it.part * THIN_ROWS + i;
-    // one part a lane: the common exponent first
-    float top = -INFINITY;
-    for (int p = lane; p < parts; p += 64) top = fmaxf(top, a.ws_ml[(at + p * step) * 2]);
+    if (groups > 1) {          // (the same for all of the block, and its threads are here once)
+      box[0][threadIdx.x] = top;
+      box[1][threadIdx.x] = total;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    float total = 0.f, acc[2] = {0.f, 0.f};
-    for (int p0 = 0; p0 < parts; p0 += 64) {
-      float w = 0.f, l = 0.f;
-      if (p0 + lane < parts) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + (at + (p0 + lane) * step) * 2);
-        w = mha_weight(ml.x, top);
-        l = ml.y * w;
-      }
-      total += wave_sum(l);
-      const int n = min(64, parts - p0);
-      const float* src = a.ws_o + (at + p0 * step) * a.Dv;
-#pragma unroll 4
-      for (int p = 0; p < n; ++p) {
-        const float wp = __shfl(w, p, 64);
+      for (int j = 0; j < 4; ++j) box[2 + j][threadIdx.x] = x[j];
+      __syncthreads();
+      if (group > 0) return;
+      float all = top;
+      for (int g = 1; g < groups; ++g) all = fmaxf(all, box[0][g * units + u]);
+      const float mine = mha_weight(top, all);
+      total *= mine;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (lane + 64 * j < a.Dv) acc[j] += src[p * step * a.Dv + lane + 64 * j] * wp;
+      for (int j = 0; j < 4; ++j) x[j] *= mine;
+      for (int g = 1; g < groups; ++g) {
+        const float w = mha_weight(box[0][g * units + u], all);
+        total += box[1][g * units + u] * w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += box[2 + j][g * units + u] * w;
       }
+      top = all;
     }
     int t, h;
-    mha_token(a, it, it.row0 + i, &t, &h);
+    mha_token(a, it, it.row0 + n, &t, &h);
     const int64_t row = (int64_t)(it.q_start + t) * a.heads + h;
     const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (lane + 64 * j < a.Dv) {
-        const float x = acc[j] * inv;
-        const bf16_t hi = f2bf(x);
-        a.out[row * a.Dv + lane + 64 * j] = hi;
-        if (a.out_low) a.out_low[row * a.Dv + lane + 64 * j] = f2bf(x - bf2f(hi));
-      }
-    if (a.lse && lane == 0)
+    for (int j = 0; j < 4; ++j) x[j] *= inv;
+    const uint2 hi = pack4_bf16(x);
+    *reinterpret_cast<uint2*>(a.out + row * a.Dv + d) = hi;
+    if (a.out_low) {
+      x[0] -= __uint_as_float(hi.x << 16);
+      x[1] -= __uint_as_float(hi.x & 0xffff0000u);
+      x[2] -= __uint_as_float(hi.y << 16);
+      x[3] -= __uint_as_float(hi.y & 0xffff0000u);
+      *reinterpret_cast<uint2*>(a.out_low + row * a.Dv + d) = pack4_bf16(x);
+    }
+    if (a.lse && d == 0)
       a.lse[row] = total == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * (1.f / LOG2E);
   }
 }
@@ -963,6 +945,7 @@ __global__ __launch_bounds__(256) void mha_join_grad_kernel(MhaArgs a) {
     const int n = i / quads, d = (i - n * quads) * 4;
     const float* src = a.ws_o + ((int64_t)it.part * ROW_TILE + n) * width + d;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int p = 0; p < it.k1; ++p) {
       const float4 x = *reinterpret_cast<const float4*>(src + p * step);
       sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
@@ -1457,7 +1440,9 @@ extern "C" int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAtten
   }
   if (plan->joins) {
     a.items = mha_list(plan, data, 3);
-    mha_join_kernel<<<dim3(plan->joins, plan->tiles ? 8 : 1), 256, 0, st>>>(a);
+    // a thousand blocks and more (few items: fewer rows a block), at most one for each row of an item
+    const int each = std::min(plan->tiles ? ROW_TILE : THIN_ROWS, std::max(plan->tiles ? 8 : 1, 1024 / plan->joins));
+    mha_join_kernel<<<dim3(plan->joins, each), 256, 0, st>>>(a);
     CG_CHECK_LAUNCH(name);
   }
   return CG_OK;

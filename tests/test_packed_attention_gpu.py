@@ -348,6 +348,8 @@ NEW_TOKENS = [
     ([20000], 8, 8, 128, 128, 20000),
     ([9001, 3], 12, 4, 96, 32, 9001),
     ([70000], 1, 1, 32, 32, 70000),
+    ([131072], 2, 2, 128, 8, 131072),               # hundreds of parts for one row
+    ([60000, 9], 9, 3, 16, 40, 60001),
     ([3001], 66, 2, 64, 64, 3001),                  # 33 shared heads: more than one wave's rows
 ]
 
