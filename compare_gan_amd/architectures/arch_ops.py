@@ -898,7 +898,8 @@ def multi_head_block(x, name, use_sn, num_heads=None, num_kv_heads=None, head_wi
   half of a head's pairs) and column (second half), every query seeing every position of its image.
 
   num_heads: query heads of head_width entries (default: as many as fill the channels, at least one);
-  num_kv_heads: key / value heads they share (default: one each)."""
+  num_kv_heads: key / value heads they share (default: one each).
+  First derivatives only, like the single-head block."""
   n, h, w, c = x.shape
   heads = max(1, c // head_width) if num_heads is None else int(num_heads)
   kv_heads = heads if num_kv_heads is None else int(num_kv_heads)

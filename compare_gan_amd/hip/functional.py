@@ -1085,7 +1085,7 @@ class PackedAttentionFn(torch.autograd.Function):
 def packed_attention(q, k, v, plan, scale=None):
   """softmax(scale q k^T) v over the sequences of a K.AttentionPlan (q [rows, heads, D], k [rows, kv_heads, D],
   v [rows, kv_heads, Dv], bf16); differentiable in q, k and v.  Rows outside every sequence give zeros and
-  get zero gradients."""
+  get zero gradients.  First derivatives only."""
   return PackedAttentionFn.apply(q, k, v, plan, scale)
 
 
