@@ -378,7 +378,7 @@ __device__ __forceinline__ void mha_store(const MhaArgs& a, const MhaItem& it, i
 
 // ---- forward, 128 rows x all keys of the item ---------------------------------------------------
 // Measured: 64 x 4096 tokens, 3 heads of 64, 950 us (870 TFLOP/s); 16 384 tokens causal, 16 heads of 128 on 4 key heads,
-// 1.05 ms (1.05 PFLOP/s counted without the masked half); ragged causal batch, 8 heads of 96 on 2, 190 us (620 TFLOP/s:
+// 1.05 ms (1.05 PFLOP/s counted without the masked half); ragged causal batch, 8 heads of 96 on 2, 170 to 190 us (620 to 690 TFLOP/s:
 // diagonals and the end of the launch).
 template <int DK, int DV, bool GRAD>
 __global__ __launch_bounds__(256, mha_wider(DK, DV) <= 64 ? 4 : mha_wider(DK, DV) <= 96 ? 3 : 2) void mha_fwd_kernel(MhaArgs a) {
