@@ -1220,9 +1220,23 @@ void mha_split(std::vector<Work>* items, int step, int tile, int units_a_part, c
   items->swap(out);
 }
 
+// Up to so many items of a one wave form (one a CU) go into the launch of a wider form if there is one anyway: they fill
+// its end, and a launch of their own is 7 to 10 us (48 new tokens, a few of them with up to 128 keys: 177 -> 168 us;
+// ragged training batch: 793 -> 776 us; two causal sequences of 2048 with 32, 128 or 256 one wave units beside them:
+// forward 41, 39, 39 -> 34, 32, 32 us, backward 88, 83, 83 -> 80, 76, 74 us).
+constexpr int FOLD = 256;
+
 int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_start, const int32_t* k_len,
              int B, int heads, int kv_heads, int causal, int32_t* data, int64_t capacity, cgAttentionPlan* info) {
   const int G = heads / kv_heads;
+  int64_t few = 0;           // units for the small form of the backward pass, and whether there are others
+  bool others = false;
+  for (int b = 0; b < B; ++b) {
+    const bool fits = (int64_t)q_len[b] * G <= 32 && k_len[b] <= 32;
+    if (!fits) others = true;
+    else if (q_len[b] > 0 || k_len[b] > 0) few += kv_heads;
+  }
+  const bool small_form = !others || few > FOLD;
   std::vector<Work> tiles, thin4, thin1, joins, dq, dq_joins, dkv, dkv_joins, small;
   std::vector<int64_t> all_rows(B), all_keys(B);
   cgAttentionPlan p = {};
@@ -1241,11 +1255,11 @@ int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_star
       for (int64_t r = 0; r < rows; r += ROW_TILE) {
         const int64_t keys = keys_of(std::min(rows, r + ROW_TILE));
         Work w = {{b, h, (int32_t)r, 0, (int32_t)keys, -1, 0, 0}, keys + 64, unit};
-        if (rows > 32 || Lk > 32) dq.push_back(w);
+        if (rows > 32 || Lk > 32 || !small_form) dq.push_back(w);
         if (rows > THIN_ROWS) tiles.push_back(w);
         else (keys <= THIN1_KEYS ? thin1 : thin4).push_back(w);
       }
-      if (rows <= 32 && Lk <= 32) {
+      if (rows <= 32 && Lk <= 32 && small_form) {
         if (rows > 0 || Lk > 0) small.push_back(Work{{b, h, 0, 0, (int32_t)Lk, -1, 0, 0}, 1, unit});
         continue;
       }
@@ -1254,6 +1268,11 @@ int mha_plan(const int32_t* q_start, const int32_t* q_len, const int32_t* k_star
         dkv.push_back(Work{{b, h, (int32_t)k, (int32_t)from, (int32_t)rows, -1, 0, 0}, rows - from + 64, unit});
       }
     }
+  }
+  if ((int64_t)thin1.size() <= FOLD && (!thin4.empty() || !tiles.empty())) {
+    std::vector<Work>& wider = thin4.empty() ? tiles : thin4;
+    wider.insert(wider.end(), thin1.begin(), thin1.end());
+    thin1.clear();
   }
   int64_t parts = 0, dq_parts = 0, dkv_parts = 0;
   mha_split(&tiles, KT, ROW_TILE, ROW_TILE / 32, all_rows, &joins, &parts);

@@ -75,6 +75,9 @@ PLANS = [
     ("few rows, many keys", [200], [70001], 2, 1, False, None),
     ("queries in front of the keys", [100, 40], [30, 0], 4, 4, True, None),
     ("odd heads", [33, 65, 31], [64, 1, 300], 15, 3, True, 512),
+    ("few small beside large", [3] * 128 + [200], None, 2, 2, True, None),
+    ("many small beside large", [3] * 129 + [200, 0], None, 2, 2, True, None),
+    ("many new tokens, few long", [1] * 300, [5] * 299 + [900], 4, 1, True, 1000),
     ("one row a head, 40 shared", [1], [3000], 40, 1, False, None),
 ]
 
@@ -98,13 +101,16 @@ def test_plan_covers_every_row_and_key_once(case):
   for name, tile, step in (("tiles", 128, 64), ("thin4", 32, 32), ("thin1", 32, 32)):
     for b, h, row0, k0, k1, part, _, _ in p[name].tolist():
       rows = q[b] * g
-      assert 0 <= h < kv_heads and row0 % tile == 0 and row0 < rows and (rows > 32) == (name == "tiles")
+      assert 0 <= h < kv_heads and row0 % tile == 0 and row0 < rows
+      # few rows and keys: in a form of their own only where they are many or alone
+      assert (rows > 32) == (name == "tiles") or (name == "tiles" and k1 <= 128 and part < 0)
       assert 0 <= k0 <= k1 <= kk[b] and k0 % step == 0
       pieces.setdefault((b, h, row0), []).append((k0, k1, part))
       if part >= 0:
         units = tile // 32
         assert not used & set(range(part, part + units))
         used |= set(range(part, part + units))
+  assert len(p["thin1"]) == 0 or len(p["thin1"]) > 256 or not len(p["thin4"]) + len(p["tiles"])
   assert len(used) == plan.info.parts and (not used or max(used) == plan.info.parts - 1)
   joins = {(b, h, r): (n, parts, unit, units) for b, h, r, n, parts, unit, units, _ in p["joins"].tolist()}
   for b, n in enumerate(q):
@@ -124,7 +130,9 @@ def test_plan_covers_every_row_and_key_once(case):
   assert not pieces and not joins
   # gradients: sequences that fit one wave as a whole, the others in tiles whose parts follow one another
   alone = sorted((b, h) for b, h, _, _, k1, _, _, _ in p["small"].tolist())
-  fits = lambda b: q[b] * g <= 32 and kk[b] <= 32
+  one_wave = [q[b] * g <= 32 and kk[b] <= 32 for b in range(len(q))]
+  own_form = all(one_wave) or kv_heads * sum(f and q[b] + kk[b] > 0 for b, f in enumerate(one_wave)) > 256
+  fits = lambda b: own_form and one_wave[b]
   assert alone == sorted((b, h) for b in range(len(q)) for h in range(kv_heads) if fits(b) and (q[b] or kk[b]))
   want_q, want_k = {}, {}
   for b in range(len(q)):

@@ -321,6 +321,10 @@ ATTENTION = [
     ([513], None, 2, 2, 104, 104, False),
     ([1000], [1100], 1, 1, 128, 128, True),
     ([7], [1900], 3, 1, 64, 64, True),
+    # small sequences beside large ones: in the large ones' launches, and (many) in their own
+    ([3, 200, 1, 0, 17, 32, 8], None, 2, 2, 64, 64, True),
+    ([1, 4, 150, 2], [30, 0, 150, 7], 4, 1, 48, 64, True),
+    ([7] * 90 + [140], None, 3, 3, 32, 40, False),
     # key and value widths in every pair of the kernels' widths of 32, 64, 96 and 128
     ([130, 17], None, 2, 1, 128, 32, True),
     ([130, 17], None, 2, 1, 16, 128, True),
@@ -348,6 +352,8 @@ NEW_TOKENS = [
     ([20000], 8, 8, 128, 128, 20000),
     ([9001, 3], 12, 4, 96, 32, 9001),
     ([70000], 1, 1, 32, 32, 70000),
+    ([5, 2000, 0, 128, 40, 129, 1], 8, 2, 64, 96, 2000),
+    ([3] * 299 + [900], 4, 1, 64, 64, 1000),
     ([131072], 2, 2, 128, 8, 131072),               # hundreds of parts for one row
     ([60000, 9], 9, 3, 16, 40, 60001),
     ([3001], 66, 2, 64, 64, 3001),                  # 33 shared heads: more than one wave's rows
