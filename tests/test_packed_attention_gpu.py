@@ -566,6 +566,41 @@ def test_new_token_with_values_that_are_not_finite_behind_it(K, Fn):
   assert torch.equal(got[:3], clean[:3]) and not torch.isfinite(got[3:].float()).any(-1).any()
 
 
+def test_rows_beyond_32_bits(K, Fn):
+  """Keys, values and tokens whose offsets pass 2^31 elements: the results of the same rows at the front, to the bit."""
+  far, lens = 17_000_000, [300, 70, 1]                     # x 128 entries: 2.2e9
+  gen = torch.Generator().manual_seed(12)
+  n = sum(lens)
+  q, dout = (normal(gen, (n, 2, 128)).cuda() for _ in range(2))
+  near = [normal(gen, (n, 1, 128)).cuda() for _ in range(2)]
+  starts = [0, far - 80, far - 1]
+  big = [torch.empty((far, 1, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+  at = 0
+  for s, m in zip(starts, lens):
+    for b, x in zip(big, near):
+      b[s:s + m] = x[at:at + m]
+    at += m
+  plans = [K.AttentionPlan(lens, heads=2, kv_heads=1, causal=True, k_starts=x, device="cuda") for x in (None, starts)]
+  results = []
+  for plan, (k, v) in zip(plans, (near, big)):
+    out, saved = K.packed_attention_fwd(q, k, v, plan)
+    dq, dk, dv = K.packed_attention_bwd(q, k, v, plan, out, saved, dout)
+    if k is big[0]:
+      dk, dv = (torch.cat([x[s:s + m] for s, m in zip(starts, lens)]) for x in (dk, dv))
+    results.append((out, dq, dk, dv))
+  for a, b in zip(*results):
+    assert torch.equal(a, b)
+  # one new token whose cache lies behind 2^31, and a rotation of far rows
+  new = K.AttentionPlan([1, 1, 1], lens, heads=2, kv_heads=1, causal=True)
+  there = K.AttentionPlan([1, 1, 1], lens, heads=2, kv_heads=1, causal=True, k_starts=starts)
+  assert torch.equal(K.packed_attention_fwd(q[:3], *near, new, want_grad=False)[0],
+                     K.packed_attention_fwd(q[:3], *big, there, want_grad=False)[0])
+  table, pos = K.RotaryTable(128), torch.arange(100, dtype=torch.int32, device="cuda")
+  rows = big[0][::170_000]
+  rows.copy_(q[:100, :1])
+  assert torch.equal(K.rotary(rows, pos, table), K.rotary(q[:100, :1].contiguous(), pos, table))
+
+
 def test_same_result_every_time(K, Fn):
   """No atomics: two runs agree to the bit, alone and with another stream's call in between."""
   gen = torch.Generator().manual_seed(8)
