@@ -42,7 +42,7 @@ struct RopeArgs {
   const double* freq;
   float* partial;    // [blocks][2][D] gain gradients
   float amplitude, eps, inv_d, sign;
-  int T, D, rot, pairs, slots, per_axis, axes, interleaved;   // slots: pairs + identities behind them
+  int T, D, rot, pairs, slots, per_axis, axes, interleaved;   // slots: pairs of whole units
   int tb, lanes, lanes_log, units, pair_units, chunks;
   FastDiv dslots, dper;
 };
@@ -116,8 +116,10 @@ __device__ __forceinline__ float2 turn_cos_sin(float turns) {
 // CU, so that the angles of one are formed while others move data
 constexpr int ROPE_LDS_FLOATS = 4096;
 
-// UPL: units (2 VP elements) a lane holds
-template <typename T, int VP, int UPL, bool NORM, bool BWD>
+// UPL: units (2 VP elements) a lane holds.  PART: the last pairs of a unit are copied entries, which stay as they are
+// (turned by the identity, 0 times an infinite neighbour would be NaN); a form of its own, since choosing costs every
+// unit of the others something: 262 144 tokens x 3 heads of 64, 36 us in place of 33 behind itself
+template <typename T, int VP, int UPL, bool NORM, bool BWD, bool PART>
 __global__ __launch_bounds__(256, NORM && VP == 8 ? 3 : BWD ? 4 : 6) void rope_kernel(RopeArgs a) {
   __shared__ __attribute__((aligned(16))) float lds[ROPE_LDS_FLOATS];
   float2* cs = reinterpret_cast<float2*>(lds);
@@ -154,10 +156,7 @@ __global__ __launch_bounds__(256, NORM && VP == 8 ? 3 : BWD ? 4 : 6) void rope_k
     __syncthreads();      // the previous chunk's angles are no longer read
     for (int i = threadIdx.x; i < nt * a.slots; i += 256) {
       const int tok = fdiv(i, a.dslots), pair = i - tok * a.slots;
-      if (pair >= a.pairs) {
-        cs[i] = make_float2(1.f, 0.f);
-        continue;
-      }
+      if (PART && pair >= a.pairs) continue;        // (read below and not used)
       const int axis = fdiv(pair, a.dper);
       const double turns = (double)a.positions[(int64_t)(t0 + tok) * a.axes + axis] * a.freq[pair];
       const float2 v = turn_cos_sin<T>((float)(turns - rint(turns)));
@@ -222,8 +221,9 @@ __global__ __launch_bounds__(256, NORM && VP == 8 ? 3 : BWD ? 4 : 6) void rope_k
             for (int j = 0; j < VP; ++j) {
               const float2 q = c[j];
               const float p0 = w[u * 2 * VP + j], p1 = w[u * 2 * VP + VP + j];
-              w[u * 2 * VP + j] = p0 * q.x - p1 * q.y;
-              w[u * 2 * VP + VP + j] = p0 * q.y + p1 * q.x;
+              const bool in = !PART || cs_at[u] + j < a.pairs;
+              w[u * 2 * VP + j] = in ? p0 * q.x - p1 * q.y : p0;
+              w[u * 2 * VP + VP + j] = in ? p0 * q.y + p1 * q.x : p1;
             }
           }
         };
@@ -373,8 +373,8 @@ int rope_plan(RopeArgs* a, const cgRotation* rot, int T, int D, int esize, bool 
   // two waves a SIMD (65 536 tokens, 12 heads of 32: 51 us, with 8 elements 38)
   int vp = bwd || esize == 4 ? 4 : 8;
   for (; vp > 1; vp >>= 1) {
-    // interleaved pairs lie one behind the other: a unit may hold the last pairs and the first copied entries (turned
-    // by the identity); with halves the two parts of a unit have to end together
+    // interleaved pairs lie one behind the other: a unit may hold the last pairs and the first copied entries; with
+    // halves the two parts of a unit have to end together
     bool ok = D % (2 * vp) == 0 && (a->interleaved || (a->pairs % vp == 0 && (D - a->rot) % (2 * vp) == 0));
     for (int s = 0; s < a->ntensors; ++s)
       ok = ok && aligned_for(a->t[s].x, a->t[s].st, a->t[s].sh, vp, esize) &&
@@ -408,18 +408,26 @@ int rope_plan(RopeArgs* a, const cgRotation* rot, int T, int D, int esize, bool 
   return vp;
 }
 
-template <typename T, bool NORM, bool BWD>
-void rope_launch(const RopeArgs& a, int vp, int grid, hipStream_t st) {
-  if constexpr (sizeof(T) == 2 && !BWD) {
-    if (vp == 8) {
-      rope_kernel<T, 8, 1, NORM, BWD><<<grid, 256, 0, st>>>(a);
+template <typename T, int VP, int UPL, bool NORM, bool BWD>
+void rope_launch_form(const RopeArgs& a, int grid, hipStream_t st) {
+  if constexpr (VP > 1) {
+    if (a.slots != a.pairs) {
+      rope_kernel<T, VP, UPL, NORM, BWD, true><<<grid, 256, 0, st>>>(a);
       return;
     }
   }
+  rope_kernel<T, VP, UPL, NORM, BWD, false><<<grid, 256, 0, st>>>(a);
+}
+
+template <typename T, bool NORM, bool BWD>
+void rope_launch(const RopeArgs& a, int vp, int grid, hipStream_t st) {
+  if constexpr (sizeof(T) == 2 && !BWD) {
+    if (vp == 8) return rope_launch_form<T, 8, 1, NORM, BWD>(a, grid, st);
+  }
   switch (vp) {
-    case 4: rope_kernel<T, 4, 1, NORM, BWD><<<grid, 256, 0, st>>>(a); break;
-    case 2: rope_kernel<T, 2, 1, NORM, BWD><<<grid, 256, 0, st>>>(a); break;
-    default: rope_kernel<T, 1, 2, NORM, BWD><<<grid, 256, 0, st>>>(a); break;
+    case 4: return rope_launch_form<T, 4, 1, NORM, BWD>(a, grid, st);
+    case 2: return rope_launch_form<T, 2, 1, NORM, BWD>(a, grid, st);
+    default: return rope_launch_form<T, 1, 2, NORM, BWD>(a, grid, st);
   }
 }
 

@@ -767,3 +767,65 @@ def test_captured_and_replayed(K, Fn):
     torch.cuda.synchronize()
     for x, y in zip(held, want):
       assert torch.equal(x, y), i
+
+
+# ------------------------------------------------------------------------------------------------
+# entries behind the turned part
+# ------------------------------------------------------------------------------------------------
+# D, rot: the last turned pairs and the first copied entries share a load of 8, 4 (twice) or 2 pairs, or none
+BEHIND = [(32, 20), (72, 36), (24, 14), (20, 14), (18, 10), (64, 32)]
+
+
+def same_bits(a, b):
+  word = {2: torch.int16, 4: torch.int32}[a.element_size()]
+  return torch.equal(a.contiguous().view(word), b.contiguous().view(word))
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,rot", BEHIND)
+def test_entries_behind_the_turned_part_are_copied(K, Fn, d, rot, dtype, layout):
+  """To the bit, whatever lies beside them (infinities, NaN, zeros of either sign), and the turned part does not notice."""
+  gen = torch.Generator().manual_seed(d)
+  table, pos = K.RotaryTable(rot, layout=layout), positions_of(gen, 9, 1, 1000)
+  clean = normal(gen, (9, 3, d), dtype).cuda()
+  want = K.rotary(clean, pos, table)
+  for poison in (float("inf"), float("-inf"), float("nan"), 0.0, -0.0):
+    for at in range(rot, min(rot + 8, d)):
+      x = clean.clone()
+      x[::2, 1:, at] = poison
+      for inverse in (False, True):
+        y = K.rotary(x, pos, table, inverse=inverse)
+        assert same_bits(y[..., rot:], x[..., rot:]), (poison, at)
+        if not inverse:
+          assert same_bits(y[..., :rot], want[..., :rot]), (poison, at)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,rot", BEHIND)
+def test_norm_beside_copied_entries_that_are_not_finite(K, Fn, d, rot, dtype):
+  """An infinite copied entry makes the head's norm infinite: it becomes NaN and the others 0, as the formula has it.  An
+  infinite incoming gradient of a copied entry reaches its own row and its own gain, no other."""
+  gen = torch.Generator().manual_seed(d + 1)
+  table, pos = K.RotaryTable(rot, layout="interleaved"), positions_of(gen, 9, 1, 1000)
+  q, k = normal(gen, (9, 3, d), dtype).cuda(), normal(gen, (9, 1, d), dtype).cuda()
+  gain = torch.ones(d, device="cuda")
+  dq, dk = normal(gen, q.shape, dtype).cuda(), normal(gen, k.shape, dtype).cuda()
+  clean = K.qk_norm_rotary(q, k, gain, gain, pos, table)
+  grads = K.qk_norm_rotary_bwd(q, k, gain, gain, pos, table, dq, dk)
+  for at in range(rot, min(rot + 8, d)):
+    x = q.clone()
+    x[4, 1, at] = float("inf")
+    y = K.qk_norm_rotary(x, k, gain, gain, pos, table)[0]
+    want = clean[0].clone()
+    want[4, 1] = 0.0
+    assert y[4, 1, at].isnan()
+    y[4, 1, at] = 0.0
+    assert torch.equal(y, want), at
+    dy = dq.clone()
+    dy[4, 1, at] = float("inf")
+    got = K.qk_norm_rotary_bwd(q, k, gain, gain, pos, table, dy, dk)
+    rest = torch.arange(d, device="cuda") != at
+    assert torch.equal(got[2][rest], grads[2][rest]) and not torch.isfinite(got[2][at]), at
+    got[0][4, 1], grads[0][4, 1] = 0.0, 0.0
+    assert torch.equal(got[0], grads[0]) and torch.equal(got[1], grads[1]) and torch.equal(got[3], grads[3])
