@@ -342,6 +342,7 @@ bool aligned_for(const void* p, int64_t st, int64_t sh, int vp, int esize) {
 int rope_check(const char* name, const cgHeadRows* x, int T, int D, int dtype) {
   if (!x || (!x->x && T != 0)) CG_FAIL(CG_ERR_BAD_ARG, "%s: null tensor", name);
   if (x->heads < 1 || T < 0 || D < 2) CG_FAIL(CG_ERR_BAD_ARG, "%s: bad sizes T=%d heads=%d D=%d", name, T, x->heads, D);
+  if (x->heads > 0x3fffffff) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: %d heads (at most 2^30 - 1)", name, x->heads);
   if (x->stride_t < 0 || x->stride_h < 0) CG_FAIL(CG_ERR_BAD_ARG, "%s: negative strides", name);
   if (D % 2 || D > 256) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: head width %d (even, at most 256)", name, D);
   if (dtype != 0 && dtype != 1) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: dtype %d (0 bf16, 1 fp32)", name, dtype);

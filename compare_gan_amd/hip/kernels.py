@@ -1089,6 +1089,7 @@ def attention_bwd(theta, phi, g, out, lse, dout):
 # multi-head attention on packed rows
 # ------------------------------------------------------------------------------------------------
 HEAD_TYPES = {BF16: 0, F32: 1}
+MOST_ROWS, MOST_HEADS = 2 ** 31 - 1, 2 ** 30 - 1
 # cgHeadRows, cgRotation and cgAttentionInput as bytes (native layout): these calls may last a few
 # microseconds, which a ctypes structure's construction is not small against
 _HEAD_ROWS = struct.Struct("@PqqiP0q")
@@ -1181,6 +1182,8 @@ def _req_heads(t, name, like=None):
         raise ValueError("%s must be a tensor on the GPU (no CPU fallback exists)" % name)
     if t.dim() != 3:
         raise ValueError("%s must be [rows, heads, width], got %d dimensions" % (name, t.dim()))
+    if t.shape[0] > MOST_ROWS or t.shape[1] > MOST_HEADS:      # (ctypes would wrap what is more than 32 bits)
+        raise ValueError("%s: at most %d rows and %d heads, got %s" % (name, MOST_ROWS, MOST_HEADS, list(t.shape)))
     if like is not None:
         if t.get_device() != like.get_device():
             raise ValueError("%s is on %s, the other tensors on %s" % (name, t.device, like.device))

@@ -575,7 +575,7 @@ typedef struct {
   float amplitude;
   int32_t axes, rot, interleaved;
 } cgRotation;
-/* dtype 0: bf16, 1: fp32.  D even, at most 256.  y [T, heads, D] contiguous.  inverse != 0: the adjoint
+/* dtype 0: bf16, 1: fp32.  D even, at most 256; fewer than 2^30 heads.  y [T, heads, D] contiguous.  inverse != 0: the adjoint
  * (turns by -angle).  x->gain is not used. */
 int cg_rotary(const cgHeadRows* x, int T, int D, int dtype, const cgRotation* rot, int inverse, void* y,
               cgStream stream);

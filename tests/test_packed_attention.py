@@ -266,3 +266,40 @@ def test_packed_structures_have_the_declared_layout():
   assert raw.amplitude == pytest.approx(table.amplitude, rel=1e-7)
   raw = _lib.AttentionInput.from_buffer_copy(K._attention_packed(rows, rows[:2], rows[:1], 0.5))
   assert [getattr(raw, n) for n, _ in raw._fields_] == [rows.data_ptr()] * 3 + [40, 16, 40, 16, 0, 16, 3, 2, 8, 8, 0.5]
+
+
+class _OnTheGpu(torch.Tensor):
+  """A tensor without memory that the checks take for one on the GPU."""
+  is_cuda = property(lambda self: True)
+
+  def get_device(self):
+    return 0
+
+
+def _shape_only(shape, dtype=torch.bfloat16):
+  return torch.empty(shape, dtype=dtype, device="meta").as_subclass(_OnTheGpu)
+
+
+def test_rows_and_heads_beyond_32_bits_are_refused(monkeypatch):
+  """Before anything is allocated or called: 2^32 rows would arrive as none, 2^32 + 5 as 5."""
+  def called(*_):
+    raise AssertionError("reached the library")
+  monkeypatch.setattr(K, "_launch", called)
+  table = K.RotaryTable(2, device="cpu")
+  table.index = 0
+  for rows, heads in ((2 ** 31, 1), (2 ** 32, 1), (2 ** 32 + 5, 1), (1, 2 ** 30), (1, 2 ** 32 + 1)):
+    x, pos = _shape_only((rows, heads, 2)), _shape_only((rows,), torch.int32)
+    few = _shape_only((rows, 1, 2))
+    with pytest.raises(ValueError, match="rows and"):
+      K.rotary(x, pos, table)
+    with pytest.raises(ValueError, match="rows and"):
+      Fn.qk_norm_rotary(few, x, None, None)
+    with pytest.raises(ValueError, match="rows and"):
+      K.qk_norm_rotary_bwd(x, few, None, None, None, None, x, few)
+    with pytest.raises(ValueError, match="rows and"):
+      Fn.packed_attention(x, few, few, K.AttentionPlan([1], device="cpu"))
+  lib = _lib.load()
+  rows = ctypes.byref(_lib.HeadRows(4096, 64, 64, 2 ** 30, None))
+  rot = ctypes.byref(_lib.Rotation(4096, 4096, 1.0, 1, 64, 0))
+  assert lib.cg_rotary(rows, 1, 64, 0, rot, 0, 4096, None) == -2
+  assert lib.cg_qk_norm_rotary_fwd(rows, rows, 1, 64, 0, 1e-6, None, 4096, 4096, None) == -2
