@@ -1097,17 +1097,39 @@ _ROTATION = struct.Struct("@PPfiii0q")
 _ATTENTION_INPUT = struct.Struct("@PPPqqqqqqiiiif0q")
 
 
-def _launch(entry, t, *args):
-    """Calls an entry point with `t`'s device current, whichever one is, and that device's current stream."""
+def _launch(entry, t, *args, constant=None):
+    """Calls an entry point with `t`'s device current, whichever one is, and that device's current stream; `constant`:
+    the _DeviceConstant that it reads, if any."""
     index = t.get_device()
     fn = getattr(lib(), entry)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if constant is not None and stream not in constant.streams:
+        constant.read_on(stream, index)
     if index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(*args, stream)
     if rc:
         check(rc, entry)
+
+
+class _DeviceConstant(object):
+    """A tensor that is made once and read on any stream.  It is there for all of them (its upload is waited for), and
+    every stream that reads it is recorded with the allocator: its memory belongs to the stream it was made on, and
+    dropped while a kernel of another one still reads it, it would be given to that stream's next tensor.  (One record a
+    stream is enough: the allocator holds the memory until all that the stream was given by then is done.)"""
+
+    def __init__(self, t):
+        self.tensor, self.streams = t, set()
+        if t.is_cuda:
+            stream = torch.cuda.current_stream(t.device)
+            stream.synchronize()
+            self.streams.add(stream.cuda_stream)
+
+    def read_on(self, stream, index):
+        self.tensor.record_stream(torch.cuda.current_stream(index))
+        self.streams.add(stream)
 
 
 class RotaryTable(object):
@@ -1123,7 +1145,8 @@ class RotaryTable(object):
                "yarn"    pairs that turn more than 32 times over original_length stay, those that turn
                          less than once are divided by factor, linear in the number of turns between
                          (NTK by parts); the turned part is scaled by 0.1 ln(factor) + 1.
-    The table lives on `device` (fp64, turns a position) and is made once; it is read-only afterwards."""
+    The table lives on `device` (fp64, turns a position) and is made once; it is read-only afterwards, on any stream.
+    A captured graph reads it on every replay: keep it as long as the graph."""
 
     SCALINGS = ("none", "linear", "ntk", "yarn")
 
@@ -1163,17 +1186,11 @@ class RotaryTable(object):
         self.freq = torch.tensor(turns * axes, dtype=F64, device=device)
         self.index = self.freq.get_device()
         self._tail = (self.freq.data_ptr(), self.amplitude, axes, rotary_dim, 1 if layout == "interleaved" else 0)
-        _ready_on_every_stream(self.freq)
+        self.constant = _DeviceConstant(self.freq)
 
     def packed(self, positions):
         """cgRotation for `positions` (its bytes)."""
         return _ROTATION.pack(positions.data_ptr(), *self._tail)
-
-
-def _ready_on_every_stream(t):
-    """Constants (tables, plans) are used on any stream: wait for their upload once, when they are made."""
-    if t.is_cuda:
-        torch.cuda.current_stream(t.device).synchronize()
 
 
 def _req_heads(t, name, like=None):
@@ -1255,7 +1272,7 @@ def _rotate(x, positions, table, inverse):
     rows, _, width = x.shape
     y = _dense_like(x)
     _launch("cg_rotary", x, _head_rows(x), rows, width, HEAD_TYPES[x.dtype], table.packed(positions),
-            1 if inverse else 0, y.data_ptr())
+            1 if inverse else 0, y.data_ptr(), constant=table.constant)
     return y
 
 
@@ -1290,9 +1307,9 @@ def _qk_rows(q, k, q_gain, k_gain, positions, table, eps):
     """qk_norm_rotary on arguments that are known to fit."""
     rows, _, width = q.shape
     q_out, k_out = _dense_like(q), _dense_like(k)
-    rot = None if table is None else table.packed(positions)
+    rot, constant = (None, None) if table is None else (table.packed(positions), table.constant)
     _launch("cg_qk_norm_rotary_fwd", q, _head_rows(q, q_gain), _head_rows(k, k_gain), rows, width,
-            HEAD_TYPES[q.dtype], eps, rot, q_out.data_ptr(), k_out.data_ptr())
+            HEAD_TYPES[q.dtype], eps, rot, q_out.data_ptr(), k_out.data_ptr(), constant=constant)
     return q_out, k_out
 
 
@@ -1314,10 +1331,10 @@ def _qk_grads(q, k, q_gain, k_gain, positions, table, dq_out, dk_out, eps):
     dqg = None if q_gain is None else torch.empty_like(q_gain)
     dkg = None if k_gain is None else torch.empty_like(k_gain)
     ws = _ws(lib().cg_qk_norm_rotary_bwd_workspace_bytes(rows, width), q)
-    rot = None if table is None else table.packed(positions)
+    rot, constant = (None, None) if table is None else (table.packed(positions), table.constant)
     _launch("cg_qk_norm_rotary_bwd", q, _head_rows(q, q_gain), _head_rows(k, k_gain), dq_out.data_ptr(),
             dk_out.data_ptr(), rows, width, HEAD_TYPES[q.dtype], eps, rot, dq.data_ptr(), dk.data_ptr(), _p(dqg),
-            _p(dkg), ws.data_ptr(), ws.numel())
+            _p(dkg), ws.data_ptr(), ws.numel(), constant=constant)
     return dq, dk, dqg, dkg
 
 
@@ -1331,7 +1348,8 @@ class AttentionPlan(object):
                             room is [sequences * capacity, heads, D] with starts at multiples of capacity.
     heads, kv_heads       : query head h reads key head h // (heads / kv_heads).
     causal                : row i of a sequence sees its keys 0 .. i + k_length - q_length (the last row
-                            sees all of them; rows in front of the first key see none and give 0)."""
+                            sees all of them; rows in front of the first key see none and give 0).
+    A plan holds for any stream.  A captured graph reads it on every replay: keep it as long as the graph."""
 
     def __init__(self, q_lengths, k_lengths=None, heads=1, kv_heads=None, causal=False, q_starts=None,
                  k_starts=None, device="cuda"):
@@ -1360,7 +1378,7 @@ class AttentionPlan(object):
         self.device = torch.device(device)
         self.data = torch.from_numpy(self.host).to(self.device)
         self.index = self.data.get_device()
-        _ready_on_every_stream(self.data)
+        self.constant = _DeviceConstant(self.data)
 
 
 def _sequences(starts, lengths, name):
@@ -1462,7 +1480,7 @@ def _attention_rows(q, k, v, plan, scale, want_grad, out=None):
         nbytes = lib().cg_packed_attention_fwd_workspace_bytes(plan.ref, shape[2])
         ws = _ws(nbytes, q)
     _launch("cg_packed_attention_fwd", q, _attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(),
-            out.data_ptr(), _p(low), _p(lse), _p(ws), nbytes)
+            out.data_ptr(), _p(low), _p(lse), _p(ws), nbytes, constant=plan.constant)
     return out, (lse, low) if want_grad else None
 
 
@@ -1496,7 +1514,7 @@ def _attention_grads(q, k, v, plan, out, lse, low, dout, scale):
         ws = _ws(nbytes, q)
     _launch("cg_packed_attention_bwd", q, _attention_packed(q, k, v, scale), plan.ref, plan.data.data_ptr(),
             out.data_ptr(), _p(low), lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-            _p(ws), nbytes)
+            _p(ws), nbytes, constant=plan.constant)
     return dq, dk, dv
 
 

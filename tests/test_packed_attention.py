@@ -303,3 +303,52 @@ def test_rows_and_heads_beyond_32_bits_are_refused(monkeypatch):
   rot = ctypes.byref(_lib.Rotation(4096, 4096, 1.0, 1, 64, 0))
   assert lib.cg_rotary(rows, 1, 64, 0, rot, 0, 4096, None) == -2
   assert lib.cg_qk_norm_rotary_fwd(rows, rows, 1, 64, 0, 1e-6, None, 4096, 4096, None) == -2
+
+
+class _Recorder(object):
+  """Stands for a constant's tensor: notes the streams that are recorded with the allocator."""
+
+  def __init__(self):
+    self.recorded = []
+
+  def record_stream(self, stream):
+    self.recorded.append(stream)
+
+
+def test_constants_are_recorded_on_every_other_stream_that_reads_them(monkeypatch):
+  """Once a stream, before the call, the one they were made on excepted; calls on other streams' handles stay apart."""
+  current = {"raw": 7}
+  calls = []
+
+  class Library(object):
+    def __getattr__(self, name):
+      if name.endswith("workspace_bytes"):
+        return lambda *_: 0
+      return lambda *args: calls.append((name, args[-1], len(seen.recorded))) or 0
+  x, pos = torch.zeros((4, 1, 8), dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int32)
+  seen = _Recorder()
+  table = K.RotaryTable(8, device="cpu")
+  plan = K.AttentionPlan([40], device="cpu")
+  monkeypatch.setattr(K, "lib", Library)
+  monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: current["raw"], raising=False)
+  monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+  monkeypatch.setattr(torch.cuda, "current_stream", lambda index=None: ("stream", current["raw"]))
+  monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+  y = torch.zeros((40, 1, 8), dtype=torch.bfloat16)
+  stats = torch.zeros((40, 1))
+  entries = [(table, lambda: K._rotate(x, pos, table, False)),
+             (table, lambda: K._qk_rows(x, x, None, None, pos, table, 1e-6)),
+             (table, lambda: K._qk_grads(x, x, None, None, pos, table, x, x, 1e-6)),
+             (plan, lambda: K._attention_rows(y, y, y, plan, 1.0, True)),
+             (plan, lambda: K._attention_grads(y, y, y, plan, y, stats, y, y, 1.0))]
+  for owner, call in entries:
+    seen = _Recorder()
+    owner.constant.tensor, owner.constant.streams = seen, {7}
+    del calls[:]
+    for raw in (7, 9, 9, 7, 11, 9):
+      current["raw"] = raw
+      call()
+    assert seen.recorded == [("stream", 9), ("stream", 11)]
+    assert [c[1:] for c in calls] == [(7, 0), (9, 1), (9, 1), (7, 1), (11, 2), (9, 2)]
+  # nothing to keep: no table
+  K._qk_rows(x, x, None, None, None, None, 1e-6)

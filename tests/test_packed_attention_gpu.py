@@ -829,3 +829,39 @@ def test_norm_beside_copied_entries_that_are_not_finite(K, Fn, d, rot, dtype):
     assert torch.equal(got[2][rest], grads[2][rest]) and not torch.isfinite(got[2][at]), at
     got[0][4, 1], grads[0][4, 1] = 0.0, 0.0
     assert torch.equal(got[0], grads[0]) and torch.equal(got[1], grads[1]) and torch.equal(got[3], grads[3])
+
+
+def test_plan_and_table_dropped_while_another_stream_reads_them(K, Fn):
+  """Their memory is not given to other tensors before that stream is done (nothing is written to those here), and the
+  results are the ones of a plan and a table that live on."""
+  gen = torch.Generator().manual_seed(13)
+  lens = [1 + (i * 37) % 300 for i in range(60)]
+  n = sum(lens)
+  q, pos = normal(gen, (n, 2, 64)).cuda(), torch.arange(n, dtype=torch.int32, device="cuda")
+
+  def make():
+    return K.RotaryTable(64), K.AttentionPlan(lens, heads=2, causal=True)
+
+  def call(table, plan):
+    return Fn.packed_attention(Fn.rotary(q, pos, table), q, q, plan)
+  table, plan = make()
+  want = call(table, plan)
+  busy = torch.randn((4096, 4096), device="cuda").bfloat16()
+  torch.matmul(busy, busy)
+  side = torch.cuda.Stream()
+  torch.cuda.synchronize()
+  del table, plan
+  table, plan = make()
+  places = {table.freq.data_ptr(): table.freq.numel() * 8, plan.data.data_ptr(): plan.data.numel() * 4}
+  with torch.cuda.stream(side):
+    for _ in range(400):             # some tens of milliseconds in front of the call
+      torch.matmul(busy, busy)
+    got = call(table, plan)
+    done = torch.cuda.Event()
+    done.record()
+  del table, plan
+  others = [torch.empty(size, dtype=torch.uint8, device="cuda") for size in places.values() for _ in range(8)]
+  assert not done.query(), "the other stream was done before the test looked"
+  assert not {x.data_ptr() for x in others} & set(places)
+  torch.cuda.synchronize()
+  assert torch.equal(got, want)
