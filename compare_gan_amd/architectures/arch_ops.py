@@ -884,11 +884,12 @@ _ATTENTION_CONSTANTS = {}
 def _attention_constants(n, h, w, heads, kv_heads, width, base, device):
   key = (n, h, w, heads, kv_heads, width, base, str(device))
   if key not in _ATTENTION_CONSTANTS:
-    cell = torch.arange(n * h * w, device=device) % (h * w)
-    positions = torch.stack((cell // w, cell % w), 1).to(torch.int32)
-    _ATTENTION_CONSTANTS[key] = (
-        positions, K.RotaryTable(width, base=base, axes=2, device=device),
-        K.AttentionPlan([h * w] * n, heads=heads, kv_heads=kv_heads, device=device))
+    with torch.inference_mode(False):     # a later training step saves the positions for its backward pass
+      cell = torch.arange(n * h * w, device=device) % (h * w)
+      positions = torch.stack((cell // w, cell % w), 1).to(torch.int32)
+      _ATTENTION_CONSTANTS[key] = (
+          positions, K.RotaryTable(width, base=base, axes=2, device=device),
+          K.AttentionPlan([h * w] * n, heads=heads, kv_heads=kv_heads, device=device))
   return _ATTENTION_CONSTANTS[key]
 
 

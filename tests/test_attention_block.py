@@ -74,3 +74,22 @@ def test_refusals(kw):
   with ops.use_store(ops.VariableStore("meta")):
     with pytest.raises(ValueError):
       ops.attention_block(x, "non_local_block", use_sn=False, **kw)
+
+
+def test_constants_first_made_in_inference_mode_serve_training():
+  with torch.inference_mode():
+    positions = ops._attention_constants(2, 3, 5, 1, 1, 16, 71.0, torch.device("cpu"))[0]
+  assert positions.tolist() == [[r, c] for _ in range(2) for r in range(3) for c in range(5)]
+
+  class Saves(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions):
+      ctx.save_for_backward(positions)
+      return x.clone()
+
+    @staticmethod
+    def backward(ctx, dy):
+      return dy, None
+  x = torch.ones(1, requires_grad=True)
+  Saves.apply(x, positions).backward()
+  assert x.grad.item() == 1.0
