@@ -10,8 +10,10 @@ graph (variables, shapes) -- there is no CPU arithmetic path.
 Fusion device: `Act(x, slope)` is a *pending* leaky-ReLU.  Convolutions, linear layers and the
 spatial reductions consume it as an input gate of their kernel instead of materialising act(x).
 """
+import collections
 import contextlib
 import math
+import threading
 
 import torch
 
@@ -876,21 +878,47 @@ def non_local_block(x, name, use_sn):
                    kernel_scale=sigma, residual=x.contiguous())
 
 
-# what multi_head_block keeps for a call shape: positions, frequencies and the plan live as long as the process (a
-# captured step reads them on every replay)
-_ATTENTION_CONSTANTS = {}
+# What multi_head_block keeps: a frequency table for each head width, and positions and a plan for each call shape.  Of the
+# shapes the last ATTENTION_SHAPES stay (training, evaluation, sampling, the last batch of a pass), and every one that a
+# captured step has read: its replays read the same memory.
+ATTENTION_SHAPES = 16
+_ATTENTION_TABLES = {}
+_ATTENTION_RECENT = collections.OrderedDict()
+_ATTENTION_CAPTURED = {}
+_ATTENTION_LOCK = threading.Lock()      # (replicas may be threads)
+
+
+def _capturing(device):
+  return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
 
 
 def _attention_constants(n, h, w, heads, kv_heads, width, base, device):
-  key = (n, h, w, heads, kv_heads, width, base, str(device))
-  if key not in _ATTENTION_CONSTANTS:
+  """(positions, table, plan) of multi_head_block on n maps of h x w."""
+  captures = _capturing(device)
+  shape, turn = (n, h, w, heads, kv_heads, str(device)), (width, base, str(device))
+  with _ATTENTION_LOCK:
+    kept = _ATTENTION_CAPTURED.get(shape) or _ATTENTION_RECENT.get(shape)
+    if captures and (kept is None or turn not in _ATTENTION_TABLES):
+      raise RuntimeError("multi_head_block: positions and plan of %d maps of %d x %d are not there yet, and cannot be made "
+                         "while a step is captured: run it once before" % (n, h, w))
     with torch.inference_mode(False):     # a later training step saves the positions for its backward pass
-      cell = torch.arange(n * h * w, device=device) % (h * w)
-      positions = torch.stack((cell // w, cell % w), 1).to(torch.int32)
-      _ATTENTION_CONSTANTS[key] = (
-          positions, K.RotaryTable(width, base=base, axes=2, device=device),
-          K.AttentionPlan([h * w] * n, heads=heads, kv_heads=kv_heads, device=device))
-  return _ATTENTION_CONSTANTS[key]
+      if turn not in _ATTENTION_TABLES:
+        _ATTENTION_TABLES[turn] = K.RotaryTable(width, base=base, axes=2, device=device)
+      if kept is None:
+        cell = torch.arange(n * h * w, device=device) % (h * w)
+        positions = torch.stack((cell // w, cell % w), 1).to(torch.int32)
+        kept = (K.DeviceConstant(positions),
+                K.AttentionPlan([h * w] * n, heads=heads, kv_heads=kv_heads, device=device))
+    if captures:
+      _ATTENTION_CAPTURED[shape] = kept
+    if shape not in _ATTENTION_CAPTURED:
+      _ATTENTION_RECENT[shape] = kept
+      _ATTENTION_RECENT.move_to_end(shape)
+      if len(_ATTENTION_RECENT) > ATTENTION_SHAPES:
+        _ATTENTION_RECENT.popitem(last=False)
+    else:
+      _ATTENTION_RECENT.pop(shape, None)
+    return kept[0].read(), _ATTENTION_TABLES[turn], kept[1]
 
 
 def multi_head_block(x, name, use_sn, num_heads=None, num_kv_heads=None, head_width=64, rotary_base=100.0):

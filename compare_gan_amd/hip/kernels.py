@@ -1099,7 +1099,7 @@ _ATTENTION_INPUT = struct.Struct("@PPPqqqqqqiiiif0q")
 
 def _launch(entry, t, *args, constant=None):
     """Calls an entry point with `t`'s device current, whichever one is, and that device's current stream; `constant`:
-    the _DeviceConstant that it reads, if any."""
+    the DeviceConstant that it reads, if any."""
     index = t.get_device()
     fn = getattr(lib(), entry)
     stream = torch._C._cuda_getCurrentRawStream(index)
@@ -1114,7 +1114,7 @@ def _launch(entry, t, *args, constant=None):
         check(rc, entry)
 
 
-class _DeviceConstant(object):
+class DeviceConstant(object):
     """A tensor that is made once and read on any stream.  It is there for all of them (its upload is waited for), and
     every stream that reads it is recorded with the allocator: its memory belongs to the stream it was made on, and
     dropped while a kernel of another one still reads it, it would be given to that stream's next tensor.  (One record a
@@ -1130,6 +1130,15 @@ class _DeviceConstant(object):
     def read_on(self, stream, index):
         self.tensor.record_stream(torch.cuda.current_stream(index))
         self.streams.add(stream)
+
+    def read(self):
+        """The tensor, to be read on its device's current stream."""
+        if self.tensor.is_cuda:
+            index = self.tensor.get_device()
+            stream = torch._C._cuda_getCurrentRawStream(index)
+            if stream not in self.streams:
+                self.read_on(stream, index)
+        return self.tensor
 
 
 class RotaryTable(object):
@@ -1186,7 +1195,7 @@ class RotaryTable(object):
         self.freq = torch.tensor(turns * axes, dtype=F64, device=device)
         self.index = self.freq.get_device()
         self._tail = (self.freq.data_ptr(), self.amplitude, axes, rotary_dim, 1 if layout == "interleaved" else 0)
-        self.constant = _DeviceConstant(self.freq)
+        self.constant = DeviceConstant(self.freq)
 
     def packed(self, positions):
         """cgRotation for `positions` (its bytes)."""
@@ -1378,7 +1387,7 @@ class AttentionPlan(object):
         self.device = torch.device(device)
         self.data = torch.from_numpy(self.host).to(self.device)
         self.index = self.data.get_device()
-        self.constant = _DeviceConstant(self.data)
+        self.constant = DeviceConstant(self.data)
 
 
 def _sequences(starts, lengths, name):

@@ -93,3 +93,46 @@ def test_constants_first_made_in_inference_mode_serve_training():
   x = torch.ones(1, requires_grad=True)
   Saves.apply(x, positions).backward()
   assert x.grad.item() == 1.0
+
+
+@pytest.fixture
+def no_constants(monkeypatch):
+  """The block's constants as in a new process, put back afterwards."""
+  for name in ("_ATTENTION_TABLES", "_ATTENTION_CAPTURED"):
+    monkeypatch.setattr(ops, name, {})
+  monkeypatch.setattr(ops, "_ATTENTION_RECENT", type(ops._ATTENTION_RECENT)())
+
+
+def _constants(n, width=32, side=4, heads=2, base=100.0):
+  return ops._attention_constants(n, side, side, heads, 1, width, base, torch.device("cpu"))
+
+
+def test_constants_are_kept_for_the_last_shapes_only(no_constants):
+  """One table a head width, whatever the batch; the shapes used last stay, the others are made again."""
+  first = _constants(1)
+  again = _constants(1)
+  assert all(a is b for a, b in zip(first, again))
+  for n in range(2, 3 * ops.ATTENTION_SHAPES):
+    positions, table, plan = _constants(n)
+    assert table is first[1] and positions.shape == (16 * n, 2) and plan.q_rows == 16 * n
+    assert _constants(1)[2] is first[2]                  # (used in between: stays)
+    assert len(ops._ATTENTION_RECENT) <= ops.ATTENTION_SHAPES
+  last = _constants(3 * ops.ATTENTION_SHAPES - 1)
+  assert last[2] is plan and _constants(2)[2].q_rows == 32
+  assert _constants(1, width=16)[1] is not first[1] and _constants(1, base=50.0)[1] is not first[1]
+  assert _constants(1, width=16)[2] is first[2]          # (positions and plan do not depend on them)
+
+
+def test_constants_that_a_capture_has_read_stay(no_constants, monkeypatch):
+  kept = _constants(1)
+  monkeypatch.setattr(ops, "_capturing", lambda device: True)
+  assert _constants(1)[2] is kept[2]
+  with pytest.raises(RuntimeError, match="run it once before"):
+    _constants(2)
+  with pytest.raises(RuntimeError, match="run it once before"):
+    _constants(1, width=64)
+  monkeypatch.setattr(ops, "_capturing", lambda device: False)
+  for n in range(2, 3 * ops.ATTENTION_SHAPES):
+    _constants(n)
+  assert all(a is b for a, b in zip(_constants(1), kept))
+  assert len(ops._ATTENTION_RECENT) <= ops.ATTENTION_SHAPES

@@ -109,3 +109,36 @@ def test_biggan_step_with_several_heads(dev, arch):
   assert not [k for k in se if not torch.equal(se[k], sg[k])]
   still = [k for k, v in before.items() if k in eager.store.trainable and torch.equal(v, eager.store.vars[k])]
   assert not still, still
+
+
+def test_block_captured_while_other_shapes_come_and_go(dev):
+  """What a captured call reads stays where it is: replays agree with eager calls after many other shapes.  A shape that
+  is first met inside a capture is refused with a message."""
+  from compare_gan_amd.architectures import arch_ops as ops
+  from compare_gan_amd.hip import functional as Fn
+  side = 12
+  rows = side * side
+  gen = torch.Generator().manual_seed(5)
+  q, k, v = (torch.randn((rows, 2, 32), generator=gen).bfloat16().to(dev) for _ in range(3))
+
+  def call():
+    positions, table, plan = ops._attention_constants(1, side, side, 2, 2, 32, 100.0, dev)
+    a, b = Fn.qk_norm_rotary(q, k, None, None, positions, table)
+    return Fn.packed_attention(a, b, v, plan)
+  call()
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    held = call()
+    with pytest.raises(RuntimeError, match="run it once before"):
+      ops._attention_constants(1, side, side + 1, 2, 2, 32, 100.0, dev)
+  others = []
+  for n in range(2, 2 * ops.ATTENTION_SHAPES):
+    ops._attention_constants(n, side, side, 2, 2, 32, 100.0, dev)
+    others.append(torch.full((rows * 2,), -1, dtype=torch.int32, device=dev))
+  for _ in range(3):
+    q.copy_(torch.randn(q.shape, generator=gen))
+    want = call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, want)
