@@ -1399,10 +1399,13 @@ def _sequences(starts, lengths, name):
     if lengths.dtype.kind not in "iu" or (starts is not None and starts.dtype.kind not in "iu"):
         raise ValueError("%s: starts and lengths must be whole numbers" % name)
     lengths = lengths.astype(np.int64)
+    # (each for itself first: the sum of two of 63 bits would wrap)
+    if (lengths < 0).any() or (lengths >= 2 ** 30).any():
+        raise ValueError("%s: starts and lengths must be in [0, 2^30)" % name)
     starts = np.cumsum(lengths) - lengths if starts is None else starts.astype(np.int64)
     if starts.size != lengths.size:
         raise ValueError("%s_starts names %d sequences, %s_lengths %d" % (name, starts.size, name, lengths.size))
-    if (lengths < 0).any() or (starts < 0).any() or (starts + lengths >= 2 ** 30).any():
+    if (starts < 0).any() or (starts >= 2 ** 30).any() or (starts + lengths >= 2 ** 30).any():
         raise ValueError("%s: starts and lengths must be in [0, 2^30)" % name)
     live = lengths > 0
     order = np.argsort(starts[live], kind="stable")

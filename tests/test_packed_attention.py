@@ -352,3 +352,12 @@ def test_constants_are_recorded_on_every_other_stream_that_reads_them(monkeypatc
     assert [c[1:] for c in calls] == [(7, 0), (9, 1), (9, 1), (7, 1), (11, 2), (9, 2)]
   # nothing to keep: no table
   K._qk_rows(x, x, None, None, None, None, 1e-6)
+
+
+@pytest.mark.parametrize("q_lengths,q_starts", [([2 ** 62 + 5], [2 ** 63 - 2 ** 32 + 10]), ([5], [2 ** 63 - 2]),
+                                                ([2 ** 63 - 1, 3], None), ([2 ** 62, 2 ** 62, 4], None)])
+def test_plan_refuses_lengths_whose_sums_wrap(q_lengths, q_starts):
+  """Their low 32 bits are lengths and starts that a plan would take."""
+  with pytest.raises(ValueError, match="2\\^30"):
+    K.AttentionPlan(np.array(q_lengths), [3] * len(q_lengths), q_starts=None if q_starts is None else np.array(q_starts),
+                    device="cpu")
