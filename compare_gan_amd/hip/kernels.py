@@ -1173,12 +1173,16 @@ class RotaryTable(object):
             raise ValueError("base must be positive and finite, got %r" % (base,))
         if not (factor >= 1.0 and math.isfinite(factor)):
             raise ValueError("factor must be finite and at least 1, got %r" % (factor,))
-        if original_length < 1:
-            raise ValueError("original_length must be positive, got %r" % (original_length,))
+        if not (original_length >= 1 and math.isfinite(original_length)):
+            raise ValueError("original_length must be finite and at least 1, got %r" % (original_length,))
         n = rotary_dim // 2 // axes
         self.amplitude = 1.0
         if scaling == "ntk" and n > 1:
+            if math.log(base) + math.log(factor) * n / (n - 1.0) > 700.0:
+                raise ValueError("base %r times factor %r is too large" % (base, factor))
             base = base * factor ** (n / (n - 1.0))
+        if base < 1e-300:        # (the last frequency, close to 1 / base, has to be a number)
+            raise ValueError("base %r is too small" % (base,))
         turns = []
         for i in range(n):
             f = base ** (-float(i) / n)

@@ -361,3 +361,19 @@ def test_plan_refuses_lengths_whose_sums_wrap(q_lengths, q_starts):
   with pytest.raises(ValueError, match="2\\^30"):
     K.AttentionPlan(np.array(q_lengths), [3] * len(q_lengths), q_starts=None if q_starts is None else np.array(q_starts),
                     device="cpu")
+
+
+@pytest.mark.parametrize("kw", [dict(scaling="yarn", factor=2.0, original_length=float("nan")),
+                                dict(scaling="yarn", factor=2.0, original_length=float("inf")),
+                                dict(scaling="ntk", base=1e300, factor=1e10), dict(scaling="ntk", factor=1e300),
+                                dict(scaling="ntk", base=1e300, factor=1e300), dict(base=1e-320),
+                                dict(scaling="ntk", base=1e-320)])
+def test_rotary_table_refuses_what_has_no_frequencies(kw):
+  with pytest.raises(ValueError):
+    K.RotaryTable(8, device="cpu", **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(scaling="ntk", base=1e150, factor=1e100), dict(base=1e-299), dict(base=1e300)])
+def test_rotary_table_at_the_ends_of_its_range(kw):
+  f = K.RotaryTable(8, device="cpu", **kw).freq
+  assert torch.isfinite(f).all() and (f > 0).all()
