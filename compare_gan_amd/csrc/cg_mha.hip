@@ -1335,6 +1335,9 @@ int mha_check(const char* name, const cgAttentionInput* in, const cgAttentionPla
   const int64_t st[6] = {in->q_stride_t, in->q_stride_h, in->k_stride_t, in->k_stride_h, in->v_stride_t, in->v_stride_h};
   for (int i = 0; i < 6; ++i)
     if (st[i] < 0 || st[i] % 8) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: strides have to be multiples of 8 elements", name);
+  for (int i = 0; i < 6; ++i)     // (no tensor is that long; the products below and the kernels' offsets stay in 64 bits)
+    if (st[i] > (1ll << 40)) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: strides too large", name);
+  if ((uintptr_t)data % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: the plan has to be 16-byte aligned", name);
   const void* ptr[3] = {in->q, in->k, in->v};
   for (int i = 0; i < 3; ++i) {
     // (no keys at all: K and V may be null, no work item reads them)
@@ -1441,7 +1444,7 @@ extern "C" int cg_packed_attention_fwd(const cgAttentionInput* in, const cgAtten
   if (rc) return rc;
   if (plan->max_q_row == 0) return CG_OK;
   if (!out) CG_FAIL(CG_ERR_BAD_ARG, "%s: null output", name);
-  if ((uintptr_t)out % 16 || (uintptr_t)out_low % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: tensors have to be 16-byte aligned", name);
+  if ((uintptr_t)out % 16 || (uintptr_t)out_low % 16 || (uintptr_t)ws % 16) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: tensors and workspace have to be 16-byte aligned", name);
   if (plan->parts > 0 && (!ws || ws_bytes < cg_packed_attention_fwd_workspace_bytes(plan, in->Dv)))
     CG_FAIL(CG_ERR_WORKSPACE, "%s: workspace of %zu bytes", name, ws_bytes);
   a.out = (bf16_t*)out;

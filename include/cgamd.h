@@ -596,7 +596,8 @@ int cg_qk_norm_rotary_bwd(const cgHeadRows* q, const cgHeadRows* k, const void* 
  * dealt to the 8 XCDs so that the tiles of one key head share an L2; few rows against many keys are
  * split over the keys.
  * cg_host_attention_plan fills `info` and, if data_host is not NULL, `info->ints` int32 there; the caller
- * copies them to the device and hands that copy and `info` to the kernels. */
+ * copies them to the device (16-byte aligned) and hands that copy and `info` to the kernels.  Sequences must not
+ * share rows of an output (not checked here; K.AttentionPlan refuses it). */
 typedef struct {
   int64_t ints;                       /* size of the plan in int32 */
   int64_t parts, dq_parts, dkv_parts; /* partial results: workspaces of the forward and backward pass */
@@ -609,10 +610,10 @@ int cg_host_attention_plan(const int32_t* q_start, const int32_t* q_len, const i
                            const int32_t* k_len, int sequences, int heads, int kv_heads, int causal,
                            int32_t* data_host, int64_t capacity, cgAttentionPlan* info);
 /* q [q_rows, heads, D], k [k_rows, kv_heads, D], v [k_rows, kv_heads, Dv] bf16, strides in elements, heads
- * contiguous inside; D and Dv multiples of 8, at most 128; scale in [1e-30, 1e30].  out [q_rows, heads, Dv] contiguous,
- * lse [q_rows, heads] fp32 and out_low like out (what its rounding left over): for the backward pass, NULL where
- * none follows (out_low also where plan->dq_tiles is 0).  Rows that see no key: out 0, lse -inf.  Rows that belong to
- * no sequence are left as they were. */
+ * contiguous inside, tensors and workspaces 16-byte aligned; D and Dv multiples of 8, at most 128; scale in
+ * [1e-30, 1e30].  out [q_rows, heads, Dv] contiguous, lse [q_rows, heads] fp32 and out_low like out (what its
+ * rounding left over): for the backward pass, NULL where none follows (out_low also where plan->dq_tiles is 0).
+ * Rows that see no key: out 0, lse -inf.  Rows that belong to no sequence are left as they were. */
 typedef struct {
   const void *q, *k, *v;
   int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;

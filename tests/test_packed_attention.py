@@ -377,3 +377,26 @@ def test_rotary_table_refuses_what_has_no_frequencies(kw):
 def test_rotary_table_at_the_ends_of_its_range(kw):
   f = K.RotaryTable(8, device="cpu", **kw).freq
   assert torch.isfinite(f).all() and (f > 0).all()
+
+
+def test_attention_entry_points_refuse_what_is_not_aligned():
+  """The plan is read and partial results are written 16 bytes at a time; strides whose products would wrap."""
+  lib, fake = _lib.load(), 4096
+  plan = K.AttentionPlan([200], [70001], heads=2, kv_heads=1, device="cpu")
+  info = ctypes.byref(plan.info)
+  need = lib.cg_packed_attention_fwd_workspace_bytes(info, 64)
+  assert plan.info.parts > 0 and need > 0
+
+  def call(data=fake, ws=fake, **kw):
+    f = dict(q=fake, k=fake, v=fake, q_stride_t=128, q_stride_h=64, k_stride_t=64, k_stride_h=64,
+             v_stride_t=64, v_stride_h=64, q_rows=200, k_rows=70001, D=64, Dv=64, scale=1.0)
+    f.update(kw)
+    arg = ctypes.byref(_lib.AttentionInput(*[f[n] for n, _ in _lib.AttentionInput._fields_]))
+    return [lib.cg_packed_attention_fwd(arg, info, data, fake, None, None, ws, need if ws else 0, None),
+            lib.cg_packed_attention_bwd(arg, info, data, fake, fake, fake, fake, fake, fake, fake, ws,
+                                        0, None)]
+  assert call(ws=None) == [-4, -4]
+  assert call(data=fake + 4) == [-2, -2] and call(data=fake + 8) == [-2, -2]
+  assert call(ws=fake + 8)[0] == -2
+  for name in ("q_stride_t", "q_stride_h", "k_stride_t", "k_stride_h", "v_stride_t", "v_stride_h"):
+    assert call(ws=None, **{name: 2 ** 61}) == [-2, -2], name
