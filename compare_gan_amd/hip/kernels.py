@@ -1461,6 +1461,15 @@ def _attention_packed(q, k, v, scale):
                                  *_row_strides(v), q.shape[0], k.shape[0], q.shape[2], v.shape[2], scale)
 
 
+def _share_memory(a, b):
+    """Whether the addresses that `a` and `b` reach from end to end meet."""
+    ends = []
+    for t in (a, b):
+        reach = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        ends.append((t.data_ptr(), t.data_ptr() + reach * t.element_size()))
+    return ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]
+
+
 def _rows_out(shape, dense, used, like):
     """A dense bf16 output on `like`'s device whose rows outside every sequence are zero."""
     return like.new_empty(shape) if dense and used == shape[0] else like.new_zeros(shape)
@@ -1471,7 +1480,7 @@ def packed_attention_fwd(q, k, v, plan, scale=None, want_grad=True, out=None):
     v [rows, kv_heads, Dv] bf16 -> (out [rows, heads, Dv] bf16, saved).  saved: what packed_attention_bwd needs
     (lse [rows, heads] fp32, and what the rounding of out left over, or None where the plan has no use for it);
     None without want_grad.  scale: 1 / sqrt(D) by default.  Rows of q outside every sequence give zeros -- or keep
-    what `out`, if given (dense), holds there."""
+    what `out`, if given (dense, sharing no memory with q, k and v, which are read to the end), holds there."""
     scale = _attention_input(q, k, v, plan, scale)
     return _attention_rows(_attention_operand(q), _attention_operand(k), _attention_operand(v), plan, scale, want_grad,
                            out)
@@ -1486,6 +1495,8 @@ def _attention_rows(q, k, v, plan, scale, want_grad, out=None):
         _req(out, BF16, "out")
         if tuple(out.shape) != shape or out.device != q.device or out.data_ptr() % 16:
             raise ValueError("out must be %s on %s, 16-byte aligned" % (list(shape), q.device))
+        if any(_share_memory(out, t) for t in (q, k, v)):
+            raise ValueError("out must not share memory with q, k or v")
     lse = low = None
     if want_grad:
         lse = torch.empty(shape[:2], dtype=F32, device=q.device)

@@ -400,3 +400,12 @@ def test_attention_entry_points_refuse_what_is_not_aligned():
   assert call(ws=fake + 8)[0] == -2
   for name in ("q_stride_t", "q_stride_h", "k_stride_t", "k_stride_h", "v_stride_t", "v_stride_h"):
     assert call(ws=None, **{name: 2 ** 61}) == [-2, -2], name
+
+
+def test_shared_memory_is_seen():
+  x = torch.zeros(10, 6, 16)
+  whole = [(x[:, :2], x[:, 2:4], True), (x[:5], x[5:], False), (x[5:], x[:5], False), (x[:6], x[5:], True),
+           (x[:1, :2], x[:1, 2:], False), (x, x.clone(), False), (x[3:4], x, True), (x[:0], x, False),
+           (x[2, :1].expand(4, 16), x[2], True), (x[2, :1].expand(4, 16), x[2, 1:], False)]
+  for a, b, want in whole:
+    assert K._share_memory(a, b) is want and K._share_memory(b, a) is want

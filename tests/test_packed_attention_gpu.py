@@ -865,3 +865,22 @@ def test_plan_and_table_dropped_while_another_stream_reads_them(K, Fn):
   assert not {x.data_ptr() for x in others} & set(places)
   torch.cuda.synchronize()
   assert torch.equal(got, want)
+
+
+def test_an_output_that_is_an_input_is_refused(K):
+  """Rows are read until the last work item is done, so none of them may be written before."""
+  gen = torch.Generator().manual_seed(14)
+  plan = K.AttentionPlan([300], heads=2)
+  q, k, v = (normal(gen, (300, 2, 64)).cuda() for _ in range(3))
+  want = K.packed_attention_fwd(q, k, v, plan)[0]
+  for out in (q, k, v):
+    with pytest.raises(ValueError, match="share memory"):
+      K.packed_attention_fwd(q, k, v, plan, out=out)
+  # neighbours in one buffer are not each other's memory; a single token's row holds q, k, v and the output
+  buffer = torch.zeros((2, 300, 2, 64), dtype=torch.bfloat16, device="cuda")
+  buffer[0] = q
+  assert torch.equal(K.packed_attention_fwd(buffer[0], k, v, plan, out=buffer[1])[0], want)
+  row = normal(gen, (1, 8, 64)).cuda()
+  one = K.AttentionPlan([1], heads=2)
+  got = K.packed_attention_fwd(row[:, :2], row[:, 2:4], row[:, 4:6], one, out=row[:, 6:])[0]
+  assert torch.equal(got, row[:, 4:6]) and torch.equal(row[:, 6:], row[:, 4:6])
