@@ -142,3 +142,71 @@ def test_block_captured_while_other_shapes_come_and_go(dev):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(held, want)
+
+
+@pytest.mark.parametrize("n,h,w,c,heads,kv_heads,width", [(2, 8, 8, 64, 1, 1, 64), (3, 4, 6, 96, 4, 2, 32),
+                                                        (1, 5, 5, 32, 2, 1, 16)])
+def test_block_with_independent_roundings(dev, n, h, w, c, heads, kv_heads, width):
+  """The block against the chain in 64 bits with a bound that 2 % of a gradient does not pass.  Between an input and a
+  gradient lie at most 16 roundings to bf16: the operand images of the four projections, q, k, v, the turned q and k, P,
+  the attention's result, its incoming gradient, dS, the gradients of the turned and of the projected queries (keys), and
+  the result's.  Each is an independent error of at most HB, HB / sqrt(3) root mean square, of what passes through:
+  sqrt(16 / 3) HB = 0.9 % of the norm.  The gradients of sigma and of the gains are sums over rows of terms of either sign
+  (of a key's gain: from rows of dS that sum to zero), each term off by its own roundings: their errors are held against
+  the norm of the terms."""
+  from compare_gan_amd.architectures import arch_ops as ops
+  gen = torch.Generator().manual_seed(n + c)
+  store = ops.VariableStore(dev, seed=1)
+  x = torch.randn((n, h, w, c), generator=gen).bfloat16().to(dev).requires_grad_(True)
+  args = dict(kind="multi_head", num_heads=heads, num_kv_heads=kv_heads, head_width=width)
+  with ops.use_store(store):
+    ops.attention_block(x.detach(), "att", False, **args)
+    with torch.no_grad():
+      for name, v in store.vars.items():
+        if name.endswith("kernel"):
+          v.copy_(torch.randn(v.shape, generator=gen).to(dev) / math.sqrt(v.shape[2]))
+        elif name.endswith("gain"):
+          v.copy_((1 + 0.2 * torch.randn(v.shape, generator=gen)).to(dev))
+        else:
+          v.fill_(0.7)
+    out = ops.attention_block(x, "att", False, **args)
+  dout = torch.randn((n, h, w, c), generator=gen).bfloat16().to(dev)
+  names = sorted(store.vars)
+  grads = torch.autograd.grad(out, [x] + [store.vars[k] for k in names], dout)
+  rows, pairs = n * h * w, width // 2
+  # gains and sigma with one entry for every term of their gradients
+  shapes = {"q_gain": (rows, heads, width), "k_gain": (rows, kv_heads, width), "sigma": (rows, c)}
+  v64 = {}
+  for k in names:
+    short, v = k.split("att/")[1], store.vars[k].detach().double().cpu()
+    v64[short] = (v.expand(shapes[short]).clone() if short in shapes else v[0, 0].clone()).requires_grad_(True)
+  x64 = x.detach().double().cpu().reshape(rows, c).requires_grad_(True)
+  cell = torch.arange(rows) % (h * w)
+  f = 100.0 ** (-torch.arange(pairs // 2, dtype=torch.float64) / (pairs // 2))
+  z = torch.polar(torch.ones(rows, pairs, dtype=torch.float64),
+                  torch.cat(((cell // w)[:, None] * f, (cell % w)[:, None] * f), 1))[:, None]
+
+  def norm_turn(t, gain):
+    t = t / torch.sqrt(t.square().mean(-1, keepdim=True) + 1e-6) * gain
+    t = torch.complex(t[..., :pairs], t[..., pairs:]) * z
+    return torch.cat((t.real, t.imag), -1)
+
+  def project(which, m):
+    return (x64 @ v64["conv2d_%s/kernel" % which]).reshape(rows, m, width)
+  q, k = norm_turn(project("q", heads), v64["q_gain"]), norm_turn(project("k", kv_heads), v64["k_gain"])
+  v = project("v", kv_heads)
+  o = torch.empty(0, heads * width, dtype=torch.float64)
+  for i in range(n):
+    mine = slice(i * h * w, (i + 1) * h * w)
+    per_head = [torch.softmax(q[mine, j] @ k[mine, j * kv_heads // heads].t() / math.sqrt(width), -1) @
+                v[mine, j * kv_heads // heads] for j in range(heads)]
+    o = torch.cat((o, torch.cat(per_head, 1)))
+  want = x64 + v64["sigma"] * (o @ v64["conv2d_o/kernel"])
+  short = [k.split("att/")[1] for k in names]
+  wgrads = torch.autograd.grad(want, [x64] + [v64[k] for k in short], dout.double().cpu().reshape(rows, c))
+  for name, a, b in zip(["out", "dx"] + short, (out,) + grads, (want,) + wgrads):
+    a, b = a.detach().double().cpu(), b.detach()
+    size = float(b.norm())
+    if name in shapes:
+      b = b.reshape(-1, a.numel()).sum(0)
+    assert float((a.flatten() - b.flatten()).norm()) <= math.sqrt(16 / 3) * HB * size, name

@@ -884,3 +884,146 @@ def test_an_output_that_is_an_input_is_refused(K):
   one = K.AttentionPlan([1], heads=2)
   got = K.packed_attention_fwd(row[:, :2], row[:, 2:4], row[:, 4:6], one, out=row[:, 6:])[0]
   assert torch.equal(got, row[:, 4:6]) and torch.equal(row[:, 6:], row[:, 4:6])
+
+
+# ------------------------------------------------------------------------------------------------
+# split items: nothing lost, nothing twice
+# ------------------------------------------------------------------------------------------------
+# The entry by entry bounds above are worst cases: where a row sees many keys whose values cancel they are as large as the
+# result, and a lost part hides in them.  So (a) whole tensors by their norm: inputs are independent and of zero mean,
+# so the errors of the rounded weights add up like the results themselves, HB / sqrt(3) of the norm, and the result's own
+# rounding is at most HB of it: 2 HB in all for out and dv (1.6 counted); dq and dk also carry delta's error, HB / sqrt(3)
+# again, and dP's: 3 HB (2.2 counted).  One lost part of n is 1 / sqrt(n) of the norm, 16 HB for 256 parts.
+def run_norms(K, Fn, *case, grad, **kw):
+  got, (q, k, v, dout, plan) = run_attention(K, Fn, *case, grad=grad, **kw)
+  q_lengths, k_lengths, heads, kv_heads, d, _, causal = case
+  kl = q_lengths if k_lengths is None else k_lengths
+  k0 = kw.get("k_starts") or [sum(kl[:i]) for i in range(len(kl))]
+  seqs = list(zip([sum(q_lengths[:i]) for i in range(len(q_lengths))], q_lengths, k0, kl))
+  want = exact_attention(q.detach(), k.detach(), v.detach(), dout, seqs, heads, kv_heads, causal, 1.0 / math.sqrt(d))
+  for name, (value, _) in want.items():
+    error = float((got[name].detach().double().cpu() - value).norm() / value.norm())
+    assert error <= (2 if name in ("out", "dv") else 3) * HB, (name, error)
+  return plan
+
+
+@pytest.mark.parametrize("case", NEW_TOKENS, ids=[str(i) for i in range(len(NEW_TOKENS))])
+def test_norm_of_new_tokens_against_a_cache(K, Fn, case):
+  k, heads, kv_heads, d, dv, capacity = case
+  n = len(k)
+  run_norms(K, Fn, [1] * n, k, heads, kv_heads, d, dv, True, grad=False, k_starts=[i * capacity for i in range(n)],
+            rows=(n, n * capacity))
+
+
+SPLIT = [
+    # q_lengths, k_lengths, heads, kv_heads, D, Dv, causal, what is split
+    ([70], [5000], 2, 1, 64, 64, True, "parts dq_parts"),
+    ([300, 3], [3000, 2000], 1, 1, 128, 96, False, "parts dq_parts"),
+    ([16], [40000], 4, 1, 72, 40, True, "parts dq_parts"),
+    ([40000], [16], 4, 1, 72, 40, False, "dkv_parts"),
+    ([9000], [200], 2, 2, 128, 128, False, "dkv_parts"),
+    ([4000], None, 2, 1, 64, 32, True, "parts dq_parts dkv_parts"),
+]
+
+
+@pytest.mark.parametrize("case", SPLIT, ids=[str(i) for i in range(len(SPLIT))])
+def test_norm_of_split_items(K, Fn, case):
+  plan = run_norms(K, Fn, *case[:7], grad=True)
+  for name in case[7].split():
+    assert getattr(plan.info, name) > 0, name
+
+
+# (b) inputs that mark the parts, and only terms of one sign in every sum: the bounds are then 2 HB or so of the result, and
+# a part that is lost or taken twice is a whole column (of at most a few blocks of 512)
+def marks(n, width):
+  x = torch.zeros(n, 1, width)
+  x[torch.arange(n), 0, (torch.arange(n) // 512) % width] = 1.0
+  return x
+
+
+@pytest.mark.parametrize("n,rows,heads,kv_heads,d,dv,causal", [
+    (131072, 1, 2, 1, 128, 128, True), (70000, 1, 1, 1, 128, 64, True), (40000, 16, 4, 1, 80, 40, True),
+    (20000, 150, 2, 1, 64, 64, False), (9001, 1, 12, 4, 24, 24, True), (6000, 300, 1, 1, 128, 128, True)])
+def test_every_part_of_the_keys_counts_once(K, Fn, n, rows, heads, kv_heads, d, dv, causal):
+  gen = torch.Generator().manual_seed(n)
+  plan = K.AttentionPlan([rows], [n], heads=heads, kv_heads=kv_heads, causal=causal)
+  assert plan.info.parts > 0 and plan.info.dq_parts > 0
+  q = 0.25 * normal(gen, (rows, heads, d), torch.float32)
+  k = marks(n, d).expand(n, kv_heads, d)
+  sign = 1.0 - 2.0 * ((torch.arange(n) // 512) % 2)
+  seqs = [(0, rows, 0, n)]
+  for v in (marks(n, dv).expand(n, kv_heads, dv), sign[:, None, None].expand(n, kv_heads, dv)):
+    q_, k_, v_ = (x.bfloat16().cuda().requires_grad_(True) for x in (q, k, v))
+    dout = normal(gen, (rows, heads, dv)).abs().cuda()
+    out = Fn.packed_attention(q_, k_, v_, plan)
+    dq, dk, dvalue = torch.autograd.grad(out, (q_, k_, v_), dout)
+    want = exact_attention(q_.detach(), k_.detach(), v_.detach(), dout, seqs, heads, kv_heads, causal, 1 / math.sqrt(d))
+    for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dvalue)):
+      within(got, want[name][0], want[name][1], name)
+    if v.min() >= 0:
+      assert float((want["out"][1] / want["out"][0].abs().clamp_min(1e-6)).max()) < 3 * HB     # (the bound is tight)
+    else:
+      assert float((want["dq"][1].norm() / want["dq"][0].norm())) < 5 * HB
+
+
+@pytest.mark.parametrize("rows,n,heads,kv_heads,d,dv", [(40000, 16, 4, 1, 72, 40), (70000, 40, 1, 1, 128, 128),
+                                                      (9000, 200, 2, 2, 64, 24)])
+def test_every_part_of_the_rows_counts_once(K, Fn, rows, n, heads, kv_heads, d, dv):
+  gen = torch.Generator().manual_seed(n)
+  plan = K.AttentionPlan([rows], [n], heads=heads, kv_heads=kv_heads)
+  assert plan.info.dkv_parts > 0
+  q = marks(rows, d).expand(rows, heads, d).bfloat16().cuda().requires_grad_(True)
+  dout = marks(rows, dv).expand(rows, heads, dv).bfloat16().cuda()
+  k = (0.25 * normal(gen, (n, kv_heads, d), torch.float32)).bfloat16().cuda().requires_grad_(True)
+  v = (1.0 - 2.0 * (torch.arange(n) % 2))[:, None, None].expand(n, kv_heads, dv).bfloat16().cuda().requires_grad_(True)
+  out = Fn.packed_attention(q, k, v, plan)
+  dq, dk, dvalue = torch.autograd.grad(out, (q, k, v), dout)
+  want = exact_attention(q.detach(), k.detach(), v.detach(), dout, [(0, rows, 0, n)], heads, kv_heads, False,
+                         1 / math.sqrt(d))
+  for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dvalue)):
+    within(got, want[name][0], want[name][1], name)
+  for name in ("dk", "dv"):
+    assert float(want[name][1].norm() / want[name][0].norm()) < 5 * HB, name
+
+
+@pytest.mark.parametrize("k_lengths,rows,heads,kv_heads,d,dv", [
+    ([131072], 1, 2, 2, 128, 8), ([70000], 1, 32, 1, 64, 128),        # groups of threads share a row's parts
+    ([4096] * 50, 1, 32, 8, 16, 64),                                  # many joins: a thread a piece of a row
+    ([5000], 70, 2, 1, 64, 64), ([3000, 2500], 300, 1, 1, 128, 96)])  # tiles
+def test_statistics_of_joined_rows(K, k_lengths, rows, heads, kv_heads, d, dv):
+  """lse against the logarithm of the sum in 64 bits: a score is off by D HF sum |q k| scale, the sum is one of at most 512
+  + parts fp32 additions in a row, the logarithm and its two products round the result three times."""
+  gen = torch.Generator().manual_seed(rows + heads)
+  count = len(k_lengths)
+  plan = K.AttentionPlan([rows] * count, k_lengths, heads=heads, kv_heads=kv_heads)
+  assert plan.info.joins > 0
+  q = normal(gen, (rows * count, heads, d))
+  k, v = normal(gen, (sum(k_lengths), kv_heads, d)), normal(gen, (sum(k_lengths), kv_heads, dv))
+  _, (lse, _) = K.packed_attention_fwd(q.cuda(), k.cuda(), v.cuda(), plan)
+  lse = lse.double().cpu()
+  at = 0
+  for i, n in enumerate(k_lengths):
+    for h in range(heads):
+      a, b = q[i * rows:(i + 1) * rows, h].double(), k[at:at + n, h * kv_heads // heads].double()
+      s = a @ b.t() / math.sqrt(d)
+      want = torch.logsumexp(s, -1)
+      tol = d * HF * float((a.abs() @ b.abs().t()).max()) / math.sqrt(d) + (512 + plan.info.parts) * HF + 3 * HF * want.abs()
+      got = lse[i * rows:(i + 1) * rows, h]
+      assert ((got - want).abs() <= tol + 2.0 ** -20).all(), (i, h)
+    at += n
+
+
+# ------------------------------------------------------------------------------------------------
+# gain gradients over more blocks of tokens than workgroups
+# ------------------------------------------------------------------------------------------------
+MANY_TOKENS = [
+    # like QK: 16 tokens a block of 256 turned entries, 1032 blocks of them for at most 1024 workgroups, the last one short
+    (16507, 1, 1, 256, 256, "half", 1, torch.bfloat16, False, True),
+    (16507, 2, 1, 256, 254, "interleaved", 1, torch.float32, True, True),
+    (33003, 1, 1, 128, 128, "half", 2, torch.bfloat16, False, True),
+]
+
+
+@pytest.mark.parametrize("case", MANY_TOKENS, ids=[str(i) for i in range(len(MANY_TOKENS))])
+def test_qk_norm_rotary_of_many_tokens(K, Fn, case):
+  test_qk_norm_rotary(K, Fn, case)
