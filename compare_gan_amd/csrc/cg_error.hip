@@ -14,7 +14,7 @@ void cg_set_error(const char* fmt, ...) {
   va_end(ap);
 }
 
-extern "C" int cg_abi_version(void) { return 8; }   // 8: + packed attention, rotary positions; 7: + cg_sum4, cg_gconv_ld (round 5: cgDeferCtx replaces cg_reduce_defer_*)
+extern "C" int cg_abi_version(void) { return 8; }   // 8: + packed attention, rotary positions; 7: + cg_sum4, cg_gconv_ld; cgDeferCtx replaces cg_reduce_defer_*
 extern "C" const char* cg_last_error(void) { return g_err; }
 
 // ---- optional per-kernel-family timing with HIP events (bench.py's roofline leg) -------------

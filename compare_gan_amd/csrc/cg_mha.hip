@@ -24,12 +24,14 @@
 // b128 reads of K (32 rows, one chunk) and the transposed reads of V (8 rows, 4 chunks) spread over all banks.
 // Rows behind the end of a sequence and columns behind D are outside the buffer descriptor and arrive as zeros.
 //
-// WHAT BOUNDS IT.  A 32 x 32 tile of scores at 64 wide heads is 8 matrix instructions of 32 cycles forward beside 16
-// exponentials and some 50 other vector instructions: both units of a SIMD are busy, and the chip lowers its clock
-// under it (1.84 to 1.9 of 2.4 GHz; on inputs of zeros the same code is 25 to 35 % faster).  A product of two 8192 x 8192
-// matrices reaches 1.45 to 1.48 PFLOP/s here.  Without effect or slower, each measured: the next tile's scores in front
-// of the softmax, fragments read ahead, alternating chains of matrix instructions, wave priorities, one workgroup more
-// or less a CU, 64 rows a wave (D = 64: 348 us in place of 327).
+// WHAT BOUNDS IT.  Forward at 64 wide heads the vector unit: a 32 x 32 tile of scores is 8 matrix instructions of 32 cycles
+// beside 16 exponentials at a quarter of the rate and some 60 other vector instructions.  Counted over 64 x 4096 tokens,
+// vector instructions are issued in 70 % of a SIMD's cycles and its matrix unit is busy in 45 %, at 1.76 of 2.4 GHz (on
+// inputs of zeros the same code is 25 to 35 % faster: the clock follows the power).  Backward 65 and 58 % (dQ), 55 and
+// 53 % (dK, dV); 128 wide forward 44 and 51 %.  A product of two 8192 x 8192 matrices reaches 1.38 to 1.48 PFLOP/s here.
+// Without effect or slower, each measured: the next tile's scores in front of the softmax, fragments read ahead,
+// alternating chains of matrix instructions, wave priorities, one workgroup more or less a CU, 64 rows a wave (D = 64:
+// 348 us in place of 327).
 #include "cg_common.h"
 
 #include <algorithm>
@@ -377,9 +379,9 @@ __device__ __forceinline__ void mha_store(const MhaArgs& a, const MhaItem& it, i
 }
 
 // ---- forward, 128 rows x all keys of the item ---------------------------------------------------
-// Measured: 64 x 4096 tokens, 3 heads of 64, 950 us (870 TFLOP/s); 16 384 tokens causal, 16 heads of 128 on 4 key heads,
-// 1.05 ms (1.05 PFLOP/s counted without the masked half); ragged causal batch, 8 heads of 96 on 2, 170 to 190 us (620 to 690 TFLOP/s:
-// diagonals and the end of the launch).
+// Measured: 64 x 4096 tokens, 3 heads of 64, 920 to 1020 us (810 to 900 TFLOP/s); 16 384 tokens causal, 16 heads of 128
+// on 4 key heads, 1.07 to 1.18 ms (0.93 to 1.03 PFLOP/s counted without the masked half); ragged causal batch, 8 heads of
+// 96 on 2, 165 to 190 us (620 to 710 TFLOP/s: diagonals and the end of the launch).
 template <int DK, int DV, bool GRAD>
 __global__ __launch_bounds__(256, mha_wider(DK, DV) <= 64 ? 4 : mha_wider(DK, DV) <= 96 ? 3 : 2) void mha_fwd_kernel(MhaArgs a) {
   constexpr int TK = KT * DK * 2, TILES = TK + KT * DV * 2;      // K, and K with V
@@ -462,8 +464,8 @@ __global__ __launch_bounds__(256, mha_wider(DK, DV) <= 64 ? 4 : mha_wider(DK, DV
 // ---- forward, at most 32 rows: the keys split over the waves --------------------------------------
 // One wave holds all rows; each of the NW waves takes every NW-th step of 32 keys through an LDS ring of its
 // own (no barrier in the loop), and the waves' results are joined at the end.  Bound by reading K and V: 48 new tokens,
-// 32 heads of 128 on 8, against up to 8192 keys each, 795 MB in 155 us (5.1 TB/s; a copy of 256 MiB reaches 5.4); of a
-// sequence with few keys (NW = 1, one wave an item), 256 x 16 tokens, 8 heads of 64: 7.5 us, what launching 2048 waves
+// 32 heads of 128 on 8, against up to 8192 keys each, 795 MB in 155 to 160 us (5.0 to 5.1 TB/s; a copy of 256 MiB reaches 5.4);
+// of a sequence with few keys (NW = 1, one wave an item), 256 x 16 tokens, 8 heads of 64: 7 to 8 us, what launching 2048 waves
 // and one trip to memory and back take.
 template <int DK, int DV, int NW, bool GRAD>
 __global__ __launch_bounds__(NW * 64) void mha_thin_kernel(MhaArgs a) {
@@ -663,9 +665,9 @@ __device__ __forceinline__ float mha_lse2(float lse) { return lse == -INFINITY ?
 // rows is formed on the way in (dO is in registers for dP) and left for the dK / dV kernel behind it.  dS = P (dP - delta)
 // is a difference: with the rounded out alone its error would come on top of the rounding of dS (dQ 1.5 instead of 1.4
 // roundings off).
-// Measured: 64 x 4096 tokens, 3 heads of 64, 1.15 ms (1.08 PFLOP/s over its three products), delta included (59 us as a
-// kernel of its own).  Three workgroups a CU at 96 wide heads (2 to 4 spills, outside the loop's products): 8 x 4096 tokens,
-// 8 heads, backward 1391 -> 1373 us; ragged training batch 769 -> 758 us.
+// Measured: 64 x 4096 tokens, 3 heads of 64, 1.19 to 1.24 ms (1.0 to 1.04 PFLOP/s over its three products), delta included
+// (59 us as a kernel of its own).  Three workgroups a CU at 96 wide heads (2 to 4 spills, outside the loop's products):
+// 8 x 4096 tokens, 8 heads, backward 1391 -> 1373 us; ragged training batch 769 -> 758 us.
 template <int DK, int DV>
 __global__ __launch_bounds__(256, mha_wider(DK, DV) <= 64 ? 4 : mha_wider(DK, DV) <= 96 ? 3 : 2) void mha_bwd_q_kernel(MhaArgs a) {
   constexpr int TK = KT * DK * 2, TILES = TK + KT * DV * 2;      // K, and K with V
@@ -778,8 +780,8 @@ __global__ __launch_bounds__(256, mha_wider(DK, DV) <= 64 ? 4 : mha_wider(DK, DV
 // columns; dV^T += dO^T P, dK^T += Q^T dS.  Item {seq, hk, key0, first row, end row}.
 // At 128 wide heads the accumulators, K and V of a wave would be 192 registers and the rest spills (each reload also
 // waits for the copies in flight): V is read from LDS there, and the tiles are 32 rows so that two workgroups fit a CU.
-// Measured: 64 x 4096 tokens, 3 heads of 64, 1.63 ms (1.01 PFLOP/s over its four products); ragged causal batch, 8 heads
-// of 96 / 64 on 2: 290 to 330 us.
+// Measured: 64 x 4096 tokens, 3 heads of 64, 1.62 to 1.84 ms (0.90 to 1.02 PFLOP/s over its four products); ragged causal
+// batch, 8 heads of 96 / 64 on 2: 285 to 330 us.
 template <int DK, int DV>
 __global__ __launch_bounds__(256, mha_wider(DK, DV) <= 64 ? 3 : 2) void mha_bwd_kv_kernel(MhaArgs a) {
   constexpr bool V_LDS = DK + DV > 224;
@@ -988,7 +990,7 @@ __global__ __launch_bounds__(256) void mha_join_grad_kernel(MhaArgs a) {
 // All gradients of a sequence with at most 32 rows and 32 keys: one wave a key head, nothing but its own Q, K, V
 // and dO read.  The scores are formed both ways round (S^T for dQ, S for dK and dV); the softmax statistics and
 // delta = sum_k P dP come from the scores themselves, exact in fp32, and reach the other orientation by lane
-// exchanges.  Bound by latency: a launch of one wave workgroups, many a CU; 256 x 16 tokens, 8 heads of 64: 11.5 us (of
+// exchanges.  Bound by latency: a launch of one wave workgroups, many a CU; 256 x 16 tokens, 8 heads of 64: 11 us (of
 // which the bytes are 6).
 template <int DK, int DV>
 __global__ __launch_bounds__(64) void mha_bwd_small_kernel(MhaArgs a) {

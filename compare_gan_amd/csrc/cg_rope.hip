@@ -17,11 +17,14 @@
 // alignment allow it.  The head's sum of squares is a butterfly over the group.
 //
 // Measured (a copy of 1 GiB: 5.0 TB/s read and written; of 128 MiB, which stays in the last-level cache, 7.1):
-//   rotation, 262 144 tokens x 3 heads of 64, bf16, 201 MB:   45 us between other work, 32 us behind itself (6.2 TB/s)
+//   rotation, 262 144 tokens x 3 heads of 64, bf16, 201 MB:   42 us between other work, 33 us behind itself (6.1 TB/s)
 //   rotation, fp32, 30 011 tokens x 5 heads of 80, 96 MB:     19 us (5 TB/s)
-//   norm + rotation, 65 536 x (32 + 8) heads of 128, 1.34 GB: 256 to 280 us (4.8 to 5.2 TB/s)
-//   its forward / backward, 65 536 x (6 + 6) heads of 32:     21 / 34 us (101 / 151 MB), gains behind it 6 us
-// A call of a few tokens is 4 to 6 us, what a launch and one trip to memory take.
+//   norm + rotation, 65 536 x (32 + 8) heads of 128, 1.34 GB: 254 to 280 us (4.8 to 5.3 TB/s)
+//   its forward / backward, 65 536 x (6 + 6) heads of 32:     20 / 33 us (101 / 151 MB), gains behind it 6 us
+//   forward / backward, 65 536 x (8 + 2) heads of 128, fp32:  142 / 217 us (671 MB / 1.0 GB, 4.7 / 4.6 TB/s)
+// A call of a few tokens is 3 to 6 us, what a launch and one trip to memory take.  A row's lanes are a power of two:
+// 72 wide heads leave 7 of 16 lanes without data (30 011 x (8 + 4) heads: 34 / 57 us, 3.1 / 2.7 TB/s; 64 wide ones 19 /
+// 37 us, 4.8 / 3.8 TB/s).
 #include "cg_common.h"
 
 namespace {

@@ -1085,7 +1085,11 @@ class PackedAttentionFn(torch.autograd.Function):
 def packed_attention(q, k, v, plan, scale=None):
   """softmax(scale q k^T) v over the sequences of a K.AttentionPlan (q [rows, heads, D], k [rows, kv_heads, D],
   v [rows, kv_heads, Dv], bf16); differentiable in q, k and v.  Rows outside every sequence give zeros and
-  get zero gradients.  First derivatives only."""
+  get zero gradients.  First derivatives only.
+  bf16 alone, as the networks are: weights and their gradients enter the matrix instructions in bf16, and 32-bit operands
+  would be rounded to it first.  The last bit of out may depend on whether a gradient is wanted: then rows that see at most
+  64 keys also add what the rounding of their weights left over, which delta = dout . out would carry into all of dS.
+  Where a causal mask cuts through a tile, a key or value entry that is not finite makes NaN of all of a row that sees it."""
   return PackedAttentionFn.apply(q, k, v, plan, scale)
 
 

@@ -1359,10 +1359,13 @@ class AttentionPlan(object):
     q_starts / k_starts   : first row of every sequence (None: one behind the other); sequences must not
                             overlap.  Rows between them belong to nobody -- a padded batch or a cache with
                             room is [sequences * capacity, heads, D] with starts at multiples of capacity.
-    heads, kv_heads       : query head h reads key head h // (heads / kv_heads).
+    heads, kv_heads       : query head h reads key head h // (heads / kv_heads); at most 4096 heads.
     causal                : row i of a sequence sees its keys 0 .. i + k_length - q_length (the last row
                             sees all of them; rows in front of the first key see none and give 0).
-    A plan holds for any stream.  A captured graph reads it on every replay: keep it as long as the graph."""
+    A plan holds for any stream.  A captured graph reads it on every replay: keep it as long as the graph.
+    It is made for these lengths, forward and backward, with an upload that is waited for: a few hundred microseconds of
+    the host for tens of sequences (48 new tokens against up to 8192 keys, 32 heads over 8: 460 us, 500 KB), again for
+    every step that lengthens a key sequence.  Calls of the same lengths share one (all layers of a network, say)."""
 
     def __init__(self, q_lengths, k_lengths=None, heads=1, kv_heads=None, causal=False, q_starts=None,
                  k_starts=None, device="cuda"):
