@@ -1210,10 +1210,11 @@ def _req_heads(t, name, like=None):
     """[T, heads, D] with the D entries of a head contiguous (other strides free)."""
     if not torch.is_tensor(t) or not t.is_cuda:
         raise ValueError("%s must be a tensor on the GPU (no CPU fallback exists)" % name)
-    if t.dim() != 3:
-        raise ValueError("%s must be [rows, heads, width], got %d dimensions" % (name, t.dim()))
-    if t.shape[0] > MOST_ROWS or t.shape[1] > MOST_HEADS:      # (ctypes would wrap what is more than 32 bits)
-        raise ValueError("%s: at most %d rows and %d heads, got %s" % (name, MOST_ROWS, MOST_HEADS, list(t.shape)))
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError("%s must be [rows, heads, width], got %d dimensions" % (name, len(shape)))
+    if shape[0] > MOST_ROWS or shape[1] > MOST_HEADS:      # (ctypes would wrap what is more than 32 bits)
+        raise ValueError("%s: at most %d rows and %d heads, got %s" % (name, MOST_ROWS, MOST_HEADS, list(shape)))
     if like is not None:
         if t.get_device() != like.get_device():
             raise ValueError("%s is on %s, the other tensors on %s" % (name, t.device, like.device))
