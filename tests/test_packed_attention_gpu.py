@@ -854,7 +854,7 @@ def test_plan_and_table_dropped_while_another_stream_reads_them(K, Fn):
   table, plan = make()
   places = {table.freq.data_ptr(): table.freq.numel() * 8, plan.data.data_ptr(): plan.data.numel() * 4}
   with torch.cuda.stream(side):
-    for _ in range(400):             # some tens of milliseconds in front of the call
+    for _ in range(1500):            # a tenth of a second and more in front of the call
       torch.matmul(busy, busy)
     got = call(table, plan)
     done = torch.cuda.Event()
